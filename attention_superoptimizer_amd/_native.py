@@ -45,6 +45,13 @@ class Mi355LaunchInfo(ctypes.Structure):
                 ("row_split", ctypes.c_int)]
 
 
+class Mi355PagedCache(ctypes.Structure):
+    """mi355_paged_cache (include/mi355_abi.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("pages", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("page_stride", ctypes.c_longlong),
+                ("token_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong), ("type", ctypes.c_int)]
+
+
 class MirageCPlan(ctypes.Structure):
     """struct mirage_c_plan (csrc/host/c_api.cc)."""
     _fields_ = [
@@ -73,6 +80,7 @@ _pf = ctypes.POINTER(ctypes.c_float)
 _pll = ctypes.POINTER(ctypes.c_longlong)
 _pplan = ctypes.POINTER(Mi355Plan)
 _pvp = ctypes.POINTER(ctypes.c_void_p)
+_ll = ctypes.c_longlong
 ABI = {
     "mi355_init": (_ci, [_sz, _pvp]),
     "mi355_shutdown": (_ci, []),
@@ -135,6 +143,11 @@ ABI = {
     "mi355_f16_unary": (_ci, [_ci, _vp, _vp, _sz]),
     "mi355_f16_binary": (_ci, [_ci, _vp, _pi, _vp, _pi, _vp, _pi, _ci]),
     "mi355_f16_reduce": (_ci, [_vp, _vp, _sz, _ci, _ci, _ci]),
+    "mi355_rotary": (_ci, [_vp, _ll, _vp, _ll, _vp, _vp] + [_ci] * 6),
+    "mi355_rotary_append": (_ci, [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _vp, ctypes.POINTER(Mi355PagedCache)] + [_ci] * 4),
+    "mi355_paged_attention": (_ci, [_vp, _ll, _vp, _ll, ctypes.POINTER(Mi355PagedCache), _vp, _ci, _vp, _ci, _ci, _ci,
+                                    ctypes.c_float, _ci]),
+    "mi355_verify_drafts": (_ci, [_vp] * 6 + [_ci] * 4),
     "mi355_emit_hip_preamble": (ctypes.c_char_p, []),
     "mi355_emit_hip_kernel": (ctypes.c_longlong, [_pplan, ctypes.c_char_p, _ci, ctypes.c_char_p,
                                                   ctypes.c_longlong]),
@@ -163,6 +176,10 @@ FACADE = {
     "mirage_graph_binary": (_vp, [_vp, _ci, _vp, _vp]),
     "mirage_graph_reduction": (_vp, [_vp, _vp, _ci, _ci]),
     "mirage_graph_customized": (_ci, [_vp, _pvp, _ci, ctypes.POINTER(MirageCPlan), _pvp, _ci]),
+    "mirage_graph_rotary": (_vp, [_vp] * 4 + [_ci]),
+    "mirage_graph_rotary_append": (_vp, [_vp] * 7 + [_ci] * 2),
+    "mirage_graph_paged_attention": (_vp, [_vp] * 6 + [ctypes.c_float, _ci, _ci]),
+    "mirage_graph_verify_drafts": (_ci, [_vp] * 5 + [_pvp]),
     "mirage_graph_pop_operator": (_ci, [_vp]),
     "mirage_op_type": (_ci, [_vp, _ci]),
     "mirage_op_num_outputs": (_ci, [_vp, _ci]),

@@ -151,6 +151,8 @@ int vendor_gemm_release();
 // mi355_customized_fp_static (tb_interp.hip); called by mi355_init with `device` current.
 int static_scratch_setup(int device);
 int fail(int code, char const *fmt, ...);
+// whether the description of a paged key-value cache holds together (paged_attention.hip)
+int check_paged_cache(mi355_paged_cache const &cache);
 
 #define MI355_HIP(expr)                                                             \
   do {                                                                              \

@@ -31,6 +31,7 @@ size_t get_datatype_size(DataType type) {
     case DT_FLOAT16:
       return 2;
     case DT_FLOAT32:
+    case DT_INT32:
       return 4;
     case DT_DOUBLE:
       return 8;
@@ -52,6 +53,10 @@ char const *to_string(KNOperatorType t) {
     case KN_MUL_OP: return "kn_mul_op";
     case KN_DIV_OP: return "kn_div_op";
     case KN_SILU_OP: return "kn_silu_op";
+    case KN_ROTARY_OP: return "kn_rotary_op";
+    case KN_ROTARY_APPEND_OP: return "kn_rotary_append_op";
+    case KN_PAGED_ATTENTION_OP: return "kn_paged_attention_op";
+    case KN_VERIFY_DRAFTS_OP: return "kn_verify_drafts_op";
     case KN_CUSTOMIZED_OP: return "kn_customized_op";
     default: return "kn_unkown";
   }

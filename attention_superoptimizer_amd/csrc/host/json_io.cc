@@ -442,6 +442,10 @@ EnumName const kKnOps[] = {
     {KN_MUL_OP, "kn_mul_op"},
     {KN_DIV_OP, "kn_div_op"},
     {KN_SILU_OP, "kn_silu_op"},  // extension
+    {KN_ROTARY_OP, "kn_rotary_op"},  // extensions: decoding.h
+    {KN_ROTARY_APPEND_OP, "kn_rotary_append_op"},
+    {KN_PAGED_ATTENTION_OP, "kn_paged_attention_op"},
+    {KN_VERIFY_DRAFTS_OP, "kn_verify_drafts_op"},
     {KN_CUSTOMIZED_OP, "kn_customized_op"},
 };
 // reference include/mirage/type.h:105-129
@@ -585,6 +589,17 @@ void to_json(json &j, KNOperator const &op) {
     mirage::threadblock::to_json(p, c.plan);
     j["bgraph"] = b;
     j["plan"] = p;
+  } else if (op.op_type == KN_ROTARY_OP) {
+    j["interleaved"] = static_cast<KNRotaryOp const &>(op).interleaved;
+  } else if (op.op_type == KN_ROTARY_APPEND_OP) {
+    auto const &r = static_cast<KNRotaryAppendOp const &>(op);
+    j["interleaved"] = r.interleaved;
+    j["heads_first"] = r.heads_first;
+  } else if (op.op_type == KN_PAGED_ATTENTION_OP) {
+    auto const &a = static_cast<KNPagedAttentionOp const &>(op);
+    j["scale"] = (double)a.scale;
+    j["window"] = a.window;
+    j["heads_first"] = a.heads_first;
   }
 }
 
@@ -688,6 +703,32 @@ void from_json(json const &j, Graph &g) {
                   (SmemLayout)enum_from_json(kSmem, jb.at("output_tensors").at(k).at("layout"));
             }
           }
+        }
+        break;
+      }
+      case KN_ROTARY_OP:
+      case KN_ROTARY_APPEND_OP:
+      case KN_PAGED_ATTENTION_OP:
+      case KN_VERIFY_DRAFTS_OP: {
+        json const &ins = jop.at("input_tensors");
+        auto in = [&](size_t i) -> DTensor const & { return tensor_of(ins.at(i)); };
+        KNOperator *op = nullptr;
+        if (op_type == KN_ROTARY_OP) {
+          op = g.create_rotary_op(in(0), in(1), in(2), jop.at("interleaved").as_bool());
+        } else if (op_type == KN_ROTARY_APPEND_OP) {
+          op = g.create_rotary_append_op(in(0), in(1), in(2), in(3), in(4), in(5), jop.at("interleaved").as_bool(),
+                                         jop.at("heads_first").as_bool());
+        } else if (op_type == KN_PAGED_ATTENTION_OP) {
+          op = g.create_paged_attention_op(in(0), in(1), in(2), in(3), in(4), (float)jop.at("scale").as_double(),
+                                           (int)jop.at("window").as_int(), jop.at("heads_first").as_bool());
+        } else {
+          bool const certain = ins.size() == 3;
+          op = g.create_verify_drafts_op(in(0), certain ? nullptr : &in(1), in(certain ? 1 : 2), in(certain ? 2 : 3));
+        }
+        json_require(op != nullptr, "json: a decoding operator's tensors do not agree");
+        g.operators.push_back(op);
+        for (size_t i = 0; i < op->output_tensors.size(); i++) {
+          bind(jop, i, op->output_tensors[i]);
         }
         break;
       }

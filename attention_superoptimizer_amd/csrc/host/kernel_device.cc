@@ -44,7 +44,10 @@ bool DTensor::has_same_fingerprint(DTensor const &ref) const {
 bool KNInputOp::profile(ProfileResult &profile) {
   require_device("KNInputOp::profile");
   DTensor const &t = output_tensors[0];
-  MIRAGE_CHECK(t.data_type == DT_FLOAT16, "only fp16 inputs are supported");
+  if (t.data_type != DT_FLOAT16) {  // (page tables, positions, probabilities: they keep what the caller wrote)
+    profile.run_time = 0.0f;
+    return true;
+  }
   MI355_CALL(mi355_f16_fill_iota(t.data_ptr, t.num_elements(), t.dim[t.num_dims - 1]));
   MI355_CALL(mi355_sync());
   profile.run_time = 0.0f;
@@ -618,6 +621,12 @@ void execute_once(KNOperator *op) {
     }
     case KN_CUSTOMIZED_OP:
       static_cast<KNCustomizedOp *>(op)->run();
+      break;
+    case KN_ROTARY_OP:
+    case KN_ROTARY_APPEND_OP:
+    case KN_PAGED_ATTENTION_OP:
+    case KN_VERIFY_DRAFTS_OP:
+      static_cast<KNDecodingOp *>(op)->run();
       break;
     default:
       MIRAGE_CHECK(false, "operator cannot be executed");

@@ -713,8 +713,30 @@ static void export_stats(mirage::search::VerifyStats const &s, mirage_verify_sta
   }
 }
 
+// Whether every operator of the graph has a fingerprint (decoding.h: some have none).  The calls below refuse one
+// that has not: its verdict would be about values nobody computed.
+static bool has_fingerprints(void const *graph) {
+  for (mirage::kernel::KNOperator const *op : static_cast<mirage::kernel::Graph const *>(graph)->operators) {
+    if (mirage::kernel::is_decoding_op(op->op_type)) {
+      std::fprintf(stderr, "mirage: %s has no fingerprint\n", mirage::type::to_string(op->op_type));
+      return false;
+    }
+  }
+  return true;
+}
+static bool have_fingerprints(void *const *graphs, int n, void const *reference) {
+  bool all = has_fingerprints(reference);
+  for (int i = 0; i < n && all; i++) {
+    all = has_fingerprints(graphs[i]);
+  }
+  return all;
+}
+
 int mirage_graph_fingerprint(void *graph, unsigned long long input_seed,
                              mirage_verify_stats *stats) {
+  if (!has_fingerprints(graph)) {
+    return -1;
+  }
   mirage::search::VerifyStats s;
   mirage::search::fingerprint_graph(*static_cast<mirage::kernel::Graph *>(graph), input_seed, &s);
   export_stats(s, stats);
@@ -729,6 +751,9 @@ int mirage_graph_fingerprint(void *graph, unsigned long long input_seed,
 // their tensors stay alive until the matching mirage_verify_batch_end returns.
 void *mirage_verify_batch_begin(void *const *candidates, int n, void *reference,
                                 unsigned long long input_seed, int fingerprint_reference) {
+  if (!have_fingerprints(candidates, n, reference)) {
+    return nullptr;
+  }
   std::vector<mirage::kernel::Graph *> c(n);
   for (int i = 0; i < n; i++) {
     c[i] = static_cast<mirage::kernel::Graph *>(candidates[i]);
@@ -766,6 +791,9 @@ int mirage_verify_batch_end(void *ticket, int n, unsigned char *equal, mirage_ve
 int mirage_verify_batch(void *const *candidates, int n, void *reference,
                         unsigned long long input_seed, unsigned char *equal,
                         mirage_verify_stats *stats) {
+  if (!have_fingerprints(candidates, n, reference)) {
+    return -1;
+  }
   std::vector<mirage::kernel::Graph *> c(n);
   for (int i = 0; i < n; i++) {
     c[i] = static_cast<mirage::kernel::Graph *>(candidates[i]);

@@ -16,7 +16,7 @@ import numpy as np
 
 from . import _native as N
 
-DT_FLOAT16 = 921
+DT_BFLOAT16, DT_FLOAT16, DT_FLOAT32, DT_DOUBLE, DT_INT32 = 920, 921, 930, 940, 950
 DMEM_LAYOUT = {"DmemRowMajor": 100, "DmemColumnMajor": 101}
 SMEM_LAYOUT = {
     "SmemRowMajor": 200, "SmemColumnMajor": 201,
@@ -50,6 +50,34 @@ def set_smem_budget(nbytes: int) -> None:
 
 def device_ready() -> bool:
     return bool(N.runtime().mirage_device_ready())
+
+
+# what write_data takes and read_data gives where it is not fp16 (bf16: the values as fp32)
+_DATA_TYPE = {DT_BFLOAT16: np.float32, DT_FLOAT32: np.float32, DT_DOUBLE: np.float64, DT_INT32: np.int32}
+
+
+def _bf16_bits(a: np.ndarray) -> np.ndarray:
+    """fp32 values rounded to the nearest bf16, ties to even; a NaN stays one."""
+    bits = np.ascontiguousarray(a, np.float32).view(np.uint32)
+    rounded = (bits + (((bits >> 16) & 1) + np.uint32(0x7fff))) >> 16
+    return np.where((bits & 0x7fffffff) > 0x7f800000, (bits >> 16) | 0x40, rounded).astype(np.uint16)
+
+
+def rotary_angles(rotary_dim: int, base: float = 10000.0, factor: float = 1.0, original_length: Optional[int] = None,
+                  fast: float = 32.0, slow: float = 1.0, amplitude: float = 1.0) -> np.ndarray:
+    """The [2, rotary_dim / 2] doubles that `KNGraph.rotary` takes: pair i turns by base^(-2 i / rotary_dim) radians a
+    position, and every pair is scaled by `amplitude`.  For contexts `factor` times as long as a model was trained on:
+    without `original_length` every frequency is divided by `factor` (positions are interpolated); with it only those
+    that turn at most `slow` times over that length, the ones that turn `fast` times and more stay, and in between
+    the two are blended linearly in the number of turns."""
+    if rotary_dim < 2 or rotary_dim % 2 or base <= 0 or factor <= 0 or fast <= slow:
+        raise ValueError("rotary_angles: an even rotary_dim, base and factor above zero and fast > slow are wanted")
+    half = rotary_dim // 2
+    turn = float(base) ** (-np.arange(half, dtype=np.float64) / half)
+    kept = np.zeros(half)
+    if original_length is not None:
+        kept = np.clip((turn * original_length / (2.0 * np.pi) - slow) / (fast - slow), 0.0, 1.0)
+    return np.stack([turn * (kept + (1.0 - kept) / factor), np.full(half, float(amplitude))])
 
 
 class DTensor:
@@ -106,13 +134,14 @@ class DTensor:
         """Uploads the LOGICAL values `a` (shape = dims).  The fp16 buffer of a DmemColumnMajor
         tensor holds each [rows, cols] matrix column by column, as the reference's fp16 loader
         reads it (include/mirage/threadblock/cuda/input_loader.h:221-247); the fingerprint
-        buffer is row-major whatever the layout (input_loader.h:457-467)."""
-        a = np.asarray(a, dtype=np.float16)
+        buffer is row-major whatever the layout (input_loader.h:457-467).  They are rounded to the
+        tensor's type (to fp16 for the types that hold no values of their own here)."""
+        a = np.asarray(a, dtype=_DATA_TYPE.get(self.data_type, np.float16))
         assert a.size == self.num_elements
         a = a.reshape(self.dims)
         if self.column_major:
             a = a.swapaxes(-1, -2)
-        a = np.ascontiguousarray(a)
+        a = _bf16_bits(a) if self.data_type == DT_BFLOAT16 else np.ascontiguousarray(a)
         rc = N.runtime().mirage_tensor_write(self._h, 0, a.ctypes.data_as(ctypes.c_void_p), a.nbytes)
         assert rc == 0, N.last_error()
 
@@ -121,9 +150,11 @@ class DTensor:
         dims = list(self.dims)
         if self.column_major:
             dims[-1], dims[-2] = dims[-2], dims[-1]
-        a = np.empty(dims, np.float16)
+        a = np.empty(dims, np.uint16 if self.data_type == DT_BFLOAT16 else _DATA_TYPE.get(self.data_type, np.float16))
         rc = N.runtime().mirage_tensor_read(self._h, 0, a.ctypes.data_as(ctypes.c_void_p), a.nbytes)
         assert rc == 0, N.last_error()
+        if self.data_type == DT_BFLOAT16:
+            a = (a.astype(np.uint32) << 16).view(np.float32)
         return np.ascontiguousarray(a.swapaxes(-1, -2)) if self.column_major else a
 
     def has_same_fingerprint(self, other: "DTensor") -> bool:
@@ -247,6 +278,50 @@ class KNGraph:
         if n < 0:
             raise InfeasibleOperator("customized")
         return [DTensor(outs[i]) for i in range(n)]
+
+    # ---- operators of a decoding step on a paged key-value cache (include/mirage/kernel/decoding.h) -----------
+    def rotary(self, x: DTensor, positions: DTensor, angles: DTensor, interleaved: bool = False) -> DTensor:
+        """x [tokens, heads, head_dim] (fp16, bf16) with rotary positions: pair i of every head, (x[i], x[i + R/2]) or,
+        interleaved, (x[2i], x[2i + 1]), turned by positions[token] * angles[0][i] and scaled by angles[1][i].
+        positions [tokens] int32, angles [2, R/2] double (`rotary_angles`), R <= head_dim: the rest of a head stays."""
+        return self._wrap(self._rt.mirage_graph_rotary(self._g, x._h, positions._h, angles._h, int(interleaved)), "rotary")
+
+    def rotary_append(self, qkv: DTensor, positions: DTensor, angles: DTensor, slots: DTensor, k_cache: DTensor,
+                      v_cache: DTensor, interleaved: bool = False, heads_first: bool = False) -> DTensor:
+        """Queries, keys and values of one projection, qkv [tokens, q_heads + 2 kv_heads, head_dim] or [tokens, their
+        product]: returns the queries with rotary positions (as `rotary`), and WRITES the keys with theirs and the values
+        into the caches, [pages, page_size, kv_heads, head_dim] or (heads_first) [pages, kv_heads, page_size, head_dim],
+        at slots[token] = page * page_size + place.  A negative slot or one past the cache stores nothing.  The slots of
+        one call differ: of one that is named twice, any element may come from either token."""
+        return self._wrap(self._rt.mirage_graph_rotary_append(self._g, qkv._h, positions._h, angles._h, slots._h, k_cache._h,
+                                                              v_cache._h, int(interleaved), int(heads_first)), "rotary_append")
+
+    def paged_attention(self, q: DTensor, k_cache: DTensor, v_cache: DTensor, table: DTensor, lengths: DTensor,
+                        scale: Optional[float] = None, window: int = 0, heads_first: bool = False) -> DTensor:
+        """softmax(scale q K^T) V of the new tokens of every sequence over its pages.  q [sequences * new, q_heads,
+        head_dim] or [sequences * new, q_heads * head_dim], a sequence's tokens in a row; table [sequences, pages] and
+        lengths [sequences] int32, a length with the new tokens, whose keys are in the caches already.  New token t sees
+        the keys before length - (new - 1 - t), of these the last `window` if that is not 0; a row that sees none, or
+        only scores of minus infinity, is zeros.  Query head h reads key-value head h // (q_heads // kv_heads).  A page number outside the cache holds no
+        keys, a length past the table counts as the table's.  scale: 1 / sqrt(head_dim) if not given."""
+        if scale is None:
+            scale = float(k_cache.dims[-1]) ** -0.5
+        return self._wrap(self._rt.mirage_graph_paged_attention(self._g, q._h, k_cache._h, v_cache._h, table._h, lengths._h,
+                                                                scale, int(window), int(heads_first)), "paged_attention")
+
+    def verify_drafts(self, target: DTensor, draft: Optional[DTensor], tokens: DTensor, uniforms: DTensor):
+        """Which drafted tokens the target's probabilities keep, and the one after them: (accepted [sequences], tokens
+        [sequences, drafts + 1]), int32, -1 behind the last.  target [sequences, drafts + 1, vocabulary] and draft
+        [sequences, drafts, vocabulary] (or their first two dimensions as one), fp16, bf16 or fp32; draft None: the drafts
+        were certain; tokens [sequences, drafts] int32, a negative one ends a sequence's drafts; uniforms [sequences,
+        drafts + 1] fp32 in [0, 1).  Draft i is taken while uniforms[i] * draft[i][token] < target[i][token]; the last
+        uniform draws the next token from max(target - draft, 0) where one was refused, from target where none was left."""
+        outs = (ctypes.c_void_p * 2)()
+        rc = self._rt.mirage_graph_verify_drafts(self._g, target._h, None if draft is None else draft._h, tokens._h,
+                                                 uniforms._h, outs)
+        if rc != 0:
+            raise InfeasibleOperator("verify_drafts")
+        return DTensor(outs[0]), DTensor(outs[1])
 
     def pop_operator(self) -> None:
         assert self._rt.mirage_graph_pop_operator(self._g) == 0

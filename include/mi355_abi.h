@@ -434,6 +434,53 @@ int mi355_f16_binary(int op, void const *in1, int const *dims1, void const *in2,
 int mi355_f16_reduce(void const *in, void *out, size_t n_out, int factor, int in_stride,
                      int out_stride);
 
+/* ---- a decoding step on a paged key-value cache ----------------------------------
+ * No counterpart in the reference.  Values are fp16 or bf16 (`type`: 921, 920 of the reference's include/mirage/type.h),
+ * arithmetic is fp32 with one rounding per stored element, indices are 32-bit, strides count elements.  Sizes and
+ * pointers are checked (MI355_ERR_INVALID; MI355_ERR_UNSUPPORTED for what no kernel takes); what positions, slots,
+ * tables and lengths hold is the device's to read, and no value of theirs makes it leave the tensors. */
+#define MI355_TYPE_BF16 920
+#define MI355_TYPE_F16 921
+#define MI355_TYPE_F32 930
+/* Keys and values: element d of head h of the token at place t of page p is at p * page_stride + t * token_stride +
+ * h * head_stride + d. */
+typedef struct mi355_paged_cache {
+  void *k, *v;
+  int pages, page_size, kv_heads, head_dim;
+  long long page_stride, token_stride, head_stride;
+  int type;
+} mi355_paged_cache;
+/* y = x with rotary positions, `heads` heads of head_dim elements in a row for every token, tokens x_stride and
+ * y_stride apart: pair i < pairs of a head, elements (i, i + pairs) or, interleaved, (2i, 2i + 1), is turned by
+ * positions[token] * angles[i] radians (computed in 64 bits) and scaled by angles[pairs + i]; the rest is copied.  y may
+ * be x with the same stride. */
+int mi355_rotary(void const *x, long long x_stride, void *y, long long y_stride, int const *positions, double const *angles,
+                 int tokens, int heads, int head_dim, int pairs, int interleaved, int type);
+/* The same for q_heads heads of q (results in q_out) and the cache's kv_heads heads of k, which go into the cache at
+ * slots[token] = page * page_size + place, the values v beside them as they are.  A slot that is negative or past the
+ * cache stores nothing.  Slots of one call differ (of one named twice, any element may come from either token). */
+int mi355_rotary_append(void const *q, long long q_stride, void const *k, long long k_stride, void const *v, long long v_stride,
+                        void *q_out, long long out_stride, int const *positions, double const *angles, int const *slots,
+                        mi355_paged_cache const *cache, int tokens, int q_heads, int pairs, int interleaved);
+/* softmax(scale q K^T) V for new_tokens tokens in a row of each sequence (tokens q_stride and out_stride apart), over
+ * the pages table[sequence][0 .. table_width - 1] names: new token t sees the keys before L = lengths[sequence] -
+ * (new_tokens - 1 - t), of these the last `window` where that is not 0.  A row without keys, or with scores of minus infinity only, is zeros; a page number
+ * outside the cache holds no keys; a length past the table counts as the table's.  Head sizes are multiples of 8 up to
+ * MI355_MAX_PAGED_HEAD_DIM, q_heads one of kv_heads, strides multiples of 8, q, out, k and v 16-byte aligned. */
+#define MI355_MAX_PAGED_HEAD_DIM 256
+int mi355_paged_attention(void const *q, long long q_stride, void *out, long long out_stride, mi355_paged_cache const *cache,
+                          int const *table, int table_width, int const *lengths, int sequences, int new_tokens, int q_heads,
+                          float scale, int window);
+/* Which of `drafts` drafted tokens a sequence keeps: draft i while uniforms[i] * draft[i][token] < target[i][token]
+ * (draft null: the drafts were certain), up to a token outside the vocabulary.  accepted[sequence] counts them;
+ * out[sequence][0 .. drafts] holds them, then a token drawn by uniforms[drafts] -- the lowest index where the sum of
+ * weights passes that share of their total -- and -1 behind it.  The weights: target, less draft and not below zero
+ * (certain: without the token) where a draft was refused, unless that leaves nothing; without any weight the token is
+ * -1.  target [sequences][drafts + 1][vocabulary], draft [sequences][drafts][vocabulary], fp16, bf16 or fp32; sums and
+ * comparisons in 64 bits. */
+int mi355_verify_drafts(void const *target, void const *draft, int const *tokens, float const *uniforms, int *accepted, int *out,
+                        int sequences, int drafts, int vocabulary, int type);
+
 /* ---- timing -----------------------------------------------------------------
  * cudaEvent pairs of every profile() in the reference (e.g. matmul_kernel.cu:63-70). */
 int mi355_timer_start(void);

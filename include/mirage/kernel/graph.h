@@ -5,6 +5,7 @@
 #pragma once
 
 #include "mirage/kernel/customized.h"
+#include "mirage/kernel/decoding.h"
 #include "mirage/kernel/device_tensor.h"
 #include "mirage/kernel/operator.h"
 #include "mirage/threadblock/graph.h"
@@ -57,6 +58,22 @@ public:
                                   mirage::threadblock::Graph const &_graph);
   KNOperator *create_customized_op(std::vector<DTensor> const &inputs,
                                    mirage::threadblock::Graph const &_graph);
+
+  // Operators of a decoding step (decoding.h says what each computes and takes).  An infeasible one is nullptr
+  // from create_*, the others abort.
+  DTensor rotary(DTensor const &x, DTensor const &positions, DTensor const &angles, bool interleaved = false);
+  KNOperator *create_rotary_op(DTensor const &x, DTensor const &positions, DTensor const &angles, bool interleaved);
+  DTensor rotary_append(DTensor const &qkv, DTensor const &positions, DTensor const &angles, DTensor const &slots,
+                        DTensor const &k_cache, DTensor const &v_cache, bool interleaved = false, bool heads_first = false);
+  KNOperator *create_rotary_append_op(DTensor const &qkv, DTensor const &positions, DTensor const &angles, DTensor const &slots,
+                                      DTensor const &k_cache, DTensor const &v_cache, bool interleaved, bool heads_first);
+  DTensor paged_attention(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table,
+                          DTensor const &lengths, float scale, int window = 0, bool heads_first = false);
+  KNOperator *create_paged_attention_op(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table,
+                                        DTensor const &lengths, float scale, int window, bool heads_first);
+  std::vector<DTensor> verify_drafts(DTensor const &target, DTensor const *draft, DTensor const &tokens, DTensor const &uniforms);
+  KNOperator *create_verify_drafts_op(DTensor const &target, DTensor const *draft, DTensor const &tokens,
+                                      DTensor const &uniforms);
 
   // Writes a self-contained HIP program for gfx950: one specialised kernel per
   // customized operator, a launcher over all of them and a main() that fills the

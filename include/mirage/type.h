@@ -31,6 +31,7 @@ enum DataType {
   DT_FLOAT16 = 921,
   DT_FLOAT32 = 930,
   DT_DOUBLE = 940,
+  DT_INT32 = 950,  // extension of this backend (not in the reference): positions, page tables, tokens
   DT_UNKNOWN = 999,
 };
 
@@ -48,6 +49,11 @@ enum KNOperatorType {
   KN_MUL_OP = 1009,
   KN_DIV_OP = 1010,
   KN_SILU_OP = 1011,  // extension of this backend (not in the reference)
+  // operators of a decoding step on a paged key-value cache (decoding.h; extensions too)
+  KN_ROTARY_OP = 1012,
+  KN_ROTARY_APPEND_OP = 1013,
+  KN_PAGED_ATTENTION_OP = 1014,
+  KN_VERIFY_DRAFTS_OP = 1015,
   KN_CUSTOMIZED_OP = 1999,
 };
 
