@@ -112,6 +112,11 @@ struct State {
   // kTickets ints, zero whenever no launch that uses them runs.
   static constexpr int kTickets = 1 << 16;
   int *tickets = nullptr;
+  // Those of launches whose workgroups join parts of each other's results (paged_attention.hip): per queue three for each
+  // of the most workgroups such a launch has, zero whenever none runs.
+  static constexpr int kJoinWorkgroups = 1024;
+  int *join_tickets = nullptr;
+  int *queue_join_tickets() const { return join_tickets + 3 * kJoinWorkgroups * tls_queue; }
 };
 
 State &state();

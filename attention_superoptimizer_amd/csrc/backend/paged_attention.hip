@@ -2,10 +2,21 @@
 //
 // o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m), s_j = scale q . k_j, over the keys a row sees, in one pass with the
 // running maximum m: when it grows, what has been summed is scaled down.
+//
+// Every key and value is read once for all rows of its head (query heads of the group x new tokens), so the bytes of
+// the cache bound a long call and the chain of trips to memory a short one.  What follows from that:
+// * the work is cut into units of 128 keys of one sequence and key-value head, numbered through the batch, and dealt
+//   in equal runs to the workgroups that fit the chip: how long each sequence is makes no difference.  The parts of
+//   a head that several workgroups have are joined by the last of them (a ticket), in the order of the keys.
+// * a wavefront has 32 keys at a time and streams them from the pages straight into LDS of its own: no barrier in the
+//   loop.  The next keys are on their way while the scores become weights, the next values while the next scores are made.
+// * scores are made transposed, S^T = K Q^T: a lane then has the weights of one row, as the operand of O^T = V^T P^T
+//   wants them, and that row's maximum, sum and scale.
 #include "common.h"
 
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 namespace mi355 {
 
@@ -25,86 +36,643 @@ int check_paged_cache(mi355_paged_cache const &c) {
 
 namespace {
 
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kTile = 32;                 // keys of a wavefront at a time
+constexpr int kUnit = kTile * kWaves;     // and of a workgroup
+constexpr int kIds = 1024;                // page numbers of a run that a workgroup holds in LDS
+constexpr int kOneLevel = 8;              // parts that are joined at once; more of them in two levels
+
 struct PagedParams {
   void const *q, *k, *v;
   void *out;
-  long long q_stride, out_stride, page_stride, token_stride, head_stride;
+  long long q_stride, out_stride;
+  uint32_t page_step, token_step, head_step;  // in 16 bytes: a cache is up to 64 GB
   int const *table, *lengths;
-  int pages, page_size, kv_heads, head_dim, table_width, sequences, new_tokens, group, window;
-  float scale;
+  float *parts;   // 2 per workgroup: the end of a head that began before it, the beginning of one that goes on after it
+  int *tickets;   // 3 per workgroup, zero between launches
+  int pages, page_size, head_dim, table_width, sequences, new_tokens, group, window;
+  int row_blocks, heads;  // of 16 RG rows, of a key-value head; key-value heads x row blocks
+  unsigned page_magic;    // 2^32 / page_size, rounded up; 0 for 1
+  float scale;            // times log2 e: weights are powers of two
 };
 
-// One wavefront per row (new token, query head); 64 keys at a time, a key a lane for the scores, 64 columns at a time
-// for the values.
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 template <class T>
-__global__ __launch_bounds__(64) void paged_attention_kernel(PagedParams const P) {
-  __shared__ float q[MI355_MAX_PAGED_HEAD_DIM], weight[64];
-  __shared__ long long place[64];
-  int const row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, kv = head / P.group;
-  int const sequence = row / P.new_tokens, t = row % P.new_tokens, D = P.head_dim;
-  T const *const query = static_cast<T const *>(P.q) + row * P.q_stride + (long long)head * D;
-  for (int d = lane; d < D; d += 64) {
-    q[d] = static_cast<float>(query[d]) * P.scale;
+struct Vec {
+  typedef T x8 __attribute__((ext_vector_type(8)));
+  typedef T x4 __attribute__((ext_vector_type(4)));
+  static constexpr uint32_t exponent = sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7c00 : 0x7f80;  // all ones: no number
+};
+
+__device__ __forceinline__ floatx4 mfma(Vec<_Float16>::x8 a, Vec<_Float16>::x8 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx4 mfma(Vec<__bf16>::x8 a, Vec<__bf16>::x8 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// What a masked key and the columns past a head's end are loaded from.
+__device__ uintx4 const kZeros = {0, 0, 0, 0};
+
+// Every lane fetches 16 bytes from an address of its own; they land at `lds` + 16 * lane (vmcnt counts the transfer; the
+// caller waits).  Inline assembly because the compiler would have the next LDS read of any address wait for all of them.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void load_to_lds(uint64_t address, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(address)
+               : "m0", "memory");
+}
+#pragma clang diagnostic pop
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
+
+// Where 16-byte chunk `chunk` of row `row` of a tile lies in it, and what lies where.  The sixteen rows of a score
+// operand read the same chunk of K, the eight of half a transposing read the same pair of V: their places are turned by
+// the row so that they fall on different banks (64 of 4 bytes: sixteen chunks in a row).  C chunks a row.
+template <int C, bool VALUES>
+__device__ __forceinline__ int turn_of(int row) {
+  return VALUES ? (C == 8 ? 2 * ((row >> 1) & 3) : C == 12 ? 2 * ((row >> 2) & 1) : C == 24 ? 2 * ((row >> 1) & 3) : 2 * (row & 7))
+                : (C == 8 ? (row >> 1) & 7 : C == 12 ? (row >> 2) & 3 : C == 24 ? (row >> 1) & 7 : row & 15);
+}
+template <int C, bool VALUES>
+__device__ __forceinline__ int place_of(int row, int chunk) {
+  int const turn = turn_of<C, VALUES>(row);
+  if constexpr ((C & (C - 1)) == 0) {
+    return chunk ^ turn;
   }
-  __syncthreads();
-  int const most = P.table_width * P.page_size, told = P.lengths[sequence], length = told < 0 ? 0 : (told < most ? told : most);
-  int const end = length - (P.new_tokens - 1 - t), begin = P.window != 0 && end > P.window ? end - P.window : 0;
-  int const *const table = P.table + (long long)sequence * P.table_width;
-  float m = -INFINITY, sum = 0.0f, acc[MI355_MAX_PAGED_HEAD_DIM / 64] = {};
-  for (int base = begin; base < end; base += 64) {
-    int const key = base + lane;
-    int const page = key < end ? table[key / P.page_size] : -1;
-    bool const seen = page >= 0 && page < P.pages;
-    long long const at = seen ? page * P.page_stride + (long long)(key % P.page_size) * P.token_stride + kv * P.head_stride : 0;
-    float s = -INFINITY;
-    if (seen) {
-      s = 0.0f;
-      for (int d = 0; d < D; d++) {
-        s += q[d] * static_cast<float>(static_cast<T const *>(P.k)[at + d]);
+  int const at = chunk + turn;
+  return at >= C ? at - C : at;
+}
+template <int C, bool VALUES>
+__device__ __forceinline__ int chunk_at(int row, int place) {
+  int const turn = turn_of<C, VALUES>(row);
+  if constexpr ((C & (C - 1)) == 0) {
+    return place ^ turn;
+  }
+  int const chunk = place - turn;
+  return chunk < 0 ? chunk + C : chunk;
+}
+
+// x[l] op x[l ^ 16] op x[l ^ 32] op x[l ^ 48] in every lane: over the four groups of lanes that share a row
+template <class Op>
+__device__ __forceinline__ float over_groups(float x, Op op) {
+  x = op(x, __shfl_xor(x, 16, 64));
+  return op(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+struct Span {
+  int from, to;  // keys, from a multiple of kTile on
+  int units;     // at least one: a head without keys has its zeros to be written
+};
+__device__ __forceinline__ Span span_of(PagedParams const &P, int sequence) {
+  int const most = P.table_width * P.page_size, told = P.lengths[sequence];
+  int const length = told < 0 ? 0 : (told < most ? told : most);
+  int const first = P.window != 0 ? length - (P.new_tokens - 1) - P.window : 0;  // (no underflow: the host bounds both)
+  Span s;
+  s.from = first > 0 ? first & ~(kTile - 1) : 0;
+  s.to = length;
+  s.units = length > s.from ? (length - s.from + kUnit - 1) / kUnit : 1;
+  return s;
+}
+
+__device__ __forceinline__ int wave_sum(int x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    x += __shfl_xor(x, off, 64);
+  }
+  return x;
+}
+
+// Parts go through the memory that all XCDs share: device-scope stores and loads, which pass by this XCD's L2.
+__device__ __forceinline__ void store_shared(float *p, float a, float b) {
+  uint64_t const both = (uint64_t)__builtin_bit_cast(uint32_t, a) | (uint64_t)__builtin_bit_cast(uint32_t, b) << 32;
+  __hip_atomic_store((__attribute__((address_space(1))) uint64_t *)(uint64_t *)p, both, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void store_shared(float *p, floatx4 v) {
+  store_shared(p, v[0], v[1]);
+  store_shared(p + 2, v[2], v[3]);
+}
+__device__ __forceinline__ uint64_t load_shared(float const *p) {
+  return __hip_atomic_load((__attribute__((address_space(1))) uint64_t const *)(uint64_t const *)p, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float low_of(uint64_t x) { return __builtin_bit_cast(float, (uint32_t)x); }
+__device__ __forceinline__ float high_of(uint64_t x) { return __builtin_bit_cast(float, (uint32_t)(x >> 32)); }
+
+template <int DP, int RG>
+constexpr int part_floats() { return 16 * RG * (DP + 4); }  // rows of numerators, then each one's maximum and sum, twice
+template <int DP>
+constexpr int tile_bytes() { return kTile * DP * 2; }
+template <int DP, int RG>
+constexpr int query_bytes() { return RG > 1 ? 16 * RG * DP * 2 : 0; }
+// tiles; queries, where they are too many for registers; page numbers; maximum and sum of every wavefront's rows; whether
+// this workgroup is the last
+template <int DP, int RG>
+constexpr int lds_bytes() {
+  return kWaves * 2 * tile_bytes<DP>() + query_bytes<DP, RG>() + (int)sizeof(int) * kIds + kWaves * 16 * RG * 8 + 16;
+}
+
+// DP: the head size, rounded up; RG: groups of 16 rows.
+template <class T, int DP, int RG>
+__global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void paged_attention_kernel(PagedParams const P) {
+  constexpr int C = DP / 8, LOADS = kTile * C / 64, KK = DP / 32, DB = DP / 16;
+  typedef typename Vec<T>::x8 x8;
+  typedef typename Vec<T>::x4 x4;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  unsigned char *const queries = lds + kWaves * 2 * tile_bytes<DP>();
+  int *const ids = reinterpret_cast<int *>(queries + query_bytes<DP, RG>());
+  float *const stat = reinterpret_cast<float *>(ids + kIds);
+  int *const is_last = reinterpret_cast<int *>(stat + kWaves * 16 * RG * 2);
+  int const tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16, c = lane % 16;
+  unsigned char *const k_tile = lds + wave * 2 * tile_bytes<DP>(), *const v_tile = k_tile + tile_bytes<DP>();
+  uint32_t const k_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void const *)k_tile;
+  uint32_t const v_lds = k_lds + tile_bytes<DP>();
+
+  // this workgroup's run of units, and the sequence it begins in
+  int total = 0;
+  for (int b = lane; b < P.sequences; b += 64) {
+    total += span_of(P, b).units;
+  }
+  total = wave_sum(total) * P.heads;
+  int const run = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+  long long const begin = (long long)blockIdx.x * run;
+  if (begin >= total) {
+    return;
+  }
+  int unit = (int)begin;
+  int const end = total - unit < run ? total : unit + run;
+  int sequence = 0, before = 0;  // units of the sequences ahead of it
+  for (int base = 0;; base += 64) {
+    int const b = base + lane;
+    int upto = b < P.sequences ? span_of(P, b).units * P.heads : 0;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      int const other = __shfl_up(upto, off, 64);
+      upto += lane >= off ? other : 0;
+    }
+    uint64_t const past = __ballot(before + upto > unit);
+    if (past != 0) {
+      int const at = __builtin_ctzll(past);
+      sequence = base + at;
+      before += at > 0 ? __shfl(upto, at - 1, 64) : 0;
+      break;
+    }
+    before += __shfl(upto, 63, 64);
+  }
+  sequence = __builtin_amdgcn_readfirstlane(sequence);
+  before = __builtin_amdgcn_readfirstlane(before);
+
+  int const R = P.new_tokens * P.group;
+  while (unit < end) {
+    Span const span = span_of(P, sequence);
+    int const head = (unit - before) / span.units, first = (unit - before) % span.units;
+    int const units = span.units - first < end - unit ? span.units - first : end - unit;
+    int const kv = head / P.row_blocks, row0 = head % P.row_blocks * 16 * RG;
+    int const *const table = P.table + (long long)sequence * P.table_width;
+
+    // rows: lane's row c of every group, the new token t it belongs to, the keys it sees
+    auto query = [&](int row, int d) {  // eight elements of a row of the head, zeros past its end
+      uintx4 x = {0, 0, 0, 0};
+      if (row < R && d < P.head_dim) {
+        x = *reinterpret_cast<uintx4 const *>(static_cast<T const *>(P.q) + ((long long)sequence * P.new_tokens + row / P.group) * P.q_stride +
+                                              (long long)(kv * P.group + row % P.group) * P.head_dim + d);
+      }
+      return x;
+    };
+    uintx4 q[KK];  // of one group of rows
+    int limit[RG], least[RG];
+#pragma unroll
+    for (int r = 0; r < RG; r++) {
+      int const row = row0 + 16 * r + c;
+      limit[r] = row < R ? span.to - (P.new_tokens - 1 - row / P.group) : 0;
+      least[r] = row < R && P.window != 0 ? limit[r] - P.window : 0;
+    }
+    if constexpr (RG == 1) {
+#pragma unroll
+      for (int kk = 0; kk < KK; kk++) {
+        q[kk] = query(row0 + c, 32 * kk + 8 * g);
+      }
+    } else {
+      for (int i = tid; i < 16 * RG * C; i += kThreads) {
+        *reinterpret_cast<uintx4 *>(queries + i / C * (2 * DP) + 16 * place_of<C, false>(i / C, i % C)) = query(row0 + i / C, i % C * 8);
       }
     }
-    float top = s;
-    for (int off = 32; off > 0; off >>= 1) {
-      top = fmaxf(top, __shfl_xor(top, off, 64));
-    }
-    float const higher = fmaxf(m, top);
-    if (__all(!seen)) {
-      continue;
-    }
-    // (no score above minus infinity yet: nothing to scale, no weight)
-    float const scaled = m == -INFINITY ? 0.0f : expf(m - higher), w = seen && s != -INFINITY ? expf(s - higher) : 0.0f;
-    m = higher;
-    weight[lane] = w;
-    place[lane] = seen ? at : -1;
-    float total = w;
-    for (int off = 32; off > 0; off >>= 1) {
-      total += __shfl_xor(total, off, 64);
-    }
-    sum = sum * scaled + total;
-    __syncthreads();
+    // the keys that every row sees lie between these (rows of a block are in the order of their tokens)
+    int const last_row = row0 + 16 * RG < R ? row0 + 16 * RG - 1 : R - 1;
+    int const all_limit = span.to - (P.new_tokens - 1 - row0 / P.group);
+    int const all_least = P.window != 0 ? span.to - (P.new_tokens - 1 - last_row / P.group) - P.window : 0;
+
+    floatx4 acc[RG][DB];
+    float m[RG], sum[RG];
 #pragma unroll
-    for (int i = 0; i < MI355_MAX_PAGED_HEAD_DIM / 64; i++) {
-      int const d = 64 * i + lane;
-      if (d < D) {
-        float a = acc[i] * scaled;
-        for (int j = 0; j < 64; j++) {
-          if (place[j] >= 0) {
-            a += weight[j] * static_cast<float>(static_cast<T const *>(P.v)[place[j] + d]);
+    for (int r = 0; r < RG; r++) {
+      m[r] = -INFINITY;
+      sum[r] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DB; d++) {
+        acc[r][d] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+      }
+    }
+    uint64_t const k_base = reinterpret_cast<uint64_t>(P.k) + 16ull * kv * P.head_step, v_base = reinterpret_cast<uint64_t>(P.v) + 16ull * kv * P.head_step;
+
+    // as many units at a time as the page numbers in LDS cover
+    int const fit = P.page_size < 1 << 16 ? (kIds - 1) * P.page_size / kUnit : 1 << 18;
+    for (int part = 0; part < units; part += fit) {
+      int const part_units = units - part < fit ? units - part : fit;
+      int const key0 = span.from + (first + part) * kUnit, key1 = key0 + part_units * kUnit < span.to ? key0 + part_units * kUnit : span.to;
+      int const page0 = key0 / P.page_size, numbers = key1 > key0 ? (key1 - 1) / P.page_size + 1 - page0 : 0;
+      __syncthreads();  // (the numbers of the part before, or the tiles as room for sums, are read)
+      for (int i = tid; i < numbers; i += kThreads) {
+        ids[i] = table[page0 + i];
+      }
+      if constexpr (RG == 1) {
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {  // the queries are here: no wait for them inside the loop
+          asm volatile("" : "+v"(q[kk]));
+        }
+      }
+      __syncthreads();
+
+      // tiles of this wavefront: 32 keys of every unit
+      int const mine = key0 + wave * kTile;
+      int const tiles = mine < key1 ? (key1 - mine + kUnit - 1) / kUnit : 0;
+      uint32_t at[LOADS];     // where the rows begin that this lane loads chunks of, in 16 bytes; all ones: zeros
+      uint32_t there = 0;     // keys that exist, a bit each
+      auto locate = [&](int tile) {
+        int const key = mine + tile * kUnit + lane % kTile;
+        int page = P.page_magic == 0 ? key : (int)__umulhi((uint32_t)key, P.page_magic);
+        page -= page * P.page_size > key ? 1 : 0;  // (the rounded reciprocal is one too many at most)
+        int const number = key < key1 ? ids[page - page0] : -1;
+        bool const is = (unsigned)number < (unsigned)P.pages;
+        there = (uint32_t)__ballot(is);
+        uint32_t const step = is ? (uint32_t)number * P.page_step + (uint32_t)(key - page * P.page_size) * P.token_step : ~0u;
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+          at[i] = (uint32_t)__shfl((int)step, (64 * i + lane) / C, 64);
+        }
+      };
+      auto load = [&](uint64_t base, uint32_t to, auto values) {
+        int chunks = P.head_dim / 8;
+        asm volatile("" : "+s"(chunks));  // (otherwise a comparison for every load is kept through the loop)
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+          int const row = (64 * i + lane) / C, chunk = chunk_at<C, decltype(values)::value>(row, (64 * i + lane) % C);
+          bool const real = at[i] != ~0u && chunk < chunks;
+          load_to_lds(real ? base + 16ull * (at[i] + chunk) : reinterpret_cast<uint64_t>(&kZeros), to + 1024 * i);
+        }
+      };
+      using Keys = std::integral_constant<bool, false>;
+      using Values = std::integral_constant<bool, true>;
+
+      if (tiles > 0) {
+        locate(0);
+        load(k_base, k_lds, Keys{});
+        load(v_base, v_lds, Values{});
+      }
+      for (int tile = 0; tile < tiles; tile++) {
+        int const key = mine + tile * kUnit;
+        uint32_t const is_there = there;
+        bool const more = tile + 1 < tiles;
+        wait_loads<LOADS>();  // keys are here, values under way
+
+        // S^T: lane has keys 4g .. 4g + 3 and 16 + 4g .. of row c
+        floatx4 s[RG][2];
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+          s[r][0] = s[r][1] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            int const row = 16 * j + c;
+            x8 const k = *reinterpret_cast<x8 const *>(k_tile + row * (2 * DP) + 16 * place_of<C, false>(row, 4 * kk + g));
+#pragma unroll
+            for (int r = 0; r < RG; r++) {
+              if constexpr (RG == 1) {
+                s[r][j] = mfma(k, __builtin_bit_cast(x8, q[kk]), s[r][j]);
+              } else {
+                int const its = 16 * r + c;
+                s[r][j] = mfma(k, *reinterpret_cast<x8 const *>(queries + its * (2 * DP) + 16 * place_of<C, false>(its, 4 * kk + g)), s[r][j]);
+              }
+            }
           }
         }
-        acc[i] = a;
+        wait_lds_reads();
+        if (more) {
+          locate(tile + 1);
+          load(k_base, k_lds, Keys{});
+        }
+
+        // weights, times 2^15 so that fp16 keeps small ones: two numbers of the value's type each, of which the second is
+        // what rounding the first lost -- one alone would put as much error into the result as rounding that does
+        bool const whole = is_there == ~0u && key >= all_least && key + kTile <= all_limit;
+        x8 p[RG], rest[RG];
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            x[e] = s[r][e / 4][e % 4] * P.scale;
+          }
+          if (!whole) {
+            int const upto = limit[r] - key, from = least[r] - key;
+            uint32_t seen = is_there;
+            seen = upto <= 0 ? 0 : (upto < kTile ? seen & ((1u << upto) - 1) : seen);
+            seen = from <= 0 ? seen : (from < kTile ? seen & ~((1u << from) - 1) : 0);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              x[e] = (seen >> (16 * (e / 4) + 4 * g + e % 4)) & 1 ? x[e] : -INFINITY;
+            }
+          }
+          float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+          top = over_groups(top, [](float a, float b) { return fmaxf(a, b); });
+          if (__any(top > m[r])) {
+            float const higher = fmaxf(m[r], top), less = exp2_fast(m[r] - (higher == -INFINITY ? 0.0f : higher));
+            m[r] = higher;
+            sum[r] *= less;
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+              acc[r][d] *= less;
+            }
+          }
+          float const base = m[r] == -INFINITY ? 0.0f : m[r] - 15.0f;
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            float const w = exp2_fast(x[e] - base);
+            sum[r] += w;
+            p[r][e] = static_cast<T>(w);
+            rest[r][e] = static_cast<T>(w - static_cast<float>(p[r][e]));
+          }
+        }
+        if (more) {
+          wait_loads<LOADS>();  // values are here, the next keys under way
+        } else {
+          wait_loads<0>();
+        }
+
+        // Rows of a tile that see other keys than their neighbours: a weight of zero does not keep an infinity or NaN among
+        // the values out of a sum.  Such keys' values are added to the rows that do see them by themselves, and zero from
+        // then on.
+        if (!whole && P.new_tokens > 1) {
+          uint32_t wild = 0;  // keys with such values
+#pragma unroll
+          for (int i = 0; i < LOADS; i++) {
+            uintx4 const x = *reinterpret_cast<uintx4 const *>(v_tile + 16 * (64 * i + lane));
+            bool none = false;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+              constexpr uint32_t top = Vec<T>::exponent;
+              none = none || (x[w] & top) == top || (x[w] & top << 16) == top << 16;
+            }
+            wild |= none ? 1u << ((64 * i + lane) / C) : 0u;
+          }
+#pragma unroll
+          for (int off = 32; off > 0; off >>= 1) {
+            wild |= (uint32_t)__shfl_xor((int)wild, off, 64);
+          }
+          for (uint32_t left = __builtin_amdgcn_readfirstlane(wild); left != 0; left &= left - 1) {
+            int const j = __builtin_ctz(left), holder = 16 * (j % 16 / 4) + c, at_e = 4 * (j / 16) + j % 4;
+            float w[RG];
+            bool sees[RG];
+#pragma unroll
+            for (int r = 0; r < RG; r++) {
+              w[r] = 0.0f;
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                w[r] = e == at_e ? static_cast<float>(p[r][e]) + static_cast<float>(rest[r][e]) : w[r];
+              }
+              w[r] = __shfl(w[r], holder, 64);
+              sees[r] = key + j < limit[r] && key + j >= least[r];
+            }
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+              x4 const x = *reinterpret_cast<x4 const *>(v_tile + j * (2 * DP) + 16 * place_of<C, true>(j, 2 * d + g / 2) + 8 * (g % 2));
+#pragma unroll
+              for (int r = 0; r < RG; r++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                  acc[r][d][e] += sees[r] ? w[r] * static_cast<float>(x[e]) : 0.0f;
+                }
+              }
+            }
+            wait_lds_reads();
+            if (lane < C) {
+              *reinterpret_cast<uintx4 *>(v_tile + j * (2 * DP) + 16 * lane) = uintx4{0, 0, 0, 0};
+            }
+          }
+        }
+
+        // O^T: lane has columns 16 d + 4g .. + 3 of row c
+#pragma unroll
+        for (int d = 0; d < DB; d++) {
+          uintx2 v[2];
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            int const row = 16 * j + 4 * g + c / 4, chunk = 2 * d + c % 4 / 2;
+            typedef short shortx4 __attribute__((ext_vector_type(4)));
+            unsigned char const *const from = v_tile + row * (2 * DP) + 16 * place_of<C, true>(row, chunk) + 8 * (c % 2);
+            v[j] = __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                  (shortx4 __attribute__((address_space(3))) *)(__attribute__((address_space(3))) void const *)from));
+          }
+          uintx4 const both = {v[0][0], v[0][1], v[1][0], v[1][1]};
+          x8 const values = __builtin_bit_cast(x8, both);
+#pragma unroll
+          for (int r = 0; r < RG; r++) {
+            acc[r][d] = mfma(values, p[r], acc[r][d]);
+            acc[r][d] = mfma(values, rest[r], acc[r][d]);
+          }
+        }
+        wait_lds_reads();
+        if (more) {
+          load(v_base, v_lds, Values{});
+        }
       }
     }
-    __syncthreads();
-  }
-  T *const out = static_cast<T *>(P.out) + row * P.out_stride + (long long)head * D;
+
+    // the wavefronts' sums together
+    int const rows = R - row0 < 16 * RG ? R - row0 : 16 * RG;
+    bool const alone = units == span.units;
+    int const w0 = (unit - first) / run, wl = (unit - first + span.units - 1) / run, count = wl - w0 + 1, index = (int)blockIdx.x - w0;
+    auto slot = [&](int i) { return P.parts + (long long)(2 * (w0 + i) + (i == 0 ? 1 : 0)) * part_floats<DP, RG>(); };
+    float *const part = slot(index);
+    T *const out = static_cast<T *>(P.out) + (long long)sequence * P.new_tokens * P.out_stride + (long long)kv * P.group * P.head_dim;
+    auto store_row = [&](int row, int d, floatx4 x) {  // row of the head, columns d .. d + 3
+      if (d < P.head_dim) {
+        x4 y;
 #pragma unroll
-  for (int i = 0; i < MI355_MAX_PAGED_HEAD_DIM / 64; i++) {
-    int const d = 64 * i + lane;
-    if (d < D) {
-      out[d] = static_cast<T>(sum == 0.0f ? 0.0f : acc[i] / sum);
+        for (int e = 0; e < 4; e++) {
+          y[e] = static_cast<T>(x[e]);
+        }
+        *reinterpret_cast<x4 *>(out + row / P.group * P.out_stride + row % P.group * P.head_dim + d) = y;
+      }
+    };
+#pragma unroll
+    for (int r = 0; r < RG; r++) {
+      float const whole_sum = over_groups(sum[r], [](float a, float b) { return a + b; });
+      if (g == 0) {
+        stat[2 * (wave * 16 * RG + 16 * r + c)] = m[r];
+        stat[2 * (wave * 16 * RG + 16 * r + c) + 1] = whole_sum;
+      }
     }
+    float *const sums = reinterpret_cast<float *>(lds);  // [wave][row][DP]
+#pragma unroll
+    for (int r = 0; r < RG; r++) {
+      __syncthreads();
+#pragma unroll
+      for (int d = 0; d < DB; d++) {
+        *reinterpret_cast<floatx4 *>(sums + (wave * 16 + c) * DP + 16 * d + 4 * g) = acc[r][d];
+      }
+      __syncthreads();
+      for (int i = tid; i < 16 * DP / 4; i += kThreads) {
+        int const row = i / (DP / 4), d = i % (DP / 4) * 4;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+          top = fmaxf(top, stat[2 * (w * 16 * RG + 16 * r + row)]);
+        }
+        float const base = top == -INFINITY ? 0.0f : top;
+        floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        float all = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+          float const less = exp2_fast(stat[2 * (w * 16 * RG + 16 * r + row)] - base);
+          all += less * stat[2 * (w * 16 * RG + 16 * r + row) + 1];
+          x += less * *reinterpret_cast<floatx4 const *>(sums + (w * 16 + row) * DP + d);
+        }
+        if (16 * r + row >= rows) {
+          continue;
+        }
+        if (alone) {
+          store_row(row0 + 16 * r + row, d, all == 0.0f ? floatx4{0.0f, 0.0f, 0.0f, 0.0f} : x / all);
+        } else {
+          store_shared(part + (16 * r + row) * DP + d, x);
+          if (d == 0) {
+            store_shared(part + 16 * RG * DP + 4 * (16 * r + row), top, all);
+          }
+        }
+      }
+    }
+
+    // the last workgroup of a head, or of a group of its parts, joins them
+    if (!alone) {
+      auto arrive = [&](int *ticket, int of) {
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+        __syncthreads();
+        if (tid == 0) {
+          int const others = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          *is_last = others == of - 1;
+          if (others == of - 1) {
+            __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
+          }
+        }
+        __syncthreads();
+        return *is_last != 0;
+      };
+      // parts i0, i0 + step, .. (n of them), into the first of them or the result.  A joined part's maximum and sum lie beside
+      // its own, which other threads may still be reading (level 0: its own, 2: the joined ones).
+      auto join = [&](int i0, int step, int n, int level, bool final) {
+        for (int i = tid; i < rows * (DP / 4); i += kThreads) {
+          int const row = i / (DP / 4), d = i % (DP / 4) * 4;
+          float top = -INFINITY, all = 0.0f;
+          floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int j = 0; j < n; j++) {
+            float const *const from = slot(i0 + j * step);
+            uint64_t const a = load_shared(from + row * DP + d), b = load_shared(from + row * DP + d + 2);
+            uint64_t const ms = load_shared(from + 16 * RG * DP + 4 * row + level);
+            float const higher = fmaxf(top, low_of(ms)), base = higher == -INFINITY ? 0.0f : higher;
+            float const less = exp2_fast(top - base), its = exp2_fast(low_of(ms) - base);
+            top = higher;
+            all = all * less + high_of(ms) * its;
+            x = x * less + its * floatx4{low_of(a), high_of(a), low_of(b), high_of(b)};
+          }
+          if (final) {
+            store_row(row0 + row, d, all == 0.0f ? floatx4{0.0f, 0.0f, 0.0f, 0.0f} : x / all);
+          } else {
+            store_shared(slot(i0) + row * DP + d, x);
+            if (d == 0) {
+              store_shared(slot(i0) + 16 * RG * DP + 4 * row + 2, top, all);
+            }
+          }
+        }
+      };
+      int per = count;
+      if (count > kOneLevel) {
+        per = (int)ceilf(sqrtf((float)count));
+      }
+      int const of_group = index / per * per, in_group = count - of_group < per ? count - of_group : per;
+      bool last = arrive(P.tickets + 3 * (w0 + of_group) + (of_group == 0 ? 0 : 1), in_group);
+      if (last) {
+        join(of_group, 1, in_group, 0, per >= count);
+        if (per < count) {
+          int const groups = (count + per - 1) / per;
+          last = arrive(P.tickets + 3 * w0 + 2, groups);
+          if (last) {
+            join(0, per, groups, 2, true);
+          }
+        }
+      }
+    }
+    unit += units;
+    if (unit - before == span.units * P.heads) {
+      before = unit;
+      sequence++;
+    }
+    __syncthreads();  // (`stat`, `is_last` and the tiles are free again)
   }
+}
+
+template <class T, int DP, int RG>
+int launch_paged(PagedParams P, int kv_heads) {
+  auto *fn = paged_attention_kernel<T, DP, RG>;
+  int const rows = P.new_tokens * P.group;
+  P.row_blocks = (rows + 16 * RG - 1) / (16 * RG);
+  P.heads = kv_heads * P.row_blocks;
+  // workgroups that fit the chip together
+  int const per_unit = RG * DP >= 256 || DP > 128 ? 1 : 2;
+  long long const most = (long long)P.sequences * P.heads * (((long long)P.table_width * P.page_size + kUnit - 1) / kUnit + 1);
+  long long const fit = (long long)State::kJoinWorkgroups < 256LL * per_unit ? (long long)State::kJoinWorkgroups : 256LL * per_unit;
+  unsigned const grid = (unsigned)(most < fit ? most : fit);
+  if ((size_t)grid * 2 * part_floats<DP, RG>() * sizeof(float) > state().scratch_bytes) {
+    return fail(MI355_ERR_INVALID, "mi355_paged_attention: its parts do not fit the workspace");
+  }
+  constexpr int lds = lds_bytes<DP, RG>();
+  static_assert(lds <= 160 * 1024 && kWaves * 16 * DP * 4 <= kWaves * 2 * tile_bytes<DP>(), "LDS of a compute unit");
+  MI355_GRANT_LDS(fn, lds);
+  MI355_HIP(launch_kernel(fn, dim3(grid), dim3(kThreads), lds, state().stream(), P));
+  return MI355_OK;
+}
+
+template <class T, int DP>
+int launch_rows(PagedParams const &P, int kv_heads) {
+  long long const rows = (long long)P.new_tokens * P.group;
+  if (rows <= 16) {
+    return launch_paged<T, DP, 1>(P, kv_heads);
+  }
+  if (rows <= 32 || DP > 128) {
+    return launch_paged<T, DP, 2>(P, kv_heads);
+  }
+  if constexpr (DP <= 128) {
+    return launch_paged<T, DP, 4>(P, kv_heads);
+  }
+  return MI355_OK;
+}
+
+template <class T>
+int launch_head(PagedParams const &P, int kv_heads) {
+  return P.head_dim <= 64    ? launch_rows<T, 64>(P, kv_heads)
+         : P.head_dim <= 96  ? launch_rows<T, 96>(P, kv_heads)
+         : P.head_dim <= 128 ? launch_rows<T, 128>(P, kv_heads)
+         : P.head_dim <= 192 ? launch_rows<T, 192>(P, kv_heads)
+                             : launch_rows<T, 256>(P, kv_heads);
 }
 
 }  // namespace
@@ -128,8 +696,9 @@ extern "C" int mi355_paged_attention(void const *q, long long q_stride, void *ou
     return fail(MI355_ERR_INVALID, "mi355_paged_attention: %d sequences of %d new tokens, %d heads over %d, table of %d, window %d",
                 sequences, new_tokens, q_heads, c.kv_heads, table_width, window);
   }
-  if (c.head_dim % 8 != 0 || c.head_dim > MI355_MAX_PAGED_HEAD_DIM || (long long)table_width * c.page_size > INT_MAX - 1024 ||
-      (long long)sequences * new_tokens > INT_MAX || q_heads > 65535) {
+  long long const keys = (long long)table_width * c.page_size;
+  if (c.head_dim % 8 != 0 || c.head_dim > MI355_MAX_PAGED_HEAD_DIM || keys > 1 << 30 || (long long)sequences * new_tokens > INT_MAX ||
+      (long long)new_tokens * q_heads > 1 << 29) {
     return fail(MI355_ERR_UNSUPPORTED, "mi355_paged_attention: heads of %d, a table of %d pages of %d, %d x %d tokens, %d heads",
                 c.head_dim, table_width, c.page_size, sequences, new_tokens, q_heads);
   }
@@ -144,29 +713,49 @@ extern "C" int mi355_paged_attention(void const *q, long long q_stride, void *ou
   if (bits % 16 != 0 || (q_stride | out_stride | c.page_stride | c.token_stride | c.head_stride) % 8 != 0) {
     return fail(MI355_ERR_INVALID, "mi355_paged_attention: tensors begin, and their strides step, 16 bytes at a time");
   }
-  PagedParams P;
+  auto steps = [](long long stride, int n) { return stride / 8 > UINT32_MAX ? UINT32_MAX : (long long)(n - 1) * (stride / 8); };
+  if (steps(c.page_stride, c.pages) > UINT32_MAX || steps(c.token_stride, c.page_size) > UINT32_MAX || steps(c.head_stride, c.kv_heads) > UINT32_MAX ||
+      steps(c.page_stride, c.pages) + steps(c.token_stride, c.page_size) + steps(c.head_stride, c.kv_heads) + c.head_dim / 8 >= UINT32_MAX) {
+    return fail(MI355_ERR_UNSUPPORTED, "mi355_paged_attention: keys or values of more than 64 GB");
+  }
+  PagedParams P{};
   P.q = q;
   P.k = c.k;
   P.v = c.v;
   P.out = out;
   P.q_stride = q_stride;
   P.out_stride = out_stride;
-  P.page_stride = c.page_stride;
-  P.token_stride = c.token_stride;
-  P.head_stride = c.head_stride;
+  P.page_step = (uint32_t)(c.page_stride / 8);
+  P.token_step = (uint32_t)(c.token_stride / 8);
+  P.head_step = (uint32_t)(c.head_stride / 8);
   P.table = table;
   P.lengths = lengths;
+  P.parts = static_cast<float *>(state().scratch());
+  P.tickets = state().queue_join_tickets();
   P.pages = c.pages;
   P.page_size = c.page_size;
-  P.kv_heads = c.kv_heads;
   P.head_dim = c.head_dim;
   P.table_width = table_width;
-  P.sequences = sequences;
   P.new_tokens = new_tokens;
   P.group = q_heads / c.kv_heads;
-  P.window = window;
-  P.scale = scale;
-  auto *fn = c.type == MI355_TYPE_F16 ? paged_attention_kernel<_Float16> : paged_attention_kernel<__bf16>;
-  MI355_HIP(launch_kernel(fn, dim3((unsigned)(sequences * new_tokens), (unsigned)q_heads), dim3(64), 0, state().stream(), P));
+  P.window = window < keys ? window : 0;
+  P.page_magic = c.page_size == 1 ? 0 : (unsigned)(((1ull << 32) + c.page_size - 1) / c.page_size);
+  P.scale = scale * 1.44269504088896341f;
+  // units are counted in 32 bits: a batch with more of them goes in slices of sequences
+  long long const per_sequence = (long long)c.kv_heads * ((long long)new_tokens * P.group / 16 + 1) * (keys / kUnit + 2);
+  if (per_sequence > INT_MAX / 4) {
+    return fail(MI355_ERR_UNSUPPORTED, "mi355_paged_attention: %d new tokens of %d heads over %lld keys", new_tokens, q_heads, keys);
+  }
+  long long const slice = INT_MAX / 2 / per_sequence;
+  for (long long at = 0; at < sequences; at += slice) {
+    P.sequences = (int)(sequences - at < slice ? sequences - at : slice);
+    P.q = static_cast<char const *>(q) + 2 * at * new_tokens * q_stride;
+    P.out = static_cast<char *>(out) + 2 * at * new_tokens * out_stride;
+    P.table = table + at * table_width;
+    P.lengths = lengths + at;
+    if (int rc = c.type == MI355_TYPE_F16 ? launch_head<_Float16>(P, c.kv_heads) : launch_head<__bf16>(P, c.kv_heads)) {
+      return rc;
+    }
+  }
   return MI355_OK;
 }

@@ -211,6 +211,9 @@ extern "C" int mi355_init(size_t arena_bytes, void **arena_base) {
   MI355_HIP(hipMalloc(reinterpret_cast<void **>(&s.tickets), sizeof(int) * State::kTickets * MI355_NUM_QUEUES));
   MI355_HIP(hipMemset(s.tickets, 0, sizeof(int) * State::kTickets * MI355_NUM_QUEUES));
   forget_tickets();
+  size_t const join_bytes = sizeof(int) * 3 * State::kJoinWorkgroups * MI355_NUM_QUEUES;
+  MI355_HIP(hipMalloc(reinterpret_cast<void **>(&s.join_tickets), join_bytes));
+  MI355_HIP(hipMemset(s.join_tickets, 0, join_bytes));
   s.ready = true;
   if (arena_base != nullptr) {
     *arena_base = s.arena;
@@ -246,6 +249,7 @@ extern "C" int mi355_shutdown(void) {
   }
   MI355_HIP(hipFree(s.scratch_base));
   MI355_HIP(hipFree(s.tickets));
+  MI355_HIP(hipFree(s.join_tickets));
   forget_tickets();
   MI355_HIP(hipFree(s.planes_base));
   s.planes_base = nullptr;

@@ -152,7 +152,7 @@ bool attention_ok(DTensor const &q, DTensor const &k, DTensor const &v, DTensor 
   }
   return positive(q) && table.num_dims == 2 && positive(table) && table.data_type == DT_INT32 && row_major(table) && has_dims(lengths, {table.dim[0]}) &&
          lengths.data_type == DT_INT32 && row_major(lengths) && q.dim[0] % table.dim[0] == 0 &&
-         (long long)table.dim[1] * c.page_size <= INT_MAX - 1024;
+         (long long)table.dim[1] * c.page_size <= 1 << 30 && (long long)(q.dim[0] / table.dim[0]) * heads <= 1 << 29;
 }
 
 // `t` as [rows, vocabulary] of `rows` rows: [sequences, per, vocabulary] or [sequences * per, vocabulary]
