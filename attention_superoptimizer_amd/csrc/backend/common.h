@@ -113,10 +113,11 @@ struct State {
   static constexpr int kTickets = 1 << 16;
   int *tickets = nullptr;
   // Those of launches whose workgroups join parts of each other's results (paged_attention.hip): per queue three for each
-  // of the most workgroups such a launch has, zero whenever none runs.
-  static constexpr int kJoinWorkgroups = 1024;
+  // of the most workgroups such a launch has, zero whenever none runs.  A line of memory each: those that share one are
+  // drawn one after the other.
+  static constexpr int kJoinWorkgroups = 1024, kJoinStep = 32;
   int *join_tickets = nullptr;
-  int *queue_join_tickets() const { return join_tickets + 3 * kJoinWorkgroups * tls_queue; }
+  int *queue_join_tickets() const { return join_tickets + (size_t)3 * kJoinWorkgroups * kJoinStep * tls_queue; }
 };
 
 State &state();

@@ -49,7 +49,7 @@ struct PagedParams {
   uint32_t page_step, token_step, head_step;  // in 16 bytes: a cache is up to 64 GB
   int const *table, *lengths;
   float *parts;   // 2 per workgroup: the end of a head that began before it, the beginning of one that goes on after it
-  int *tickets;   // 3 per workgroup, zero between launches
+  int *tickets;   // 3 per workgroup, kJoinStep apart, zero between launches
   int pages, page_size, head_dim, table_width, sequences, new_tokens, group, window;
   int row_blocks, heads;  // of 16 RG rows, of a key-value head; key-value heads x row blocks
   unsigned page_magic;    // 2^32 / page_size, rounded up; 0 for 1
@@ -609,12 +609,12 @@ __global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void 
         per = (int)ceilf(sqrtf((float)count));
       }
       int const of_group = index / per * per, in_group = count - of_group < per ? count - of_group : per;
-      bool last = arrive(P.tickets + 3 * (w0 + of_group) + (of_group == 0 ? 0 : 1), in_group);
+      bool last = arrive(P.tickets + State::kJoinStep * (3 * (w0 + of_group) + (of_group == 0 ? 0 : 1)), in_group);
       if (last) {
         join(of_group, 1, in_group, 0, per >= count);
         if (per < count) {
           int const groups = (count + per - 1) / per;
-          last = arrive(P.tickets + 3 * w0 + 2, groups);
+          last = arrive(P.tickets + State::kJoinStep * (3 * w0 + 2), groups);
           if (last) {
             join(0, per, groups, 2, true);
           }
