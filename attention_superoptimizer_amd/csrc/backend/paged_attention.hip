@@ -13,6 +13,7 @@
 // * scores are made transposed, S^T = K Q^T: a lane then has the weights of one row, as the operand of O^T = V^T P^T
 //   wants them, and that row's maximum, sum and scale.
 #include "common.h"
+#include "mi355_kernels/kernarg.h"
 
 #include <climits>
 #include <cmath>
@@ -36,11 +37,9 @@ int check_paged_cache(mi355_paged_cache const &c) {
 
 namespace {
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kTile = 32;                 // keys of a wavefront at a time
-constexpr int kUnit = kTile * kWaves;     // and of a workgroup
 constexpr int kIds = 1024;                // page numbers of a run that a workgroup holds in LDS
-constexpr int kOneLevel = 8;              // parts that are joined at once; more of them in two levels
+constexpr int kAtOnce = 8;                // parts that a thread reads together; more are joined in two levels
 
 struct PagedParams {
   void const *q, *k, *v;
@@ -52,9 +51,17 @@ struct PagedParams {
   int *tickets;   // 3 per workgroup, kJoinStep apart, zero between launches
   int pages, page_size, head_dim, table_width, sequences, new_tokens, group, window;
   int row_blocks, heads;  // of 16 RG rows, of a key-value head; key-value heads x row blocks
-  unsigned page_magic;    // 2^32 / page_size, rounded up; 0 for 1
-  float scale;            // times log2 e: weights are powers of two
+  unsigned page_magic, group_magic;  // see quotient
+  uint32_t q_keep, q_flip;           // bits of queries: a scale of zero or below zero is in them
+  float scale;                       // its magnitude, times log2 e: weights are powers of two
 };
+
+// n / d for 0 <= n < 2^31 - d by magic = 2^32 / d, rounded up (0 for d = 1): one too many at most
+__device__ __forceinline__ int quotient(int n, int d, unsigned magic) {
+  int const q = magic == 0 ? n : (int)__umulhi((uint32_t)n, magic);
+  return q - (q * d > n ? 1 : 0);
+}
+unsigned magic_of(int d) { return d == 1 ? 0 : (unsigned)(((1ull << 32) + d - 1) / d); }
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
@@ -120,34 +127,59 @@ __device__ __forceinline__ int chunk_at(int row, int place) {
   return chunk < 0 ? chunk + C : chunk;
 }
 
-// x[l] op x[l ^ 16] op x[l ^ 32] op x[l ^ 48] in every lane: over the four groups of lanes that share a row
+// x[l] op x[l ^ 16] op x[l ^ 32] op x[l ^ 48] in every lane: over the four groups of lanes that share a row.  By the
+// instructions that exchange rows of 16 lanes and halves of a wavefront between two registers; a shuffle is a trip through
+// LDS.  (Inline assembly: the compiler's builtin returns the first result twice.  The wait states cover a write just before.)
 template <class Op>
 __device__ __forceinline__ float over_groups(float x, Op op) {
-  x = op(x, __shfl_xor(x, 16, 64));
-  return op(x, __shfl_xor(x, 32, 64));
+  float a = x, b = x;
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  a = b = op(a, b);
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  return op(a, b);
 }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Two weights as two numbers of the value's type each, of which the second is what cutting the first short lost.
+__device__ __forceinline__ void split(float w0, float w1, uint32_t &first, uint32_t &rest, _Float16) {
+  auto const cut = __builtin_amdgcn_cvt_pkrtz(w0, w1);
+  auto const less = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(-1.0f, static_cast<float>(cut[0]), w0), __builtin_fmaf(-1.0f, static_cast<float>(cut[1]), w1));
+  first = __builtin_bit_cast(uint32_t, cut);
+  rest = __builtin_bit_cast(uint32_t, less);
+}
+__device__ __forceinline__ void split(float w0, float w1, uint32_t &first, uint32_t &rest, __bf16) {
+  uint32_t const b0 = __builtin_bit_cast(uint32_t, w0), b1 = __builtin_bit_cast(uint32_t, w1);
+  first = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  pair const less = {static_cast<__bf16>(w0 - __builtin_bit_cast(float, b0 & 0xffff0000u)),
+                     static_cast<__bf16>(w1 - __builtin_bit_cast(float, b1 & 0xffff0000u))};
+  rest = __builtin_bit_cast(uint32_t, less);
+}
 
 struct Span {
   int from, to;  // keys, from a multiple of kTile on
   int units;     // at least one: a head without keys has its zeros to be written
 };
-__device__ __forceinline__ Span span_of(PagedParams const &P, int sequence) {
-  int const most = P.table_width * P.page_size, told = P.lengths[sequence];
+template <int UNIT>
+__device__ __forceinline__ Span span_of(PagedParams const &P, int told) {  // of the sequence with that length
+  int const most = P.table_width * P.page_size;
   int const length = told < 0 ? 0 : (told < most ? told : most);
   int const first = P.window != 0 ? length - (P.new_tokens - 1) - P.window : 0;  // (no underflow: the host bounds both)
   Span s;
   s.from = first > 0 ? first & ~(kTile - 1) : 0;
   s.to = length;
-  s.units = length > s.from ? (length - s.from + kUnit - 1) / kUnit : 1;
+  s.units = length > s.from ? (length - s.from + UNIT - 1) / UNIT : 1;
   return s;
 }
 
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    x += __shfl_xor(x, off, 64);
-  }
+// the sum of the lanes up to this one, by moves between registers: within rows of 16, then the ends of rows
+__device__ __forceinline__ int wave_upto(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // from 1, 2, 4, 8 lanes before in the row
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true);  // the end of rows 0 and 2 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);  // the end of row 1 to rows 2 and 3
   return x;
 }
 
@@ -175,14 +207,20 @@ template <int DP, int RG>
 constexpr int query_bytes() { return RG > 1 ? 16 * RG * DP * 2 : 0; }
 // tiles; queries, where they are too many for registers; page numbers; maximum and sum of every wavefront's rows; whether
 // this workgroup is the last
-template <int DP, int RG>
+template <int DP, int RG, int WAVES>
 constexpr int lds_bytes() {
-  return kWaves * 2 * tile_bytes<DP>() + query_bytes<DP, RG>() + (int)sizeof(int) * kIds + kWaves * 16 * RG * 8 + 16;
+  return WAVES * 2 * tile_bytes<DP>() + query_bytes<DP, RG>() + (int)sizeof(int) * kIds + WAVES * 16 * RG * 8 + 16;
 }
 
-// DP: the head size, rounded up; RG: groups of 16 rows.
-template <class T, int DP, int RG>
-__global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void paged_attention_kernel(PagedParams const P) {
+// Workgroups that a compute unit's LDS and registers hold.
+template <int DP, int RG, int WAVES>
+constexpr int per_compute_unit() { return WAVES == 4 && DP <= 128 && RG < 4 && RG * DP <= 288 ? 2 : 1; }
+
+// DP: the head size, rounded up; RG: groups of 16 rows; WAVES: wavefronts of a workgroup.
+template <class T, int DP, int RG, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, (WAVES / 4 * per_compute_unit<DP, RG, WAVES>())) void paged_attention_kernel(PagedParams const P) {
+  fetch_kernel_arguments<sizeof(PagedParams), 1>();  // one trip for all of them
+  constexpr int kWaves = WAVES, kThreads = 64 * WAVES, kUnit = kTile * WAVES;
   constexpr int C = DP / 8, LOADS = kTile * C / 64, KK = DP / 32, DB = DP / 16;
   typedef typename Vec<T>::x8 x8;
   typedef typename Vec<T>::x4 x4;
@@ -196,65 +234,82 @@ __global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void 
   uint32_t const k_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void const *)k_tile;
   uint32_t const v_lds = k_lds + tile_bytes<DP>();
 
-  // this workgroup's run of units, and the sequence it begins in
-  int total = 0;
-  for (int b = lane; b < P.sequences; b += 64) {
-    total += span_of(P, b).units;
+  // This workgroup's units.  Every head cut into equal parts of at most `run` units, a workgroup each, where that gives
+  // no more parts than workgroups; otherwise (heads shorter than a run) runs of units that go on from one head to the next.
+  int const own_length = lane < P.sequences ? P.lengths[lane] : 0;
+  int const own_units = lane < P.sequences ? span_of<kUnit>(P, own_length).units : 0;
+  auto over_sequences = [&](auto value) {  // the sum of value(units of a sequence)
+    int x = lane < P.sequences ? value(own_units) : 0;
+    for (int b = lane + 64; b < P.sequences; b += 64) {
+      x += value(span_of<kUnit>(P, P.lengths[b]).units);
+    }
+    return __builtin_amdgcn_readlane(wave_upto(x), 63) * P.heads;
+  };
+  int const total = over_sequences([](int units) { return units; }), me = (int)blockIdx.x, all = (int)gridDim.x;
+  int run = (total + all - 1) / all;
+  auto parts_of = [&](int units) { return run == 1 ? units : (units + run - 1) / run; };
+  bool apart = over_sequences(parts_of) <= all;
+  if (!apart && run >= 8) {  // (an eighth of a run more is less than what a second head costs)
+    run++;
+    apart = over_sequences(parts_of) <= all;
+    run -= apart ? 0 : 1;
   }
-  total = wave_sum(total) * P.heads;
-  int const run = (total + (int)gridDim.x - 1) / (int)gridDim.x;
-  long long const begin = (long long)blockIdx.x * run;
-  if (begin >= total) {
+  long long const begin = (long long)me * run;
+  if (!apart && begin >= total) {
     return;
   }
-  int unit = (int)begin;
+  int unit = apart ? me : (int)begin;  // (apart: the number of a part)
   int const end = total - unit < run ? total : unit + run;
-  int sequence = 0, before = 0;  // units of the sequences ahead of it
+  int sequence = 0, before = 0, length = 0;  // before: units (parts) of the sequences ahead of it
   for (int base = 0;; base += 64) {
-    int const b = base + lane;
-    int upto = b < P.sequences ? span_of(P, b).units * P.heads : 0;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      int const other = __shfl_up(upto, off, 64);
-      upto += lane >= off ? other : 0;
+    if (base >= P.sequences) {
+      return;  // (fewer parts than workgroups)
     }
+    int const b = base + lane, its = base == 0 ? own_length : (b < P.sequences ? P.lengths[b] : 0);
+    int units = base == 0 ? own_units : (b < P.sequences ? span_of<kUnit>(P, its).units : 0);
+    units = apart ? parts_of(units) : units;
+    int const upto = wave_upto(units) * P.heads;
     uint64_t const past = __ballot(before + upto > unit);
     if (past != 0) {
       int const at = __builtin_ctzll(past);
       sequence = base + at;
-      before += at > 0 ? __shfl(upto, at - 1, 64) : 0;
+      length = __builtin_amdgcn_readlane(its, at);
+      before += __builtin_amdgcn_readlane(upto - units * P.heads, at);
       break;
     }
-    before += __shfl(upto, 63, 64);
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
-  sequence = __builtin_amdgcn_readfirstlane(sequence);
-  before = __builtin_amdgcn_readfirstlane(before);
+  Span span = span_of<kUnit>(P, length);
+  int const cuts = apart ? parts_of(span.units) : span.units;
+  int head = (unit - before) / cuts, first = (unit - before) - head * cuts, part_index = first;
+  int kv = P.row_blocks == 1 ? head : head / P.row_blocks, row_block = head - kv * P.row_blocks;
+  int past_it = span.units;  // the unit behind this workgroup's last of the head
+  if (apart && cuts > 1) {
+    int const each = span.units / cuts, more = span.units - each * cuts;
+    first = part_index * each + (part_index < more ? part_index : more);
+    past_it = first + each + (part_index < more ? 1 : 0);
+  }
 
   int const R = P.new_tokens * P.group;
-  while (unit < end) {
-    Span const span = span_of(P, sequence);
-    int const head = (unit - before) / span.units, first = (unit - before) % span.units;
-    int const units = span.units - first < end - unit ? span.units - first : end - unit;
-    int const kv = head / P.row_blocks, row0 = head % P.row_blocks * 16 * RG;
+  for (;;) {
+    int const units = apart ? past_it - first : (span.units - first < end - unit ? span.units - first : end - unit);
+    int const row0 = row_block * 16 * RG;
     int const *const table = P.table + (long long)sequence * P.table_width;
+    int const next_length = sequence + 1 < P.sequences ? P.lengths[sequence + 1] : 0;
 
     // rows: lane's row c of every group, the new token t it belongs to, the keys it sees
     auto query = [&](int row, int d) {  // eight elements of a row of the head, zeros past its end
       uintx4 x = {0, 0, 0, 0};
       if (row < R && d < P.head_dim) {
-        x = *reinterpret_cast<uintx4 const *>(static_cast<T const *>(P.q) + ((long long)sequence * P.new_tokens + row / P.group) * P.q_stride +
-                                              (long long)(kv * P.group + row % P.group) * P.head_dim + d);
+        int const t = P.new_tokens == 1 ? 0 : quotient(row, P.group, P.group_magic);
+        x = *reinterpret_cast<uintx4 const *>(static_cast<T const *>(P.q) + ((long long)sequence * P.new_tokens + t) * P.q_stride +
+                                              (long long)(kv * P.group + row - t * P.group) * P.head_dim + d);
       }
       return x;
     };
+    auto as_scaled = [&](uintx4 x) { return uintx4{(x[0] & P.q_keep) ^ P.q_flip, (x[1] & P.q_keep) ^ P.q_flip, (x[2] & P.q_keep) ^ P.q_flip, (x[3] & P.q_keep) ^ P.q_flip}; };
     uintx4 q[KK];  // of one group of rows
     int limit[RG], least[RG];
-#pragma unroll
-    for (int r = 0; r < RG; r++) {
-      int const row = row0 + 16 * r + c;
-      limit[r] = row < R ? span.to - (P.new_tokens - 1 - row / P.group) : 0;
-      least[r] = row < R && P.window != 0 ? limit[r] - P.window : 0;
-    }
     if constexpr (RG == 1) {
 #pragma unroll
       for (int kk = 0; kk < KK; kk++) {
@@ -262,13 +317,20 @@ __global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void 
       }
     } else {
       for (int i = tid; i < 16 * RG * C; i += kThreads) {
-        *reinterpret_cast<uintx4 *>(queries + i / C * (2 * DP) + 16 * place_of<C, false>(i / C, i % C)) = query(row0 + i / C, i % C * 8);
+        *reinterpret_cast<uintx4 *>(queries + i / C * (2 * DP) + 16 * place_of<C, false>(i / C, i % C)) = as_scaled(query(row0 + i / C, i % C * 8));
       }
+    }
+#pragma unroll
+    for (int r = 0; r < RG; r++) {
+      int const row = row0 + 16 * r + c;
+      limit[r] = row < R ? span.to - (P.new_tokens - 1 - (P.new_tokens == 1 ? 0 : quotient(row, P.group, P.group_magic))) : 0;
+      least[r] = row < R && P.window != 0 ? limit[r] - P.window : 0;
     }
     // the keys that every row sees lie between these (rows of a block are in the order of their tokens)
     int const last_row = row0 + 16 * RG < R ? row0 + 16 * RG - 1 : R - 1;
-    int const all_limit = span.to - (P.new_tokens - 1 - row0 / P.group);
-    int const all_least = P.window != 0 ? span.to - (P.new_tokens - 1 - last_row / P.group) - P.window : 0;
+    bool const one = P.new_tokens == 1;
+    int const all_limit = span.to - (one ? 0 : P.new_tokens - 1 - quotient(row0, P.group, P.group_magic));
+    int const all_least = P.window != 0 ? span.to - (one ? 0 : P.new_tokens - 1 - quotient(last_row, P.group, P.group_magic)) - P.window : 0;
 
     floatx4 acc[RG][DB];
     float m[RG], sum[RG];
@@ -288,7 +350,8 @@ __global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void 
     for (int part = 0; part < units; part += fit) {
       int const part_units = units - part < fit ? units - part : fit;
       int const key0 = span.from + (first + part) * kUnit, key1 = key0 + part_units * kUnit < span.to ? key0 + part_units * kUnit : span.to;
-      int const page0 = key0 / P.page_size, numbers = key1 > key0 ? (key1 - 1) / P.page_size + 1 - page0 : 0;
+      int const page0 = quotient(key0, P.page_size, P.page_magic);
+      int const numbers = key1 > key0 ? quotient(key1 - 1, P.page_size, P.page_magic) + 1 - page0 : 0;
       __syncthreads();  // (the numbers of the part before, or the tiles as room for sums, are read)
       for (int i = tid; i < numbers; i += kThreads) {
         ids[i] = table[page0 + i];
@@ -296,6 +359,7 @@ __global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void 
       if constexpr (RG == 1) {
 #pragma unroll
         for (int kk = 0; kk < KK; kk++) {  // the queries are here: no wait for them inside the loop
+          q[kk] = part == 0 ? as_scaled(q[kk]) : q[kk];
           asm volatile("" : "+v"(q[kk]));
         }
       }
@@ -308,8 +372,7 @@ __global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void 
       uint32_t there = 0;     // keys that exist, a bit each
       auto locate = [&](int tile) {
         int const key = mine + tile * kUnit + lane % kTile;
-        int page = P.page_magic == 0 ? key : (int)__umulhi((uint32_t)key, P.page_magic);
-        page -= page * P.page_size > key ? 1 : 0;  // (the rounded reciprocal is one too many at most)
+        int const page = quotient(key, P.page_size, P.page_magic);
         int const number = key < key1 ? ids[page - page0] : -1;
         bool const is = (unsigned)number < (unsigned)P.pages;
         there = (uint32_t)__ballot(is);
@@ -372,16 +435,16 @@ __global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void 
           load(k_base, k_lds, Keys{});
         }
 
-        // weights, times 2^15 so that fp16 keeps small ones: two numbers of the value's type each, of which the second is
-        // what rounding the first lost -- one alone would put as much error into the result as rounding that does
+        // weights, times 2^15 so that fp16 keeps small ones: two numbers of the value's type each -- one alone would put as
+        // much error into the result as rounding that does
         bool const whole = is_there == ~0u && key >= all_least && key + kTile <= all_limit;
-        x8 p[RG], rest[RG];
+        uintx4 p[RG], rest[RG];
 #pragma unroll
         for (int r = 0; r < RG; r++) {
           float x[8];
 #pragma unroll
           for (int e = 0; e < 8; e++) {
-            x[e] = s[r][e / 4][e % 4] * P.scale;
+            x[e] = s[r][e / 4][e % 4];
           }
           if (!whole) {
             int const upto = limit[r] - key, from = least[r] - key;
@@ -396,7 +459,7 @@ __global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void 
           float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
           top = over_groups(top, [](float a, float b) { return fmaxf(a, b); });
           if (__any(top > m[r])) {
-            float const higher = fmaxf(m[r], top), less = exp2_fast(m[r] - (higher == -INFINITY ? 0.0f : higher));
+            float const higher = fmaxf(m[r], top), less = exp2_fast((m[r] - (higher == -INFINITY ? 0.0f : higher)) * P.scale);
             m[r] = higher;
             sum[r] *= less;
 #pragma unroll
@@ -404,13 +467,15 @@ __global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void 
               acc[r][d] *= less;
             }
           }
-          float const base = m[r] == -INFINITY ? 0.0f : m[r] - 15.0f;
+          float const base = m[r] == -INFINITY ? 0.0f : 15.0f - m[r] * P.scale;
 #pragma unroll
-          for (int e = 0; e < 8; e++) {
-            float const w = exp2_fast(x[e] - base);
-            sum[r] += w;
-            p[r][e] = static_cast<T>(w);
-            rest[r][e] = static_cast<T>(w - static_cast<float>(p[r][e]));
+          for (int e = 0; e < 8; e += 2) {
+            float const w0 = exp2_fast(__builtin_fmaf(x[e], P.scale, base)), w1 = exp2_fast(__builtin_fmaf(x[e + 1], P.scale, base));
+            sum[r] += w0 + w1;
+            uint32_t one_pair, its_rest;
+            split(w0, w1, one_pair, its_rest, T());
+            p[r][e / 2] = one_pair;
+            rest[r][e / 2] = its_rest;
           }
         }
         if (more) {
@@ -448,7 +513,7 @@ __global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void 
               w[r] = 0.0f;
 #pragma unroll
               for (int e = 0; e < 8; e++) {
-                w[r] = e == at_e ? static_cast<float>(p[r][e]) + static_cast<float>(rest[r][e]) : w[r];
+                w[r] = e == at_e ? static_cast<float>(__builtin_bit_cast(x8, p[r])[e]) + static_cast<float>(__builtin_bit_cast(x8, rest[r])[e]) : w[r];
               }
               w[r] = __shfl(w[r], holder, 64);
               sees[r] = key + j < limit[r] && key + j >= least[r];
@@ -487,8 +552,8 @@ __global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void 
           x8 const values = __builtin_bit_cast(x8, both);
 #pragma unroll
           for (int r = 0; r < RG; r++) {
-            acc[r][d] = mfma(values, p[r], acc[r][d]);
-            acc[r][d] = mfma(values, rest[r], acc[r][d]);
+            acc[r][d] = mfma(values, __builtin_bit_cast(x8, p[r]), acc[r][d]);
+            acc[r][d] = mfma(values, __builtin_bit_cast(x8, rest[r]), acc[r][d]);
           }
         }
         wait_lds_reads();
@@ -501,62 +566,68 @@ __global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void 
     // the wavefronts' sums together
     int const rows = R - row0 < 16 * RG ? R - row0 : 16 * RG;
     bool const alone = units == span.units;
-    int const w0 = (unit - first) / run, wl = (unit - first + span.units - 1) / run, count = wl - w0 + 1, index = (int)blockIdx.x - w0;
-    auto slot = [&](int i) { return P.parts + (long long)(2 * (w0 + i) + (i == 0 ? 1 : 0)) * part_floats<DP, RG>(); };
-    float *const part = slot(index);
+    float *const mine = P.parts + (2 * (long long)me + (first == 0 ? 1 : 0)) * part_floats<DP, RG>();
     T *const out = static_cast<T *>(P.out) + (long long)sequence * P.new_tokens * P.out_stride + (long long)kv * P.group * P.head_dim;
-    auto store_row = [&](int row, int d, floatx4 x) {  // row of the head, columns d .. d + 3
+    auto store_row = [&](int row, int d, floatx4 x, float all) {  // row of the head, columns d .. d + 3
       if (d < P.head_dim) {
+        int const t = P.new_tokens == 1 ? 0 : quotient(row, P.group, P.group_magic);
+        float const by = all == 0.0f ? 0.0f : 1.0f / all;
         x4 y;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          y[e] = static_cast<T>(x[e]);
+          y[e] = static_cast<T>(x[e] * by);
         }
-        *reinterpret_cast<x4 *>(out + row / P.group * P.out_stride + row % P.group * P.head_dim + d) = y;
+        *reinterpret_cast<x4 *>(out + t * P.out_stride + (row - t * P.group) * P.head_dim + d) = y;
       }
     };
 #pragma unroll
     for (int r = 0; r < RG; r++) {
       float const whole_sum = over_groups(sum[r], [](float a, float b) { return a + b; });
       if (g == 0) {
-        stat[2 * (wave * 16 * RG + 16 * r + c)] = m[r];
+        stat[2 * (wave * 16 * RG + 16 * r + c)] = m[r] * P.scale;
         stat[2 * (wave * 16 * RG + 16 * r + c) + 1] = whole_sum;
       }
     }
-    float *const sums = reinterpret_cast<float *>(lds);  // [wave][row][DP]
+    float *const sums = reinterpret_cast<float *>(lds);  // [wave][row][DP] of two groups of rows: what the tiles have room for
 #pragma unroll
-    for (int r = 0; r < RG; r++) {
+    for (int r0 = 0; r0 < RG; r0 += 2) {
+      constexpr int kPass = RG == 1 ? 16 : 32;
       __syncthreads();
+      if (16 * r0 >= rows) {
+        break;
+      }
 #pragma unroll
-      for (int d = 0; d < DB; d++) {
-        *reinterpret_cast<floatx4 *>(sums + (wave * 16 + c) * DP + 16 * d + 4 * g) = acc[r][d];
+      for (int r = r0; r < r0 + 2 && r < RG; r++) {
+#pragma unroll
+        for (int d = 0; d < DB; d++) {
+          *reinterpret_cast<floatx4 *>(sums + (wave * kPass + 16 * (r - r0) + c) * DP + 16 * d + 4 * g) = acc[r][d];
+        }
       }
       __syncthreads();
-      for (int i = tid; i < 16 * DP / 4; i += kThreads) {
+      int const pass_rows = rows - 16 * r0 < kPass ? rows - 16 * r0 : kPass;
+      for (int i = tid; i < pass_rows * (DP / 4); i += kThreads) {
         int const row = i / (DP / 4), d = i % (DP / 4) * 4;
-        float top = -INFINITY;
+        float its[kWaves][2], top = -INFINITY, whole_sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; w++) {
-          top = fmaxf(top, stat[2 * (w * 16 * RG + 16 * r + row)]);
+          its[w][0] = stat[2 * (w * 16 * RG + 16 * r0 + row)];
+          its[w][1] = stat[2 * (w * 16 * RG + 16 * r0 + row) + 1];
+          top = fmaxf(top, its[w][0]);
         }
         float const base = top == -INFINITY ? 0.0f : top;
         floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-        float all = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; w++) {
-          float const less = exp2_fast(stat[2 * (w * 16 * RG + 16 * r + row)] - base);
-          all += less * stat[2 * (w * 16 * RG + 16 * r + row) + 1];
-          x += less * *reinterpret_cast<floatx4 const *>(sums + (w * 16 + row) * DP + d);
-        }
-        if (16 * r + row >= rows) {
-          continue;
+          float const less = exp2_fast(its[w][0] - base);
+          whole_sum += less * its[w][1];
+          x += less * *reinterpret_cast<floatx4 const *>(sums + (w * kPass + row) * DP + d);
         }
         if (alone) {
-          store_row(row0 + 16 * r + row, d, all == 0.0f ? floatx4{0.0f, 0.0f, 0.0f, 0.0f} : x / all);
+          store_row(row0 + 16 * r0 + row, d, x, whole_sum);
         } else {
-          store_shared(part + (16 * r + row) * DP + d, x);
+          store_shared(mine + (16 * r0 + row) * DP + d, x);
           if (d == 0) {
-            store_shared(part + 16 * RG * DP + 4 * (16 * r + row), top, all);
+            store_shared(mine + 16 * RG * DP + 4 * (16 * r0 + row), top, whole_sum);
           }
         }
       }
@@ -564,6 +635,9 @@ __global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void 
 
     // the last workgroup of a head, or of a group of its parts, joins them
     if (!alone) {
+      int const w0 = apart ? me - part_index : (first == 0 ? me : (unit - first) / run), index = me - w0;
+      int const count = apart ? cuts : (unit - first + span.units - 1) / run - w0 + 1;
+      auto slot = [&](int i) { return P.parts + (2 * (long long)(w0 + i) + (i == 0 ? 1 : 0)) * part_floats<DP, RG>(); };
       auto arrive = [&](int *ticket, int of) {
         asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
         __syncthreads();
@@ -577,93 +651,140 @@ __global__ __launch_bounds__(kThreads, RG * DP >= 256 || DP > 128 ? 1 : 2) void 
         __syncthreads();
         return *is_last != 0;
       };
-      // parts i0, i0 + step, .. (n of them), into the first of them or the result.  A joined part's maximum and sum lie beside
-      // its own, which other threads may still be reading (level 0: its own, 2: the joined ones).
+      // Parts i0, i0 + step, .. (n of them), into the first of them or the result; kAtOnce of them are asked for together: a
+      // trip to the memory that all XCDs share is a microsecond.  A joined part's maximum and sum lie beside its own, which
+      // other threads may still be reading (level 0: its own, 2: the joined ones).
       auto join = [&](int i0, int step, int n, int level, bool final) {
-        for (int i = tid; i < rows * (DP / 4); i += kThreads) {
-          int const row = i / (DP / 4), d = i % (DP / 4) * 4;
-          float top = -INFINITY, all = 0.0f;
-          floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-          for (int j = 0; j < n; j++) {
-            float const *const from = slot(i0 + j * step);
-            uint64_t const a = load_shared(from + row * DP + d), b = load_shared(from + row * DP + d + 2);
-            uint64_t const ms = load_shared(from + 16 * RG * DP + 4 * row + level);
-            float const higher = fmaxf(top, low_of(ms)), base = higher == -INFINITY ? 0.0f : higher;
-            float const less = exp2_fast(top - base), its = exp2_fast(low_of(ms) - base);
-            top = higher;
-            all = all * less + high_of(ms) * its;
-            x = x * less + its * floatx4{low_of(a), high_of(a), low_of(b), high_of(b)};
+        constexpr int kItems = RG > 1 ? 2 : 1;
+        int const items = rows * (DP / 4);
+        for (int first_item = tid; first_item < items; first_item += kItems * kThreads) {
+          int row[kItems], d[kItems];
+          float top[kItems], all_sum[kItems];
+          floatx4 x[kItems];
+#pragma unroll
+          for (int k = 0; k < kItems; k++) {
+            int const i = first_item + k * kThreads < items ? first_item + k * kThreads : items - 1;
+            row[k] = i / (DP / 4);
+            d[k] = i % (DP / 4) * 4;
+            top[k] = -INFINITY;
+            all_sum[k] = 0.0f;
+            x[k] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
           }
-          if (final) {
-            store_row(row0 + row, d, all == 0.0f ? floatx4{0.0f, 0.0f, 0.0f, 0.0f} : x / all);
-          } else {
-            store_shared(slot(i0) + row * DP + d, x);
-            if (d == 0) {
-              store_shared(slot(i0) + 16 * RG * DP + 4 * row + 2, top, all);
+          for (int j0 = 0; j0 < n; j0 += kAtOnce) {
+            uint64_t a[kItems][kAtOnce], b[kItems][kAtOnce], ms[kItems][kAtOnce];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; j++) {
+              float const *const from = slot(i0 + (j0 + j < n ? j0 + j : n - 1) * step);
+#pragma unroll
+              for (int k = 0; k < kItems; k++) {
+                ms[k][j] = load_shared(from + 16 * RG * DP + 4 * row[k] + level);
+                a[k][j] = load_shared(from + row[k] * DP + d[k]);
+                b[k][j] = load_shared(from + row[k] * DP + d[k] + 2);
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < kAtOnce; j++) {  // (read whether they count or not: under the condition each is a trip of its own)
+#pragma unroll
+              for (int k = 0; k < kItems; k++) {
+                asm volatile("" : "+v"(a[k][j]), "+v"(b[k][j]), "+v"(ms[k][j]));
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < kAtOnce; j++) {
+              if (j0 + j < n) {
+#pragma unroll
+                for (int k = 0; k < kItems; k++) {
+                  float const higher = fmaxf(top[k], low_of(ms[k][j])), base = higher == -INFINITY ? 0.0f : higher;
+                  float const less = exp2_fast(top[k] - base), its = exp2_fast(low_of(ms[k][j]) - base);
+                  top[k] = higher;
+                  all_sum[k] = all_sum[k] * less + high_of(ms[k][j]) * its;
+                  x[k] = x[k] * less + its * floatx4{low_of(a[k][j]), high_of(a[k][j]), low_of(b[k][j]), high_of(b[k][j])};
+                }
+              }
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < kItems; k++) {
+            if (first_item + k * kThreads >= items) {
+              break;
+            }
+            if (final) {
+              store_row(row0 + row[k], d[k], x[k], all_sum[k]);
+            } else {
+              store_shared(slot(i0) + row[k] * DP + d[k], x[k]);
+              if (d[k] == 0) {
+                store_shared(slot(i0) + 16 * RG * DP + 4 * row[k] + 2, top[k], all_sum[k]);
+              }
             }
           }
         }
       };
-      int per = count;
-      if (count > kOneLevel) {
-        per = (int)ceilf(sqrtf((float)count));
-      }
+      int const per = count > kAtOnce ? (int)ceilf(sqrtf((float)count)) : count;
       int const of_group = index / per * per, in_group = count - of_group < per ? count - of_group : per;
-      bool last = arrive(P.tickets + State::kJoinStep * (3 * (w0 + of_group) + (of_group == 0 ? 0 : 1)), in_group);
-      if (last) {
+      if (arrive(P.tickets + State::kJoinStep * (3 * (w0 + of_group) + (of_group == 0 ? 0 : 1)), in_group)) {
         join(of_group, 1, in_group, 0, per >= count);
         if (per < count) {
           int const groups = (count + per - 1) / per;
-          last = arrive(P.tickets + State::kJoinStep * (3 * w0 + 2), groups);
-          if (last) {
+          if (arrive(P.tickets + State::kJoinStep * (3 * w0 + 2), groups)) {
             join(0, per, groups, 2, true);
           }
         }
       }
     }
     unit += units;
+    if (apart || unit >= end) {
+      return;
+    }
+    // the next head begins at its first unit
+    first = 0;
+    if (++row_block == P.row_blocks) {
+      row_block = 0;
+      kv++;
+    }
     if (unit - before == span.units * P.heads) {
       before = unit;
       sequence++;
+      kv = 0;
+      span = span_of<kUnit>(P, next_length);
     }
     __syncthreads();  // (`stat`, `is_last` and the tiles are free again)
   }
 }
 
-template <class T, int DP, int RG>
+template <class T, int DP, int RG, int WAVES>
 int launch_paged(PagedParams P, int kv_heads) {
-  auto *fn = paged_attention_kernel<T, DP, RG>;
+  auto *fn = paged_attention_kernel<T, DP, RG, WAVES>;
+  constexpr int kUnit = kTile * WAVES, lds = lds_bytes<DP, RG, WAVES>(), per_unit = per_compute_unit<DP, RG, WAVES>();
+  static_assert(lds <= 160 * 1024 && WAVES * (RG == 1 ? 16 : 32) * DP * 4 <= WAVES * 2 * tile_bytes<DP>(), "LDS of a compute unit");
   int const rows = P.new_tokens * P.group;
   P.row_blocks = (rows + 16 * RG - 1) / (16 * RG);
   P.heads = kv_heads * P.row_blocks;
   // workgroups that fit the chip together
-  int const per_unit = RG * DP >= 256 || DP > 128 ? 1 : 2;
   long long const most = (long long)P.sequences * P.heads * (((long long)P.table_width * P.page_size + kUnit - 1) / kUnit + 1);
   long long const fit = (long long)State::kJoinWorkgroups < 256LL * per_unit ? (long long)State::kJoinWorkgroups : 256LL * per_unit;
   unsigned const grid = (unsigned)(most < fit ? most : fit);
   if ((size_t)grid * 2 * part_floats<DP, RG>() * sizeof(float) > state().scratch_bytes) {
     return fail(MI355_ERR_INVALID, "mi355_paged_attention: its parts do not fit the workspace");
   }
-  constexpr int lds = lds_bytes<DP, RG>();
-  static_assert(lds <= 160 * 1024 && kWaves * 16 * DP * 4 <= kWaves * 2 * tile_bytes<DP>(), "LDS of a compute unit");
   MI355_GRANT_LDS(fn, lds);
-  MI355_HIP(launch_kernel(fn, dim3(grid), dim3(kThreads), lds, state().stream(), P));
+  MI355_HIP(launch_kernel(fn, dim3(grid), dim3(64 * WAVES), lds, state().stream(), P));
   return MI355_OK;
 }
 
+#ifndef MANY
+#define MANY 4
+#endif
 template <class T, int DP>
 int launch_rows(PagedParams const &P, int kv_heads) {
   long long const rows = (long long)P.new_tokens * P.group;
-  if (rows <= 16) {
-    return launch_paged<T, DP, 1>(P, kv_heads);
-  }
-  if (rows <= 32 || DP > 128) {
-    return launch_paged<T, DP, 2>(P, kv_heads);
-  }
   if constexpr (DP <= 128) {
-    return launch_paged<T, DP, 4>(P, kv_heads);
+    return rows <= 16   ? launch_paged<T, DP, 1, MANY>(P, kv_heads)
+           : rows <= 32 ? launch_paged<T, DP, 2, MANY>(P, kv_heads)
+           : rows <= 48 ? launch_paged<T, DP, 3, DP <= 64 ? MANY : 4>(P, kv_heads)
+                        : launch_paged<T, DP, 4, 4>(P, kv_heads);
+  } else {
+    return rows <= 16 ? launch_paged<T, DP, 1, 4>(P, kv_heads) : launch_paged<T, DP, 2, 4>(P, kv_heads);
   }
-  return MI355_OK;
 }
 
 template <class T>
@@ -739,10 +860,13 @@ extern "C" int mi355_paged_attention(void const *q, long long q_stride, void *ou
   P.new_tokens = new_tokens;
   P.group = q_heads / c.kv_heads;
   P.window = window < keys ? window : 0;
-  P.page_magic = c.page_size == 1 ? 0 : (unsigned)(((1ull << 32) + c.page_size - 1) / c.page_size);
-  P.scale = scale * 1.44269504088896341f;
+  P.page_magic = magic_of(c.page_size);
+  P.group_magic = magic_of(P.group);
+  P.q_keep = scale == 0.0f ? 0 : ~0u;
+  P.q_flip = scale < 0.0f ? 0x80008000u : 0;
+  P.scale = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504088896341f;
   // units are counted in 32 bits: a batch with more of them goes in slices of sequences
-  long long const per_sequence = (long long)c.kv_heads * ((long long)new_tokens * P.group / 16 + 1) * (keys / kUnit + 2);
+  long long const per_sequence = (long long)c.kv_heads * ((long long)new_tokens * P.group / 16 + 1) * (keys / (4 * kTile) + 2);
   if (per_sequence > INT_MAX / 4) {
     return fail(MI355_ERR_UNSUPPORTED, "mi355_paged_attention: %d new tokens of %d heads over %lld keys", new_tokens, q_heads, keys);
   }
