@@ -588,7 +588,10 @@ __global__ __launch_bounds__(64 * WAVES, (WAVES / 4 * per_compute_unit<DP, RG, W
         stat[2 * (wave * 16 * RG + 16 * r + c) + 1] = whole_sum;
       }
     }
-    float *const sums = reinterpret_cast<float *>(lds);  // [wave][row][DP] of two groups of rows: what the tiles have room for
+    // [wave][row][kRow] of two groups of rows: what the tiles, and the queries behind them, have room for.  Rows begin at
+    // other banks than their neighbours: a lane of each writes at once (a row after the other took 1 us).
+    float *const sums = reinterpret_cast<float *>(lds);
+    constexpr int kRow = DP + 4;
 #pragma unroll
     for (int r0 = 0; r0 < RG; r0 += 2) {
       constexpr int kPass = RG == 1 ? 16 : 32;
@@ -600,7 +603,7 @@ __global__ __launch_bounds__(64 * WAVES, (WAVES / 4 * per_compute_unit<DP, RG, W
       for (int r = r0; r < r0 + 2 && r < RG; r++) {
 #pragma unroll
         for (int d = 0; d < DB; d++) {
-          *reinterpret_cast<floatx4 *>(sums + (wave * kPass + 16 * (r - r0) + c) * DP + 16 * d + 4 * g) = acc[r][d];
+          *reinterpret_cast<floatx4 *>(sums + (wave * kPass + 16 * (r - r0) + c) * kRow + 16 * d + 4 * g) = acc[r][d];
         }
       }
       __syncthreads();
@@ -620,7 +623,7 @@ __global__ __launch_bounds__(64 * WAVES, (WAVES / 4 * per_compute_unit<DP, RG, W
         for (int w = 0; w < kWaves; w++) {
           float const less = exp2_fast(its[w][0] - base);
           whole_sum += less * its[w][1];
-          x += less * *reinterpret_cast<floatx4 const *>(sums + (w * kPass + row) * DP + d);
+          x += less * *reinterpret_cast<floatx4 const *>(sums + (w * kPass + row) * kRow + d);
         }
         if (alone) {
           store_row(row0 + 16 * r0 + row, d, x, whole_sum);
@@ -755,7 +758,7 @@ template <class T, int DP, int RG, int WAVES>
 int launch_paged(PagedParams P, int kv_heads) {
   auto *fn = paged_attention_kernel<T, DP, RG, WAVES>;
   constexpr int kUnit = kTile * WAVES, lds = lds_bytes<DP, RG, WAVES>(), per_unit = per_compute_unit<DP, RG, WAVES>();
-  static_assert(lds <= 160 * 1024 && WAVES * (RG == 1 ? 16 : 32) * DP * 4 <= WAVES * 2 * tile_bytes<DP>(), "LDS of a compute unit");
+  static_assert(lds <= 160 * 1024 && WAVES * (RG == 1 ? 16 : 32) * (DP + 4) * 4 <= WAVES * 2 * tile_bytes<DP>() + query_bytes<DP, RG>(), "LDS of a compute unit");
   int const rows = P.new_tokens * P.group;
   P.row_blocks = (rows + 16 * RG - 1) / (16 * RG);
   P.heads = kv_heads * P.row_blocks;
