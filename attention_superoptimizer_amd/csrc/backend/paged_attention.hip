@@ -774,20 +774,36 @@ int launch_paged(PagedParams P, int kv_heads) {
   return MI355_OK;
 }
 
-#ifndef MANY
-#define MANY 4
-#endif
+// Two workgroups of four wavefronts to a compute unit, or one of eight: fewer parts to join and, from HBM, wavefronts that
+// keep step (of two workgroups the second is served last), but twice the keys to a unit.  Eight where few heads have much
+// to read: measured (us, four and eight) 107 - 114 of 1 sequence x 8 heads x 131072 keys, 13.5 and 11.8 of 4 x 8 x 2000, 26.6
+// and 20.2 of 16 x 4 x 4096 with forty rows; against it 8.8 and 10.4 of 8 x 8 x 500, 33.3 and 39.5 of 128 x 8 x 500, 36.1 and
+// 38.4 of 16 x 8 x 4096.
+template <class T, int DP, int RG>
+int launch_group(PagedParams const &P, int kv_heads) {
+  if constexpr ((DP <= 128 && RG <= 2) || (DP <= 64 && RG == 3)) {
+    long long const heads = (long long)P.sequences * kv_heads * ((P.new_tokens * P.group + 16 * RG - 1) / (16 * RG));
+    long long const units = heads * (((long long)P.table_width * P.page_size + 4 * kTile - 1) / (4 * kTile));
+    if (heads <= (RG == 1 ? 96 : 256) && units >= 512) {
+      return launch_paged<T, DP, RG, 8>(P, kv_heads);
+    }
+  }
+  return launch_paged<T, DP, RG, 4>(P, kv_heads);
+}
+
 template <class T, int DP>
 int launch_rows(PagedParams const &P, int kv_heads) {
   long long const rows = (long long)P.new_tokens * P.group;
-  if constexpr (DP <= 128) {
-    return rows <= 16   ? launch_paged<T, DP, 1, MANY>(P, kv_heads)
-           : rows <= 32 ? launch_paged<T, DP, 2, MANY>(P, kv_heads)
-           : rows <= 48 ? launch_paged<T, DP, 3, DP <= 64 ? MANY : 4>(P, kv_heads)
-                        : launch_paged<T, DP, 4, 4>(P, kv_heads);
-  } else {
-    return rows <= 16 ? launch_paged<T, DP, 1, 4>(P, kv_heads) : launch_paged<T, DP, 2, 4>(P, kv_heads);
+  if (rows <= 16) {
+    return launch_group<T, DP, 1>(P, kv_heads);
   }
+  if (rows <= 32 || DP > 128) {
+    return launch_group<T, DP, 2>(P, kv_heads);
+  }
+  if constexpr (DP <= 128) {
+    return rows <= 48 ? launch_group<T, DP, 3>(P, kv_heads) : launch_group<T, DP, 4>(P, kv_heads);
+  }
+  return MI355_OK;
 }
 
 template <class T>
