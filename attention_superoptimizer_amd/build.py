@@ -38,7 +38,7 @@ DEVICE_FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17",
 
 
 # source file -> kernels that must build without register spills (see build_backend)
-NO_SPILL_KERNELS = {"fp_mfma.hip": ["fp_mfma_matmul_big_kernel"], "paged_attention.hip": ["paged_attention_kernel"]}
+NO_SPILL_KERNELS = {"fp_mfma.hip": ["fp_mfma_matmul_big_kernel"]}
 # fewest wavefronts per SIMD those kernels are written for (two workgroups per compute unit):
 # fewer means the register allocation is no longer the one the hand-placed loads and waits
 # were checked against
