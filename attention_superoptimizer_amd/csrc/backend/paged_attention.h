@@ -5,11 +5,13 @@
 //
 // Every key and value is read once for all rows of its head (query heads of the group x new tokens), so the bytes of
 // the cache bound a long call and the chain of trips to memory a short one.  What follows from that:
-// * the work is cut into units of 128 keys of one sequence and key-value head, numbered through the batch, and dealt
-//   in equal runs to the workgroups that fit the chip: how long each sequence is makes no difference.  The parts of
-//   a head that several workgroups have are joined by the last of them (a ticket), in the order of the keys.
+// * the work is cut into units of 128 keys (256 where a workgroup has eight wavefronts) of one sequence and key-value
+//   head.  Every head goes in equal parts to as many workgroups as its share of the chip is, or, where heads are more or
+//   shorter than that, units are dealt in equal runs that go on from one head to the next.  The parts of a head are joined
+//   by the last of its workgroups (a ticket), in the order of the keys; more than eight in two levels.
 // * a wavefront has 32 keys at a time and streams them from the pages straight into LDS of its own: no barrier in the
 //   loop.  The next keys are on their way while the scores become weights, the next values while the next scores are made.
+//   Waits count the transfers of the younger tile; anything else in flight would only make them wait for more.
 // * scores are made transposed, S^T = K Q^T: a lane then has the weights of one row, as the operand of O^T = V^T P^T
 //   wants them, and that row's maximum, sum and scale.
 #pragma once
@@ -156,7 +158,8 @@ __device__ __forceinline__ void split(float w0, float w1, uint32_t &first, uint3
 }
 
 struct Span {
-  int from, to;  // keys, from a multiple of kTile on
+  int first, to;  // the keys that any row sees
+  int from;       // the tile that the first of them lies in
   int units;     // at least one: a head without keys has its zeros to be written
 };
 template <int UNIT>
@@ -165,7 +168,8 @@ __device__ __forceinline__ Span span_of(PagedParams const &P, int told) {  // of
   int const length = told < 0 ? 0 : (told < most ? told : most);
   int const first = P.window != 0 ? length - (P.new_tokens - 1) - P.window : 0;  // (no underflow: the host bounds both)
   Span s;
-  s.from = first > 0 ? first & ~(kTile - 1) : 0;
+  s.first = first > 0 ? first : 0;
+  s.from = s.first & ~(kTile - 1);
   s.to = length;
   s.units = length > s.from ? (length - s.from + UNIT - 1) / UNIT : 1;
   return s;
@@ -346,7 +350,7 @@ __global__ __launch_bounds__(64 * WAVES, (WAVES / 4 * per_compute_unit<DP, RG, W
     uint64_t const k_base = reinterpret_cast<uint64_t>(P.k) + 16ull * kv * P.head_step, v_base = reinterpret_cast<uint64_t>(P.v) + 16ull * kv * P.head_step;
 
     // as many units at a time as the page numbers in LDS cover
-    int const fit = P.page_size < 1 << 16 ? (kIds - 1) * P.page_size / kUnit : 1 << 18;
+    int const fit = P.page_size < 1 << 16 ? (kIds - 1) * P.page_size / kUnit : 1 << 17;
     for (int part = 0; part < units; part += fit) {
       int const part_units = units - part < fit ? units - part : fit;
       int const key0 = span.from + (first + part) * kUnit, key1 = key0 + part_units * kUnit < span.to ? key0 + part_units * kUnit : span.to;
@@ -373,7 +377,7 @@ __global__ __launch_bounds__(64 * WAVES, (WAVES / 4 * per_compute_unit<DP, RG, W
       auto locate = [&](int tile) {
         int const key = mine + tile * kUnit + lane % kTile;
         int const page = quotient(key, P.page_size, P.page_magic);
-        int const number = key < key1 ? ids[page - page0] : -1;
+        int const number = key >= span.first && key < key1 ? ids[page - page0] : -1;
         bool const is = (unsigned)number < (unsigned)P.pages;
         there = (uint32_t)__ballot(is);
         uint32_t const step = is ? (uint32_t)number * P.page_step + (uint32_t)(key - page * P.page_size) * P.token_step : ~0u;

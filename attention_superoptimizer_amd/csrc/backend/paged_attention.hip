@@ -41,9 +41,12 @@ extern "C" int mi355_paged_attention(void const *q, long long q_stride, void *ou
   }
   long long const keys = (long long)table_width * c.page_size;
   if (c.head_dim % 8 != 0 || c.head_dim > MI355_MAX_PAGED_HEAD_DIM || keys > 1 << 30 || (long long)sequences * new_tokens > INT_MAX ||
-      (long long)new_tokens * q_heads > 1 << 29) {
+      (long long)new_tokens * q_heads > 1 << 29 || (long long)q_heads * c.head_dim > INT_MAX) {
     return fail(MI355_ERR_UNSUPPORTED, "mi355_paged_attention: heads of %d, a table of %d pages of %d, %d x %d tokens, %d heads",
                 c.head_dim, table_width, c.page_size, sequences, new_tokens, q_heads);
+  }
+  if ((long long)sequences * new_tokens > 1 && out_stride < (long long)q_heads * c.head_dim) {
+    return fail(MI355_ERR_INVALID, "mi355_paged_attention: results of %d heads of %d lie %lld apart", q_heads, c.head_dim, out_stride);
   }
   if (sequences == 0) {
     return MI355_OK;

@@ -3,7 +3,8 @@
 // A pair (a, b) of a head at position p becomes (a c - b s, b c + a s) with c = m cos(p w), s = m sin(p w).  p w is
 // computed in 64 bits and reduced to a fraction of a turn before it is rounded: in 32 bits the angle of position 10^6
 // would be 0.06 radians off.  The sines and cosines of a token are the same for all of its heads, so a workgroup
-// computes them once, one pair a thread, into LDS.
+// computes them once, one pair a thread, into LDS.  Bound by the launch for a few tokens (3.9 us of 16), by HBM for many: 8192
+// tokens with 32 + 8 heads of 128 move 201 MB in 40 us, the rate of a copy.
 #include "common.h"
 
 namespace mi355 {
@@ -19,7 +20,7 @@ struct RotaryParams {
   long long out_stride, page_stride, token_stride, head_stride;
   int const *positions, *slots;
   double const *angles;
-  int tokens, q_heads, kv_heads, head_dim, pairs, page_size, slot_count, head_split;
+  int tokens, q_heads, kv_heads, head_dim, pairs, page_size, slot_count, head_split;  // workgroups of a token
 };
 
 __device__ __forceinline__ float to_float(_Float16 x) { return static_cast<float>(x); }
@@ -102,21 +103,46 @@ bool wide(RotaryParams const &P, bool interleaved) {
   return bits % 16 == 0 && strides % 8 == 0;
 }
 
+// A token's heads by as many workgroups as give each thread one unit of work, up to 1024 of them: measured (us, one workgroup
+// and this) 4.3 and 3.9 of 16 tokens with 32 + 8 heads of 128, 5.7 and 3.9 of one with 128 + 16, 5.3 and 4.5 of 256 with
+// 64 + 8.  Past that each computes the sines again for nothing: 40.2 of 8192 tokens would be 42.2 by two a token.
 template <class T>
 int launch_rotary(RotaryParams P, bool interleaved) {
-  P.head_split = 1;
-  auto *fn = wide(P, interleaved) ? (interleaved ? rotary_kernel<T, 8, true> : rotary_kernel<T, 8, false>)
+  bool const by_eight = wide(P, interleaved);
+  long long const units = (long long)(P.q_heads + P.kv_heads) * (P.head_dim - (interleaved && by_eight ? 0 : P.pairs)) + (long long)P.kv_heads * P.head_dim;
+  long long const each = kThreads * (by_eight ? 8 : 1), most = P.tokens < 1024 ? 1024 / P.tokens : 1;
+  P.head_split = (int)((units + each - 1) / each < most ? (units + each - 1) / each : most);
+  auto *fn = by_eight ? (interleaved ? rotary_kernel<T, 8, true> : rotary_kernel<T, 8, false>)
                                   : (interleaved ? rotary_kernel<T, 1, true> : rotary_kernel<T, 1, false>);
-  MI355_HIP(launch_kernel(fn, dim3((unsigned)P.tokens, (unsigned)P.head_split), dim3(kThreads), 0, state().stream(), P));
+  constexpr int kMostTokens = 1 << 23;  // of a launch, which has less than 2^32 threads
+  for (int at = 0; at < P.tokens; at += kMostTokens) {
+    RotaryParams Q = P;
+    for (int i = 0; i < 3; i++) {
+      Q.src[i] = static_cast<T const *>(P.src[i]) + at * P.src_stride[i];
+    }
+    Q.q_out = static_cast<T *>(P.q_out) + at * P.out_stride;
+    Q.positions = P.positions + at;
+    Q.slots = P.slots != nullptr ? P.slots + at : nullptr;
+    int const count = P.tokens - at < kMostTokens ? P.tokens - at : kMostTokens;
+    MI355_HIP(launch_kernel(fn, dim3((unsigned)count, (unsigned)P.head_split), dim3(kThreads), 0, state().stream(), Q));
+    if (count < kMostTokens) {
+      break;
+    }
+  }
   return MI355_OK;
 }
 
 int rotary(RotaryParams const &P, int interleaved, int type) {
-  if (P.tokens < 0 || P.q_heads < 1 || P.head_dim < 1 || P.pairs < 1 || P.pairs > P.head_dim / 2 || P.out_stride < 0) {
+  if (P.tokens < 0 || P.q_heads < 1 || P.head_dim < 1 || P.pairs < 1 || P.pairs > P.head_dim / 2) {
     return fail(MI355_ERR_INVALID, "rotary: %d tokens, %d heads of %d, %d pairs", P.tokens, P.q_heads, P.head_dim, P.pairs);
   }
   if (P.pairs > kMostPairs || (long long)(P.q_heads + 2LL * P.kv_heads) * P.head_dim > (1 << 30)) {
     return fail(MI355_ERR_UNSUPPORTED, "rotary: %d pairs of a head, or too many heads", P.pairs);
+  }
+  if (P.src_stride[0] < 0 || P.src_stride[1] < 0 || P.src_stride[2] < 0 || P.out_stride < 0 ||
+      (P.tokens > 1 && P.out_stride < (long long)P.q_heads * P.head_dim)) {
+    return fail(MI355_ERR_INVALID, "rotary: a stride below zero, or results of %d heads of %d that lie %lld apart", P.q_heads, P.head_dim,
+                P.out_stride);
   }
   if (type != MI355_TYPE_F16 && type != MI355_TYPE_BF16) {
     return fail(MI355_ERR_UNSUPPORTED, "rotary: type %d", type);

@@ -91,6 +91,57 @@ def test_long_cache_split_over_workgroups(rt, kind, head, new, group):
     _check(head, [5000, 37, 2900], new=new, group=group, head=head, kind=kind, std=2.0)
 
 
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("head", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("group,new", [(5, 4), (8, 5), (16, 4), (8, 9), (3, 37)])
+def test_many_rows_split_over_workgroups(rt, kind, head, group, new):
+    """Rows for two, three, four groups of sixteen and for several blocks of them, a head's keys with several workgroups."""
+    _check(head + new, [900, 33], new=new, kv_heads=1, group=group, head=head, kind=kind, std=2.0)
+
+
+@pytest.mark.parametrize("head,group,new,lengths,kv_heads", [(64, 4, 1, [3000, 100], 2), (96, 1, 1, [1500], 1), (128, 8, 1, [4100, 0, 257], 2),
+                                                             (64, 8, 3, [2100, 700], 2), (96, 16, 2, [300, 1300], 1), (128, 9, 3, [2000], 2),
+                                                             (64, 12, 4, [2500, 31], 1), (64, 4, 1, list(range(20, 900, 30)), 3)])
+@pytest.mark.parametrize("window", [0, 700])
+def test_wide_tables(rt, head, group, new, lengths, kv_heads, window):
+    """Tables that name room for far more keys than there are: few heads that may have much to read."""
+    kind = "bf16" if head == 96 else "fp16"
+    x = _case(head + new, lengths, new, kv_heads, group, head, 16, kind, width=4200)
+    want, bound = attention(*x, float(np.float32(0.11)), window, kind)
+    check(_run(*x, kind, float(np.float32(0.11)), window), want, bound)
+
+
+@pytest.mark.parametrize("kind,code", [("fp16", 921), ("bf16", 920)])
+@pytest.mark.parametrize("head,group,new", [(64, 4, 1), (72, 8, 3), (96, 2, 2), (128, 8, 1), (128, 8, 4), (128, 8, 5), (64, 11, 4), (160, 3, 1), (192, 7, 3),
+                                            (256, 2, 1), (256, 8, 4)])
+def test_caches_larger_than_the_last_level_cache(rt, abi, kind, code, head, group, new):
+    """A cache of which the table could name more than is kept on the chip (and names a few pages)."""
+    lengths, kv_heads, size, width = [1300, 5, 0, 640], 2, 16, 1 << 15
+    q, k, v, table, n = _case(head + new, lengths, new, kv_heads, group, head, size, kind, width=width)
+    g = G.KNGraph()
+    try:
+        tq, tk, tv, tt, tl = put(g, q.reshape(-1, kv_heads * group, head), kind), put(g, k, kind), put(g, v, kind), put(g, table), put(g, n)
+        o = put(g, np.full(q.shape, 7.0).reshape(-1, kv_heads * group, head), kind)
+        c = N.Mi355PagedCache(tk.device_ptr(False), tv.device_ptr(False), 1 << 17, size, kv_heads, head, size * kv_heads * head,
+                              kv_heads * head, head, code)
+        stride = kv_heads * group * head
+        rc = abi.mi355_paged_attention(tq.device_ptr(False), stride, o.device_ptr(False), stride, ctypes.byref(c), tt.device_ptr(False),
+                                       width, tl.device_ptr(False), len(lengths), new, kv_heads * group, 0.125, 0)
+        assert rc == 0, N.last_error()
+        want, bound = attention(q, k, v, table, n, 0.125, 0, kind)
+        check(read(o).reshape(q.shape), want, bound)
+    finally:
+        g.close()
+
+
+@pytest.mark.parametrize("window", [0, 200])
+def test_more_heads_than_workgroups(rt, window):
+    """Workgroups go on from one head to the next and share the longer ones; the last parts of heads join out of turn."""
+    rng = np.random.default_rng(17)
+    lengths = [int(n) for n in rng.integers(0, 90, 90)] + [2500, 0, 1] + [int(n) for n in rng.integers(200, 500, 20)]
+    _check(18, lengths, new=2, kv_heads=8, group=2, window=window, page_size=32, kind="fp16")
+
+
 def test_many_short_sequences(rt):
     rng = np.random.default_rng(2)
     _check(1, [int(n) for n in rng.integers(0, 60, 300)], kv_heads=4, group=2, kind="bf16")
@@ -168,7 +219,7 @@ def test_sequences_share_pages(rt):
 
 
 @pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
-@pytest.mark.parametrize("new,window", [(1, 0), (4, 0), (4, 50)])
+@pytest.mark.parametrize("new,window", [(1, 0), (4, 0), (4, 50), (1, 50), (1, 64)])
 def test_masked_places_hold_anything(rt, value, new, window):
     """Behind a sequence's end, before its window and, for all new tokens but the last, at the last token's key: no row
     that does not see the key changes by a bit."""
@@ -178,7 +229,7 @@ def test_masked_places_hold_anything(rt, value, new, window):
     plain = _run(q, k, v, table, n, "bf16", 0.125, window, passes=1)
     for b, length in enumerate(lengths):
         for j in range(-(-length // 16) * 16):
-            if j >= length - 1 or (window and j < length - new - window):
+            if j >= length - 1 or (window and j <= length - new - window):
                 if new > 1 or j != length - 1:
                     k[table[b, j // 16], j % 16] = v[table[b, j // 16], j % 16] = value
     got = _run(q, k, v, table, n, "bf16", 0.125, window, passes=1)
@@ -313,7 +364,7 @@ def test_refusals(rt, abi):
         assert call(cache(), sequences=0) == 0
         for change in (dict(q=None), dict(out=None), dict(table=None), dict(lengths=None), dict(q=at + 2), dict(out=at + 8200),
                        dict(q_stride=132), dict(out_stride=129), dict(width=0), dict(sequences=-1), dict(new=0), dict(heads=0),
-                       dict(scale=float("nan")), dict(window=-1), dict(q_stride=-128)):
+                       dict(scale=float("nan")), dict(window=-1), dict(q_stride=-128), dict(out_stride=120)):
             assert call(cache(), **change) == -3, change
         assert call(None) == -3
         for change, code in ((dict(kv_heads=3), -3), (dict(k=None), -3), (dict(v=at + 16384), -3), (dict(page_stride=4), -3),
@@ -321,5 +372,7 @@ def test_refusals(rt, abi):
                              (dict(pages=0), -3), (dict(k=at + 8), -3)):
             assert call(cache(**change)) == code, change
         assert call(cache(), width=1 << 29) == -4
+        assert call(cache(head_dim=256, token_stride=256, page_stride=2048), heads=1 << 24, q_stride=1 << 32, out_stride=1 << 32) == -4
+        assert call(cache(), sequences=1, out_stride=0) == 0  # one row
     finally:
         g.close()

@@ -19,7 +19,8 @@ def _angles(half, far=False):
 @pytest.mark.parametrize("kind", ["fp16", "bf16"])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("tokens,heads,head,half", [(1, 1, 64, 32), (3, 5, 128, 64), (70, 40, 128, 64), (9, 3, 80, 16), (5, 7, 96, 20),
-                                                    (4, 2, 10, 3), (2, 3, 7, 2), (6, 1, 256, 128), (300, 4, 64, 4), (1, 2, 640, 320)])
+                                                    (4, 2, 10, 3), (2, 3, 7, 2), (6, 1, 256, 128), (300, 4, 64, 4), (1, 2, 640, 320), (1, 128, 64, 32),
+                                                    (40, 33, 90, 45)])
 def test_rotary(rt, kind, interleaved, tokens, heads, head, half):
     rng = np.random.default_rng(tokens * 1000 + head)
     x = normal(rng, (tokens, heads, head), kind)
@@ -54,6 +55,31 @@ def test_angle_of_far_positions(rt, kind):
         check(read(y), want, rotary_bound(want, parts, kind) + 2.0 ** -19)
     finally:
         g.close()
+
+
+def test_more_tokens_than_a_launch_has(rt, abi):
+    """2^23 + 5 tokens of one pair, a slot each."""
+    import torch
+    tokens = (1 << 23) + 5
+    x = torch.randn(3, tokens, 2, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    out, cache = torch.zeros(tokens, 2, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, tokens, 2, dtype=torch.bfloat16, device="cuda")
+    positions = torch.arange(tokens, dtype=torch.int32, device="cuda") % 5000
+    slots = torch.arange(tokens - 1, -1, -1, dtype=torch.int32, device="cuda")
+    angles = torch.tensor([0.5, 1.0], dtype=torch.float64, device="cuda")
+    torch.cuda.synchronize()
+    c = N.Mi355PagedCache(cache[0].data_ptr(), cache[1].data_ptr(), tokens, 1, 1, 2, 2, 2, 2, 920)
+    rc = abi.mi355_rotary_append(x[0].data_ptr(), 2, x[1].data_ptr(), 2, x[2].data_ptr(), 2, out.data_ptr(), 2, positions.data_ptr(),
+                                 angles.data_ptr(), slots.data_ptr(), ctypes.byref(c), tokens, 1, 1, 0)
+    assert rc == 0, N.last_error()
+    assert abi.mi355_sync() == 0
+    assert torch.equal(cache[1], x[2].flip(0))
+    turn = positions.double() * 0.5
+    cos, sin = turn.cos(), turn.sin()
+    for got, of in ((out, x[0]), (cache[0].flip(0), x[1])):
+        a, b = of.double().unbind(1)
+        want = torch.stack([a * cos - b * sin, b * cos + a * sin], 1)
+        bound = 2.0 ** -8 * want.abs() + 2.0 ** -20 * (a.abs() + b.abs())[:, None]  # (rotary_bound, rounded up)
+        assert ((got.double() - want).abs() <= bound).all()
 
 
 def _append(rt, kind, tokens, q_heads, kv_heads, head, half, page_size, pages, heads_first, interleaved, flat, slots, seed):
@@ -207,7 +233,7 @@ def test_refusals(rt, abi):
         a = put(g, np.zeros(64)).device_ptr(False)
         good = [at, 64, at + 4096, 64, i, a, 4, 1, 64, 32, 0, 921]
         assert abi.mi355_rotary(*good) == 0
-        for place, value, code in ((6, -1, -3), (7, 0, -3), (8, 0, -3), (9, 33, -3), (9, 0, -3), (11, 930, -4), (0, None, -3),
+        for place, value, code in ((6, -1, -3), (7, 0, -3), (8, 0, -3), (9, 33, -3), (9, 0, -3), (11, 930, -4), (0, None, -3), (1, -64, -3), (3, -64, -3), (3, 56, -3),
                                    (2, None, -3), (4, None, -3), (5, None, -3)):
             assert abi.mi355_rotary(*[value if n == place else x for n, x in enumerate(good)]) == code, (place, value)
         assert abi.mi355_rotary(at, 64, at, 72, i, a, 4, 1, 64, 32, 0, 921) == -3
