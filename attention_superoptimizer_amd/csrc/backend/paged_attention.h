@@ -5,7 +5,7 @@
 //
 // Every key and value is read once for all rows of its head (query heads of the group x new tokens), so the bytes of
 // the cache bound a long call and the chain of trips to memory a short one.  What follows from that:
-// * the work is cut into units of 128 keys (256 where a workgroup has eight wavefronts) of one sequence and key-value
+// * the work is cut into units of 128 keys (32 a wavefront, of which a workgroup has one, four or eight) of one sequence and key-value
 //   head.  Every head goes in equal parts to as many workgroups as its share of the chip is, or, where heads are more or
 //   shorter than that, units are dealt in equal runs that go on from one head to the next.  The parts of a head are joined
 //   by the last of its workgroups (a ticket), in the order of the keys; more than eight in two levels.
@@ -27,7 +27,8 @@ namespace mi355 {
 namespace paged {
 
 constexpr int kTile = 32;                 // keys of a wavefront at a time
-constexpr int kIds = 1024;                // page numbers of a run that a workgroup holds in LDS
+template <int WAVES>
+constexpr int kIdsOf = WAVES == 1 ? 256 : 1024;  // page numbers of a run that a workgroup holds in LDS
 constexpr int kAtOnce = 8;                // parts that a thread reads together; more are joined in two levels
 
 struct PagedParams {
@@ -212,19 +213,22 @@ constexpr int query_bytes() { return RG > 1 ? 16 * RG * DP * 2 : 0; }
 // this workgroup is the last
 template <int DP, int RG, int WAVES>
 constexpr int lds_bytes() {
-  return WAVES * 2 * tile_bytes<DP>() + query_bytes<DP, RG>() + (int)sizeof(int) * kIds + WAVES * 16 * RG * 8 + 16;
+  return WAVES * 2 * tile_bytes<DP>() + query_bytes<DP, RG>() + (int)sizeof(int) * kIdsOf<WAVES> + WAVES * 16 * RG * 8 + 16;
 }
 
 // Workgroups that a compute unit's LDS and registers hold.
 template <int DP, int RG, int WAVES>
-constexpr int per_compute_unit() { return WAVES == 4 && DP <= 128 && RG < 4 && RG * DP <= 288 ? 2 : 1; }
+constexpr int per_compute_unit() {
+  constexpr int by_lds = 160 * 1024 / lds_bytes<DP, RG, WAVES>(), by_registers = (DP <= 128 && RG < 4 && RG * DP <= 288 ? 8 : 4) / WAVES;
+  return WAVES == 8 ? 1 : (by_lds < by_registers ? by_lds : by_registers);
+}
 
 // DP: the head size, rounded up; RG: groups of 16 rows; WAVES: wavefronts of a workgroup; PASSING: keys and values are not to
 // be kept in the caches.
 template <class T, int DP, int RG, int WAVES, bool PASSING>
-__global__ __launch_bounds__(64 * WAVES, (WAVES / 4 * per_compute_unit<DP, RG, WAVES>())) void paged_attention_kernel(PagedParams const P) {
+__global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVES>() + 3) / 4)) void paged_attention_kernel(PagedParams const P) {
   fetch_kernel_arguments<sizeof(PagedParams), 1>();  // one trip for all of them
-  constexpr int kWaves = WAVES, kThreads = 64 * WAVES, kUnit = kTile * WAVES;
+  constexpr int kWaves = WAVES, kThreads = 64 * WAVES, kUnit = kTile * WAVES, kIds = kIdsOf<WAVES>;
   constexpr int C = DP / 8, LOADS = kTile * C / 64, KK = DP / 32, DB = DP / 16;
   typedef typename Vec<T>::x8 x8;
   typedef typename Vec<T>::x4 x4;
@@ -299,7 +303,12 @@ __global__ __launch_bounds__(64 * WAVES, (WAVES / 4 * per_compute_unit<DP, RG, W
     int const units = apart ? past_it - first : (span.units - first < end - unit ? span.units - first : end - unit);
     int const row0 = row_block * 16 * RG;
     int const *const table = P.table + (long long)sequence * P.table_width;
-    int const next_length = sequence + 1 < P.sequences ? P.lengths[sequence + 1] : 0;
+    int next_length = 0;  // by a vector load: a scalar one is waited for at once, its register being short
+    if (!apart && sequence + 1 < P.sequences) {
+      int same = 0;
+      asm volatile("" : "+v"(same));
+      next_length = P.lengths[sequence + 1 + same];
+    }
 
     // rows: lane's row c of every group, the new token t it belongs to, the keys it sees
     auto query = [&](int row, int d) {  // eight elements of a row of the head, zeros past its end
@@ -752,7 +761,7 @@ __global__ __launch_bounds__(64 * WAVES, (WAVES / 4 * per_compute_unit<DP, RG, W
       before = unit;
       sequence++;
       kv = 0;
-      span = span_of<kUnit>(P, next_length);
+      span = span_of<kUnit>(P, __builtin_amdgcn_readfirstlane(next_length));
     }
     __syncthreads();  // (`stat`, `is_last` and the tiles are free again)
   }
@@ -768,7 +777,8 @@ int launch_paged(PagedParams P, int kv_heads) {
   P.heads = kv_heads * P.row_blocks;
   // workgroups that fit the chip together
   long long const most = (long long)P.sequences * P.heads * (((long long)P.table_width * P.page_size + kUnit - 1) / kUnit + 1);
-  long long const fit = (long long)State::kJoinWorkgroups < 256LL * per_unit ? (long long)State::kJoinWorkgroups : 256LL * per_unit;
+  long long const room = (long long)(state().scratch_bytes / (2 * part_floats<DP, RG>() * sizeof(float)));
+  long long const fit = room < 256LL * per_unit ? room : 256LL * per_unit;
   unsigned const grid = (unsigned)(most < fit ? most : fit);
   if ((size_t)grid * 2 * part_floats<DP, RG>() * sizeof(float) > state().scratch_bytes) {
     return fail(MI355_ERR_INVALID, "mi355_paged_attention: its parts do not fit the workspace");
@@ -780,15 +790,23 @@ int launch_paged(PagedParams P, int kv_heads) {
 
 // Two workgroups of four wavefronts to a compute unit, or one of eight: fewer parts to join and, from HBM, wavefronts that
 // keep step (of two workgroups the second is served last), but twice the keys to a unit.  Eight where few heads have much
-// to read, or all of them more than the caches keep: measured (us, four and eight) 114 - 115 and 107 of 1 sequence x 8 heads x
-// 131072 keys, 97.6 and 95.8 of 64 x 8 x 4096, 13.5 and 11.8 of 4 x 8 x 2000, 26.6 and 20.2 of 16 x 4 x 4096 with forty rows;
-// against it 8.8 and 10.4 of 8 x 8 x 500, 33.3 and 39.5 of 128 x 8 x 500, 36.1 and 38.4 of 16 x 8 x 4096.
+// to read, or all of them more than the caches keep: measured (us, four and eight) 115 and 107 of 1 sequence x 8 heads x
+// 131072 keys, 97.6 and 95.5 of 64 x 8 x 4096, 13.5 and 11.8 of 4 x 8 x 2000, 26.6 and 20.2 of 16 x 4 x 4096 with forty rows;
+// against it 8.8 and 10.4 of 8 x 8 x 500, 33.3 and 39.5 of 128 x 8 x 500, 36.1 and 38.4 of 16 x 8 x 4096, 186 and 226 of 1024 x 8 x 400.
+// Eight workgroups of one wavefront for thousands of heads that are short: no wavefront waits for another at a head's end (four
+// and one: 95 and 75 us of 1024 sequences x 8 heads x 100 keys, 352 and 244 of 4096 x 8 x 100, 186 and 176 of 1024 x 8 x 400;
+// against it 98 and 104 of 64 x 8 x 4096, 33.4 and 33.2 of 128 x 8 x 500, 7.7 and 11.4 of 64 x 8 x 100).
 template <class T, int DP, int RG>
 int launch_group(PagedParams const &P, int kv_heads, bool passing) {
   if constexpr ((DP <= 128 && RG <= 2) || (DP <= 64 && RG == 3)) {
     long long const heads = (long long)P.sequences * kv_heads * ((P.new_tokens * P.group + 16 * RG - 1) / (16 * RG));
-    long long const units = heads * (((long long)P.table_width * P.page_size + 4 * kTile - 1) / (4 * kTile));
-    if (RG <= 2 && passing) {
+    long long const keys = (long long)P.table_width * P.page_size, units = heads * ((keys + 4 * kTile - 1) / (4 * kTile));
+    if constexpr (RG == 1) {
+      if (heads >= 2048 && keys <= 512) {
+        return passing ? launch_paged<T, DP, RG, 1, true>(P, kv_heads) : launch_paged<T, DP, RG, 1, false>(P, kv_heads);
+      }
+    }
+    if (RG <= 2 && passing && keys >= 1024) {
       return launch_paged<T, DP, RG, 8, RG <= 2>(P, kv_heads);
     }
     if (heads <= (RG == 1 ? 96 : 256) && units >= 512) {

@@ -111,27 +111,44 @@ def test_wide_tables(rt, head, group, new, lengths, kv_heads, window):
     check(_run(*x, kind, float(np.float32(0.11)), window), want, bound)
 
 
-@pytest.mark.parametrize("kind,code", [("fp16", 921), ("bf16", 920)])
-@pytest.mark.parametrize("head,group,new", [(64, 4, 1), (72, 8, 3), (96, 2, 2), (128, 8, 1), (128, 8, 4), (128, 8, 5), (64, 11, 4), (160, 3, 1), (192, 7, 3),
-                                            (256, 2, 1), (256, 8, 4)])
-def test_caches_larger_than_the_last_level_cache(rt, abi, kind, code, head, group, new):
-    """A cache of which the table could name more than is kept on the chip (and names a few pages)."""
-    lengths, kv_heads, size, width = [1300, 5, 0, 640], 2, 16, 1 << 15
-    q, k, v, table, n = _case(head + new, lengths, new, kv_heads, group, head, size, kind, width=width)
+def _claimed(abi, x, kind, pages, window=0):
+    """The same by the C ABI, of a cache that is said to have `pages` pages (the table names those there are)."""
+    q, k, v, table, n = x
+    size, kv_heads, head = k.shape[1:]
+    q_heads = q.shape[2]
     g = G.KNGraph()
     try:
-        tq, tk, tv, tt, tl = put(g, q.reshape(-1, kv_heads * group, head), kind), put(g, k, kind), put(g, v, kind), put(g, table), put(g, n)
-        o = put(g, np.full(q.shape, 7.0).reshape(-1, kv_heads * group, head), kind)
-        c = N.Mi355PagedCache(tk.device_ptr(False), tv.device_ptr(False), 1 << 17, size, kv_heads, head, size * kv_heads * head,
-                              kv_heads * head, head, code)
-        stride = kv_heads * group * head
-        rc = abi.mi355_paged_attention(tq.device_ptr(False), stride, o.device_ptr(False), stride, ctypes.byref(c), tt.device_ptr(False),
-                                       width, tl.device_ptr(False), len(lengths), new, kv_heads * group, 0.125, 0)
+        tq, tk, tv, tt, tl = put(g, q.reshape(-1, q_heads, head), kind), put(g, k, kind), put(g, v, kind), put(g, table), put(g, n)
+        o = put(g, np.full((q.shape[0] * q.shape[1], q_heads, head), 7.0), kind)
+        c = N.Mi355PagedCache(tk.device_ptr(False), tv.device_ptr(False), pages, size, kv_heads, head, size * kv_heads * head,
+                              kv_heads * head, head, TYPES[kind])
+        rc = abi.mi355_paged_attention(tq.device_ptr(False), q_heads * head, o.device_ptr(False), q_heads * head, ctypes.byref(c),
+                                       tt.device_ptr(False), table.shape[1], tl.device_ptr(False), q.shape[0], q.shape[1], q_heads, 0.125,
+                                       window)
         assert rc == 0, N.last_error()
-        want, bound = attention(q, k, v, table, n, 0.125, 0, kind)
+        want, bound = attention(*x, 0.125, window, kind)
         check(read(o).reshape(q.shape), want, bound)
     finally:
         g.close()
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("head,group,new", [(64, 4, 1), (72, 8, 3), (96, 2, 2), (128, 8, 1), (128, 8, 4), (128, 8, 5), (64, 11, 4), (160, 3, 1), (192, 7, 3),
+                                            (256, 2, 1), (256, 8, 4)])
+def test_caches_larger_than_the_last_level_cache(rt, abi, kind, head, group, new):
+    """A cache of which the table could name more than is kept on the chip (and names a few pages)."""
+    _claimed(abi, _case(head + new, [1300, 5, 0, 640], new, 2, group, head, 16, kind, width=1 << 15), kind, 1 << 17)
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("head,group,new,width", [(64, 1, 1, 8), (80, 3, 1, 20), (96, 4, 2, 32), (128, 4, 1, 32), (128, 2, 8, 5), (256, 1, 1, 8)])
+@pytest.mark.parametrize("pages", [0, 1 << 15])
+def test_many_heads_over_short_tables(rt, abi, kind, head, group, new, width, pages):
+    """Thousands of key-value heads of a few hundred keys at most, of caches small and large."""
+    rng = np.random.default_rng(head + width)
+    lengths = [int(n) for n in rng.integers(0, min(16 * width, 90), 256)] + [16 * width, 0, 1]
+    x = _case(head + new, lengths, new, 8, group, head, 16, kind, width=width)
+    _claimed(abi, x, kind, max(pages, x[1].shape[0]), window=37 if width == 20 else 0)
 
 
 @pytest.mark.parametrize("window", [0, 200])
