@@ -209,12 +209,19 @@ template <int DP>
 constexpr int tile_bytes() { return kTile * DP * 2; }
 template <int DP, int RG>
 constexpr int query_bytes() { return RG > 1 ? 16 * RG * DP * 2 : 0; }
-// tiles; queries, where they are too many for registers; page numbers; maximum and sum of every wavefront's rows; whether
-// this workgroup is the last
+// tiles, and queries where they are too many for registers; at a head's end in their place the wavefronts' sums, whose rows
+// begin at other banks than their neighbours (a lane of each writes at once: a row after the other took 1 us)
+template <int DP>
+constexpr int sum_row() { return DP + 4; }
 template <int DP, int RG, int WAVES>
-constexpr int lds_bytes() {
-  return WAVES * 2 * tile_bytes<DP>() + query_bytes<DP, RG>() + (int)sizeof(int) * kIdsOf<WAVES> + WAVES * 16 * RG * 8 + 16;
+constexpr int tiles_bytes() {
+  constexpr int tiles = WAVES * 2 * tile_bytes<DP>() + query_bytes<DP, RG>(), sums = WAVES * 16 * RG * sum_row<DP>() * 4;
+  return tiles > sums ? tiles : sums;
 }
+// behind them page numbers; maximum and sum of every wavefront's rows; what a row is to be multiplied by; whether this workgroup
+// is the last
+template <int DP, int RG, int WAVES>
+constexpr int lds_bytes() { return tiles_bytes<DP, RG, WAVES>() + (int)sizeof(int) * kIdsOf<WAVES> + WAVES * 16 * RG * 8 + 16 * RG * 4 + 16; }
 
 // Workgroups that a compute unit's LDS and registers hold.
 template <int DP, int RG, int WAVES>
@@ -234,9 +241,10 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
   typedef typename Vec<T>::x4 x4;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   unsigned char *const queries = lds + kWaves * 2 * tile_bytes<DP>();
-  int *const ids = reinterpret_cast<int *>(queries + query_bytes<DP, RG>());
+  int *const ids = reinterpret_cast<int *>(lds + tiles_bytes<DP, RG, WAVES>());
   float *const stat = reinterpret_cast<float *>(ids + kIds);
-  int *const is_last = reinterpret_cast<int *>(stat + kWaves * 16 * RG * 2);
+  float *const row_by = stat + kWaves * 16 * RG * 2;
+  int *const is_last = reinterpret_cast<int *>(row_by + 16 * RG);
   int const tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16, c = lane % 16;
   unsigned char *const k_tile = lds + wave * 2 * tile_bytes<DP>(), *const v_tile = k_tile + tile_bytes<DP>();
   uint32_t const k_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void const *)k_tile;
@@ -501,21 +509,33 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
         // the values out of a sum.  Such keys' values are added to the rows that do see them by themselves, and zero from
         // then on.
         if (!whole && P.new_tokens > 1) {
-          uint32_t wild = 0;  // keys with such values
+          constexpr uint32_t top = Vec<T>::exponent;
+          typedef uint16_t shortx2 __attribute__((ext_vector_type(2)));
+          shortx2 most = {0, 0};
 #pragma unroll
           for (int i = 0; i < LOADS; i++) {
             uintx4 const x = *reinterpret_cast<uintx4 const *>(v_tile + 16 * (64 * i + lane));
-            bool none = false;
 #pragma unroll
             for (int w = 0; w < 4; w++) {
-              constexpr uint32_t top = Vec<T>::exponent;
-              none = none || (x[w] & top) == top || (x[w] & top << 16) == top << 16;
+              most = __builtin_elementwise_max(most, __builtin_bit_cast(shortx2, x[w] & (top << 16 | top)));
             }
-            wild |= none ? 1u << ((64 * i + lane) / C) : 0u;
           }
+          uint32_t wild = 0;  // keys with such values
+          if (__any(most[0] == top || most[1] == top)) {
 #pragma unroll
-          for (int off = 32; off > 0; off >>= 1) {
-            wild |= (uint32_t)__shfl_xor((int)wild, off, 64);
+            for (int i = 0; i < LOADS; i++) {
+              uintx4 const x = *reinterpret_cast<uintx4 const *>(v_tile + 16 * (64 * i + lane));
+              bool none = false;
+#pragma unroll
+              for (int w = 0; w < 4; w++) {
+                none = none || (x[w] & top) == top || (x[w] & top << 16) == top << 16;
+              }
+              wild |= none ? 1u << ((64 * i + lane) / C) : 0u;
+            }
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) {
+              wild |= (uint32_t)__shfl_xor((int)wild, off, 64);
+            }
           }
           for (uint32_t left = __builtin_amdgcn_readfirstlane(wild); left != 0; left &= left - 1) {
             int const j = __builtin_ctz(left), holder = 16 * (j % 16 / 4) + c, at_e = 4 * (j / 16) + j % 4;
@@ -580,11 +600,11 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
     int const rows = R - row0 < 16 * RG ? R - row0 : 16 * RG;
     bool const alone = units == span.units;
     float *const mine = P.parts + (2 * (long long)me + (first == 0 ? 1 : 0)) * part_floats<DP, RG>();
+    auto of_sum = [](float all) { return all == 0.0f ? 0.0f : 1.0f / all; };
     T *const out = static_cast<T *>(P.out) + (long long)sequence * P.new_tokens * P.out_stride + (long long)kv * P.group * P.head_dim;
-    auto store_row = [&](int row, int d, floatx4 x, float all) {  // row of the head, columns d .. d + 3
+    auto store_row = [&](int row, int d, floatx4 x, float by) {  // row of the head, columns d .. d + 3
       if (d < P.head_dim) {
         int const t = P.new_tokens == 1 ? 0 : quotient(row, P.group, P.group_magic);
-        float const by = all == 0.0f ? 0.0f : 1.0f / all;
         x4 y;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -601,51 +621,48 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
         stat[2 * (wave * 16 * RG + 16 * r + c) + 1] = whole_sum;
       }
     }
-    // [wave][row][kRow] of two groups of rows: what the tiles, and the queries behind them, have room for.  Rows begin at
-    // other banks than their neighbours: a lane of each writes at once (a row after the other took 1 us).
-    float *const sums = reinterpret_cast<float *>(lds);
-    constexpr int kRow = DP + 4;
+    float *const sums = reinterpret_cast<float *>(lds);  // [wave][row][kRow]
+    constexpr int kRow = sum_row<DP>();
+    __syncthreads();
 #pragma unroll
-    for (int r0 = 0; r0 < RG; r0 += 2) {
-      constexpr int kPass = RG == 1 ? 16 : 32;
-      __syncthreads();
-      if (16 * r0 >= rows) {
-        break;
+    for (int r = 0; r < RG; r++) {
+      int const row = 16 * r + c;
+      float its[kWaves][2], top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) {
+        its[w][0] = stat[2 * (w * 16 * RG + row)];
+        its[w][1] = stat[2 * (w * 16 * RG + row) + 1];
+        top = fmaxf(top, its[w][0]);
       }
+      float const base = top == -INFINITY ? 0.0f : top, less = exp2_fast(m[r] * P.scale - base);
 #pragma unroll
-      for (int r = r0; r < r0 + 2 && r < RG; r++) {
-#pragma unroll
-        for (int d = 0; d < DB; d++) {
-          *reinterpret_cast<floatx4 *>(sums + (wave * kPass + 16 * (r - r0) + c) * kRow + 16 * d + 4 * g) = acc[r][d];
-        }
+      for (int d = 0; d < DB; d++) {
+        *reinterpret_cast<floatx4 *>(sums + (wave * 16 * RG + row) * kRow + 16 * d + 4 * g) = acc[r][d] * less;
       }
-      __syncthreads();
-      int const pass_rows = rows - 16 * r0 < kPass ? rows - 16 * r0 : kPass;
-      for (int i = tid; i < pass_rows * (DP / 4); i += kThreads) {
-        int const row = i / (DP / 4), d = i % (DP / 4) * 4;
-        float its[kWaves][2], top = -INFINITY, whole_sum = 0.0f;
+      if (wave == r % kWaves && g == 0 && row < rows) {
+        float whole_sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; w++) {
-          its[w][0] = stat[2 * (w * 16 * RG + 16 * r0 + row)];
-          its[w][1] = stat[2 * (w * 16 * RG + 16 * r0 + row) + 1];
-          top = fmaxf(top, its[w][0]);
+          whole_sum += exp2_fast(its[w][0] - base) * its[w][1];
         }
-        float const base = top == -INFINITY ? 0.0f : top;
-        floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        row_by[row] = of_sum(whole_sum);
+        if (!alone) {
+          store_shared(mine + 16 * RG * DP + 4 * row, top, whole_sum);
+        }
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < rows * (DP / 4); i += kThreads) {
+      int const row = i / (DP / 4), d = i % (DP / 4) * 4;
+      floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-          float const less = exp2_fast(its[w][0] - base);
-          whole_sum += less * its[w][1];
-          x += less * *reinterpret_cast<floatx4 const *>(sums + (w * kPass + row) * kRow + d);
-        }
-        if (alone) {
-          store_row(row0 + 16 * r0 + row, d, x, whole_sum);
-        } else {
-          store_shared(mine + (16 * r0 + row) * DP + d, x);
-          if (d == 0) {
-            store_shared(mine + 16 * RG * DP + 4 * (16 * r0 + row), top, whole_sum);
-          }
-        }
+      for (int w = 0; w < kWaves; w++) {
+        x += *reinterpret_cast<floatx4 const *>(sums + (w * 16 * RG + row) * kRow + d);
+      }
+      if (alone) {
+        store_row(row0 + row, d, x, row_by[row]);
+      } else {
+        store_shared(mine + row * DP + d, x);
       }
     }
 
@@ -725,7 +742,7 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
               break;
             }
             if (final) {
-              store_row(row0 + row[k], d[k], x[k], all_sum[k]);
+              store_row(row0 + row[k], d[k], x[k], of_sum(all_sum[k]));
             } else {
               store_shared(slot(i0) + row[k] * DP + d[k], x[k]);
               if (d[k] == 0) {
@@ -771,7 +788,7 @@ template <class T, int DP, int RG, int WAVES, bool PASSING>
 int launch_paged(PagedParams P, int kv_heads) {
   auto *fn = paged_attention_kernel<T, DP, RG, WAVES, PASSING>;
   constexpr int kUnit = kTile * WAVES, lds = lds_bytes<DP, RG, WAVES>(), per_unit = per_compute_unit<DP, RG, WAVES>();
-  static_assert(lds <= 160 * 1024 && WAVES * (RG == 1 ? 16 : 32) * (DP + 4) * 4 <= WAVES * 2 * tile_bytes<DP>() + query_bytes<DP, RG>(), "LDS of a compute unit");
+  static_assert(lds <= 160 * 1024, "LDS of a compute unit");
   int const rows = P.new_tokens * P.group;
   P.row_blocks = (rows + 16 * RG - 1) / (16 * RG);
   P.heads = kv_heads * P.row_blocks;
