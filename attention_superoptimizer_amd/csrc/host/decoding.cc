@@ -50,7 +50,7 @@ bool room_for(std::initializer_list<size_t> data_bytes, std::initializer_list<si
   size_t need = 0;
   for (auto const &list : {data_bytes, fingerprint_bytes}) {
     for (size_t b : list) {
-      need += (b + 15) / 16 * 16;
+      need += (b + 15) / 16 * 16 + 256;  // (a large tensor may skip to a cache line)
     }
   }
   DeviceMemoryManager *dmm = DeviceMemoryManager::get_instance();

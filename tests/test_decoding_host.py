@@ -231,3 +231,22 @@ def test_bf16_values_round_to_the_nearest_even():
     np.testing.assert_array_equal(got.view(np.uint32), want.view(np.uint32))
     nan = G._bf16_bits(np.array([np.nan, np.uint32(0x7f800001).view(np.float32)], np.float32))
     assert ((nan & 0x7f80) == 0x7f80).all() and ((nan & 0x7f) != 0).all()
+
+
+def test_large_tensors_begin_with_a_cache_line():
+    """Wherever the arena stands, and give back what that skipped; small ones follow one another."""
+    rt = N.runtime()
+    base = rt.mirage_arena_offset()
+    for before in (1, 8, 9, 100, 1000):
+        g = G.KNGraph()
+        g.new_input((before,), G.DT_INT32)
+        small = g.new_input((3, 5), G.DT_BFLOAT16)
+        large = g.new_input((1 << 19,), G.DT_BFLOAT16)
+        assert large.device_ptr(False) % 256 == 0 and 0 <= large.device_ptr(False) - small.device_ptr(False) < 1024
+        at = rt.mirage_arena_offset()
+        other = g.new_input((1 << 10, 1 << 10), G.DT_FLOAT32)
+        assert other.device_ptr(False) % 256 == 0
+        g.pop_operator()
+        assert rt.mirage_arena_offset() == at
+        g.close()
+        assert rt.mirage_arena_offset() == base
