@@ -807,11 +807,12 @@ int launch_paged(PagedParams P, int kv_heads) {
 
 // Two workgroups of four wavefronts to a compute unit, or one of eight: fewer parts to join and, from HBM, wavefronts that
 // keep step (of two workgroups the second is served last), but twice the keys to a unit.  Eight where few heads have much
-// to read, or all of them more than the caches keep: measured (us, four and eight) 115 and 107 of 1 sequence x 8 heads x
-// 131072 keys, 97.6 and 95.5 of 64 x 8 x 4096, 13.5 and 11.8 of 4 x 8 x 2000, 26.6 and 20.2 of 16 x 4 x 4096 with forty rows;
-// against it 8.8 and 10.4 of 8 x 8 x 500, 33.3 and 39.5 of 128 x 8 x 500, 36.1 and 38.4 of 16 x 8 x 4096, 186 and 226 of 1024 x 8 x 400.
+// to read, or all of them more than the caches keep: measured (us, four and eight) 99.7 and 95.7 of 1 sequence x 8 heads x
+// 131072 keys, 98.7 and 94.7 of 64 x 8 x 4096, 12.8 and 11.2 of 4 x 8 x 2000, 47.3 and 38.3 of 16 x 4 x 8192 with 32 rows; against it
+// 8.8 and 10.4 of 8 x 8 x 500, 32.9 and 38.9 of 128 x 8 x 500, 31.6 and 34.8 of 16 x 8 x 4096, 181 and 222 of 1024 x 8 x 400, and heads
+// of 64, of which less is on its way: 37.9 and 41.0 of 47 x 5 x 6280.
 // Eight workgroups of one wavefront for thousands of heads that are short: no wavefront waits for another at a head's end (four
-// and one: 95 and 75 us of 1024 sequences x 8 heads x 100 keys, 352 and 244 of 4096 x 8 x 100, 186 and 176 of 1024 x 8 x 400;
+// and one: 93 and 74 us of 1024 sequences x 8 heads x 100 keys, 355 and 244 of 4096 x 8 x 100, 181 and 177 of 1024 x 8 x 400;
 // against it 98 and 104 of 64 x 8 x 4096, 33.4 and 33.2 of 128 x 8 x 500, 7.7 and 11.4 of 64 x 8 x 100).
 template <class T, int DP, int RG>
 int launch_group(PagedParams const &P, int kv_heads, bool passing) {
@@ -823,8 +824,10 @@ int launch_group(PagedParams const &P, int kv_heads, bool passing) {
         return passing ? launch_paged<T, DP, RG, 1, true>(P, kv_heads) : launch_paged<T, DP, RG, 1, false>(P, kv_heads);
       }
     }
-    if (RG <= 2 && passing && keys >= 1024) {
-      return launch_paged<T, DP, RG, 8, RG <= 2>(P, kv_heads);
+    if constexpr (RG <= 2) {
+      if (passing && keys >= 1024) {
+        return launch_paged<T, DP, RG, (DP <= 64 ? 4 : 8), true>(P, kv_heads);
+      }
     }
     if (heads <= (RG == 1 ? 96 : 256) && units >= 512) {
       return launch_paged<T, DP, RG, 8, false>(P, kv_heads);

@@ -90,10 +90,11 @@ extern "C" int mi355_paged_attention(void const *q, long long q_stride, void *ou
   P.q_keep = scale == 0.0f ? 0 : ~0u;
   P.q_flip = scale < 0.0f ? 0x80008000u : 0;
   P.scale = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504088896341f;
-  // Loads that are not to be kept in the caches, from what the 256 MB of the last-level cache hold on: 109 -> 98 us for 539 MB
-  // of 64 sequences; of 150 MB that are read again it costs 3 % (36.9 -> 38.0 us).
+  // Loads that are not to be kept in the caches, from three quarters of the 256 MB on that the last-level cache holds: measured
+  // (us, kept and not) 106 and 95 of 539 MB in 64 sequences, 49.5 and 45.8 of 201 MB in 24, 53.6 and 47.6 of 255 MB in 9; against it
+  // 31.6 and 32.4 of 150 MB in 16, 28.2 and 29.3 of 136 MB in 14.
   long long const slots = (long long)sequences * keys < (long long)c.pages * c.page_size ? (long long)sequences * keys : (long long)c.pages * c.page_size;
-  bool const passing = 4 * slots * c.kv_heads * c.head_dim > 256LL << 20;
+  bool const passing = 4 * slots * c.kv_heads * c.head_dim > 192LL << 20;
   // units are counted in 32 bits: a batch with more of them goes in slices of sequences
   long long const per_sequence = (long long)c.kv_heads * ((long long)new_tokens * P.group / 16 + 1) * (keys / (4 * kTile) + 2);
   if (per_sequence > INT_MAX / 4) {
