@@ -302,8 +302,10 @@ class KNGraph:
         head_dim] or [sequences * new, q_heads * head_dim], a sequence's tokens in a row; table [sequences, pages] and
         lengths [sequences] int32, a length with the new tokens, whose keys are in the caches already.  New token t sees
         the keys before length - (new - 1 - t), of these the last `window` if that is not 0; a row that sees none, or
-        only scores of minus infinity, is zeros.  Query head h reads key-value head h // (q_heads // kv_heads).  A page number outside the cache holds no
-        keys, a length past the table counts as the table's.  scale: 1 / sqrt(head_dim) if not given."""
+        only scores of minus infinity, is zeros.  Query head h reads key-value head h // (q_heads // kv_heads).  A page
+        number outside the cache holds no keys, a length past the table counts as the table's.  What lies in places that a
+        row does not see never reaches it; a seen value that is no number leaves its column none.  scale: 1 /
+        sqrt(head_dim) if not given."""
         if scale is None:
             scale = float(k_cache.dims[-1]) ** -0.5
         return self._wrap(self._rt.mirage_graph_paged_attention(self._g, q._h, k_cache._h, v_cache._h, table._h, lengths._h,
