@@ -11,7 +11,7 @@ namespace mi355 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMostPairs = 1024;  // of a head: their sines and cosines are 8 KB of LDS
+constexpr int kMostPairs = MI355_MAX_ROTARY_PAIRS;  // of a head: their sines and cosines are 8 KB of LDS
 
 struct RotaryParams {
   void const *src[3];  // queries, keys, values

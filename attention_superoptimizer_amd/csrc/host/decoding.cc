@@ -118,11 +118,12 @@ int heads_in(DTensor const &t, int head_dim) {
 
 bool angles_ok(DTensor const &positions, DTensor const &angles, int tokens, int head_dim) {
   return positive(positions) && positive(angles) && has_dims(positions, {tokens}) && positions.data_type == DT_INT32 && row_major(positions) && angles.num_dims == 2 &&
-         angles.dim[0] == 2 && angles.dim[1] <= head_dim / 2 && angles.data_type == DT_DOUBLE && row_major(angles);
+         angles.dim[0] == 2 && angles.dim[1] <= head_dim / 2 && angles.dim[1] <= MI355_MAX_ROTARY_PAIRS && angles.data_type == DT_DOUBLE && row_major(angles);
 }
 
 bool rotary_ok(DTensor const &x, DTensor const &positions, DTensor const &angles) {
-  return x.num_dims == 3 && positive(x) && half_type(x) && row_major(x) && angles_ok(positions, angles, x.dim[0], x.dim[2]);
+  return x.num_dims == 3 && positive(x) && half_type(x) && row_major(x) && (long long)x.dim[1] * x.dim[2] <= 1 << 30 &&
+         angles_ok(positions, angles, x.dim[0], x.dim[2]);
 }
 
 // queries' heads of the projection; 0: infeasible
@@ -133,7 +134,7 @@ int append_q_heads(DTensor const &qkv, DTensor const &positions, DTensor const &
   }
   CacheShape const c(k, heads_first);
   int const heads = heads_in(qkv, c.head_dim);
-  if (heads <= 2 * c.kv_heads || !angles_ok(positions, angles, qkv.dim[0], c.head_dim) || !has_dims(slots, {qkv.dim[0]}) ||
+  if ((long long)heads <= 2LL * c.kv_heads || (long long)heads * c.head_dim > 1 << 30 || !angles_ok(positions, angles, qkv.dim[0], c.head_dim) || !has_dims(slots, {qkv.dim[0]}) ||
       slots.data_type != DT_INT32 || !row_major(slots) || qkv.data_ptr == k.data_ptr || qkv.data_ptr == v.data_ptr) {
     return 0;
   }
@@ -148,6 +149,13 @@ bool attention_ok(DTensor const &q, DTensor const &k, DTensor const &v, DTensor 
   CacheShape const c(k, heads_first);
   int const heads = heads_in(q, c.head_dim);
   if (heads == 0 || heads % c.kv_heads != 0 || c.head_dim % 8 != 0 || c.head_dim > MI355_MAX_PAGED_HEAD_DIM) {
+    return false;
+  }
+  // what mi355_paged_attention counts in 32 bits: places of a token, 16-byte steps into a cache, units of work of a sequence
+  long long const new_tokens = table.num_dims == 2 && positive(table) ? q.dim[0] / table.dim[0] : 0;
+  long long const keys = table.num_dims == 2 ? (long long)table.dim[1] * c.page_size : 0;
+  if (new_tokens * heads > 1 << 29 || keys > 1 << 30 || (long long)heads * c.head_dim > INT_MAX || (unsigned long long)k.num_elements() / 8 >= UINT_MAX ||
+      c.kv_heads * (new_tokens * (heads / c.kv_heads) / 16 + 1) * (keys / 128 + 2) > INT_MAX / 4) {
     return false;
   }
   return positive(q) && table.num_dims == 2 && positive(table) && table.data_type == DT_INT32 && row_major(table) && has_dims(lengths, {table.dim[0]}) &&

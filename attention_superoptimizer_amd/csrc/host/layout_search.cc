@@ -288,13 +288,26 @@ struct Searcher {
     }
     DmemLayout const before = op->output_tensors[ts_idx].layout;
     for (DmemLayout l : {DmemRowMajor, DmemColumnMajor}) {
-      if (op->op_type == KN_MATMUL_OP && l != DmemRowMajor) {
+      if (l != DmemRowMajor && (op->op_type == KN_MATMUL_OP || of_decoding(op, ts_idx))) {
         continue;
       }
       set_dtensor_layout(op_idx, ts_idx, l);
       walk(op_idx, ts_idx + 1, -1, -1);
     }
     set_dtensor_layout(op_idx, ts_idx, before);
+  }
+
+  // Operators of a decoding step read and write their tensors row by row, whatever a caller's cost says of other orders.
+  bool of_decoding(KNOperator const *op, int ts_idx) const {
+    bool is = mirage::kernel::is_decoding_op(op->op_type);
+    for (KNOperator const *other : g.operators) {
+      if (mirage::kernel::is_decoding_op(other->op_type)) {
+        for (DTensor const &t : other->input_tensors) {
+          is = is || t.guid == op->output_tensors[ts_idx].guid;
+        }
+      }
+    }
+    return is;
   }
 
   void apply_best() {

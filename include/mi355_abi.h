@@ -450,10 +450,11 @@ typedef struct mi355_paged_cache {
   long long page_stride, token_stride, head_stride;
   int type;
 } mi355_paged_cache;
+#define MI355_MAX_ROTARY_PAIRS 1024
 /* y = x with rotary positions, `heads` heads of head_dim elements in a row for every token, tokens x_stride and
  * y_stride apart: pair i < pairs of a head, elements (i, i + pairs) or, interleaved, (2i, 2i + 1), is turned by
  * positions[token] * angles[i] radians (computed in 64 bits) and scaled by angles[pairs + i]; the rest is copied.  y may
- * be x with the same stride. */
+ * be x with the same stride.  Up to MI355_MAX_ROTARY_PAIRS pairs and 2^30 elements a token. */
 int mi355_rotary(void const *x, long long x_stride, void *y, long long y_stride, int const *positions, double const *angles,
                  int tokens, int heads, int head_dim, int pairs, int interleaved, int type);
 /* The same for q_heads heads of q (results in q_out) and the cache's kv_heads heads of k, which go into the cache at

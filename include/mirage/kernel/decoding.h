@@ -19,7 +19,7 @@ class KNDecodingOp : public KNOperator {
 public:
   KNDecodingOp(mirage::type::KNOperatorType type, std::vector<DTensor> inputs);
   ~KNDecodingOp();
-  // false, and nothing run, where a layout search has declared one of the tensors column-major
+  // false, and nothing run, where a caller has declared one of the tensors column-major (a layout search does not)
   bool profile(ProfileResult &result) override;
   bool fingerprint(void) override { return false; }
   operator json() const override;

@@ -71,7 +71,7 @@ def test_rotary_append_refuses_one_tensor_as_both_caches(g):
 
 
 @pytest.mark.parametrize("change", [dict(x=(5, 64)), dict(kind=F32), dict(positions=(6,)), dict(angles=(2, 33)), dict(angles=(3, 8)),
-                                    dict(index=F16)])
+                                    dict(index=F16), dict(x=(5, 1, 4096), angles=(2, 1025))])
 def test_rotary_refuses(g, change):
     x = g.new_input(change.get("x", (5, 3, 64)), change.get("kind", F16))
     positions = g.new_input(change.get("positions", (5,)), change.get("index", I32))
@@ -84,7 +84,7 @@ def test_rotary_refuses(g, change):
     dict(q=(7, 8, 64)), dict(q=(6, 9, 64)), dict(q=(6, 8, 72)), dict(q=(6, 65)), dict(kind=BF16), dict(kind=F32, cache_kind=F32),
     dict(cache=(7, 16, 2, 60), q=(6, 8, 60)), dict(cache=(7, 16, 2, 264), q=(6, 8, 264)), dict(cache=(7, 16, 128)),
     dict(table=(3,)), dict(table=(4, 5)), dict(lengths=(2,)), dict(index=F32), dict(scale=math.inf), dict(scale=math.nan),
-    dict(window=-1),
+    dict(window=-1), dict(table=(3, 1 << 27)), dict(table=(3, 1 << 26), q=(6, 512, 64), cache=(7, 16, 256, 64)),
 ])
 def test_paged_attention_refuses(g, change):
     cache = change.get("cache", (7, 16, 2, 64))
@@ -250,3 +250,13 @@ def test_large_tensors_begin_with_a_cache_line():
         assert rt.mirage_arena_offset() == at
         g.close()
         assert rt.mirage_arena_offset() == base
+
+
+def test_layout_search_leaves_their_tensors_row_major(g):
+    """Whatever a cost says of column-major ones; the tensors of other operators are searched as before."""
+    x, y = g.new_input((4, 2, 64)), g.new_input((4, 64))
+    g.rotary(g.exp(x), g.new_input((4,), I32), g.new_input((2, 32), F64))
+    g.exp(y)
+    found = G.optimize_layout(g, lambda op, layouts: 1.0 + sum(1.0 for l in layouts if l == 100))
+    layouts = [[t.layout for t in g.outputs(i)] for i in range(g.num_operators)]
+    assert layouts == [[101], [101], [100], [100], [100], [100], [101]] and found["assignments"] == 8
