@@ -159,6 +159,11 @@ def test_more_heads_than_workgroups(rt, window):
     _check(18, lengths, new=2, kv_heads=8, group=2, window=window, page_size=32, kind="fp16")
 
 
+def test_a_page_a_sequence(rt):
+    """Pages of more keys than 16 bits count: a cache without paging."""
+    _check(19, [70100, 300, 0], kv_heads=1, group=2, page_size=70000, kind="bf16")
+
+
 def test_many_short_sequences(rt):
     rng = np.random.default_rng(2)
     _check(1, [int(n) for n in rng.integers(0, 60, 300)], kv_heads=4, group=2, kind="bf16")
