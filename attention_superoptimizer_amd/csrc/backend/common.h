@@ -112,12 +112,12 @@ struct State {
   // kTickets ints, zero whenever no launch that uses them runs.
   static constexpr int kTickets = 1 << 16;
   int *tickets = nullptr;
-  // Those of launches whose workgroups join parts of each other's results (paged_attention.hip): per queue three for each
+  // Those of launches whose workgroups join parts of each other's results (paged_attention.h): per queue five for each
   // of the most workgroups such a launch has, zero whenever none runs.  A line of memory each: those that share one are
   // drawn one after the other.
-  static constexpr int kJoinWorkgroups = 4096, kJoinStep = 32;
+  static constexpr int kJoinWorkgroups = 4096, kTicketsEach = 5, kJoinStep = 32;
   int *join_tickets = nullptr;
-  int *queue_join_tickets() const { return join_tickets + (size_t)3 * kJoinWorkgroups * kJoinStep * tls_queue; }
+  int *queue_join_tickets() const { return join_tickets + (size_t)kTicketsEach * kJoinWorkgroups * kJoinStep * tls_queue; }
 };
 
 State &state();

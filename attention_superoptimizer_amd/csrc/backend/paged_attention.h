@@ -8,7 +8,7 @@
 // * the work is cut into units of 128 keys (32 a wavefront, of which a workgroup has one, four or eight) of one sequence and key-value
 //   head.  Every head goes in equal parts to as many workgroups as its share of the chip is, or, where heads are more or
 //   shorter than that, units are dealt in equal runs that go on from one head to the next.  The parts of a head are joined
-//   by the last of its workgroups (a ticket), in the order of the keys; more than eight in two levels.
+//   by the last of its workgroups (a ticket), in the order of the keys; more than eight in levels.
 // * a wavefront has 32 keys at a time and streams them from the pages straight into LDS of its own: no barrier in the
 //   loop.  The next keys are on their way while the scores become weights, the next values while the next scores are made.
 //   Waits count the transfers of the younger tile; anything else in flight would only make them wait for more.
@@ -29,7 +29,7 @@ namespace paged {
 constexpr int kTile = 32;                 // keys of a wavefront at a time
 template <int WAVES>
 constexpr int kIdsOf = WAVES == 1 ? 256 : 1024;  // page numbers of a run that a workgroup holds in LDS
-constexpr int kAtOnce = 8;                // parts that a thread reads together; more are joined in two levels
+constexpr int kAtOnce = 8;                // parts that a thread reads together; more are joined in levels
 
 struct PagedParams {
   void const *q, *k, *v;
@@ -38,7 +38,7 @@ struct PagedParams {
   uint32_t page_step, token_step, head_step;  // in 16 bytes: a cache is up to 64 GB
   int const *table, *lengths;
   float *parts;   // 2 per workgroup: the end of a head that began before it, the beginning of one that goes on after it
-  int *tickets;   // 3 per workgroup, kJoinStep apart, zero between launches
+  int *tickets;   // kTicketsEach per workgroup, kJoinStep apart, zero between launches
   int pages, page_size, head_dim, table_width, sequences, new_tokens, group, window;
   int row_blocks, heads;  // of 16 RG rows, of a key-value head; key-value heads x row blocks
   unsigned page_magic, group_magic;  // see quotient
@@ -684,9 +684,9 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
         __syncthreads();
         return *is_last != 0;
       };
-      // Parts i0, i0 + step, .. (n of them), into the first of them or the result; kAtOnce of them are asked for together: a
-      // trip to the memory that all XCDs share is a microsecond.  A joined part's maximum and sum lie beside its own, which
-      // other threads may still be reading (level 0: its own, 2: the joined ones).
+      // Parts i0, i0 + step, .. (n of them), into the first of them or the result; they are asked for together: a trip to the
+      // memory that all XCDs share is a microsecond.  A joined part's maximum and sum go beside those it is made of, which
+      // other threads may still be reading (level 0 and 2: which of them are read).
       auto join = [&](int i0, int step, int n, int level, bool final) {
         constexpr int kItems = RG > 1 ? 2 : 1;
         int const items = rows * (DP / 4);
@@ -746,22 +746,32 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
             } else {
               store_shared(slot(i0) + row[k] * DP + d[k], x[k]);
               if (d[k] == 0) {
-                store_shared(slot(i0) + 16 * RG * DP + 4 * row[k] + 2, top[k], all_sum[k]);
+                store_shared(slot(i0) + 16 * RG * DP + 4 * row[k] + 2 - level, top[k], all_sum[k]);
               }
             }
           }
         }
       };
-      int const per = count > kAtOnce ? (int)ceilf(sqrtf((float)count)) : count;
-      int const of_group = index / per * per, in_group = count - of_group < per ? count - of_group : per;
-      if (arrive(P.tickets + State::kJoinStep * (3 * (w0 + of_group) + (of_group == 0 ? 0 : 1)), in_group)) {
-        join(of_group, 1, in_group, 0, per >= count);
-        if (per < count) {
-          int const groups = (count + per - 1) / per;
-          if (arrive(P.tickets + State::kJoinStep * (3 * w0 + 2), groups)) {
-            join(0, per, groups, 2, true);
-          }
+      // in one, two or three levels of groups of up to kAtOnce: a compute unit reads what others wrote at a few bytes a cycle
+      int per = count <= kAtOnce ? count : 2;
+      while ((count <= kAtOnce * kAtOnce ? per * per : per * per * per) < count) {
+        per++;
+      }
+      for (int at = index, left = count, step = 1, depth = 0;; depth++) {
+        int const group = at / per * per, n = left - group < per ? left - group : per;
+        bool const final = left <= per;
+        // (a workgroup may begin a group of the head that it goes on with, and those of the head that it begins)
+        int const ticket = State::kTicketsEach * (w0 + group * step) + (final ? 4 : 2 * depth + (group == 0 ? 0 : 1));
+        if (!arrive(P.tickets + State::kJoinStep * ticket, n)) {
+          break;
         }
+        join(group * step, step, n, depth % 2 * 2, final);
+        if (final) {
+          break;
+        }
+        at = group / per;
+        left = (left + per - 1) / per;
+        step *= per;
       }
     }
     unit += units;

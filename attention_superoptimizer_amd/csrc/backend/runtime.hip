@@ -211,7 +211,7 @@ extern "C" int mi355_init(size_t arena_bytes, void **arena_base) {
   MI355_HIP(hipMalloc(reinterpret_cast<void **>(&s.tickets), sizeof(int) * State::kTickets * MI355_NUM_QUEUES));
   MI355_HIP(hipMemset(s.tickets, 0, sizeof(int) * State::kTickets * MI355_NUM_QUEUES));
   forget_tickets();
-  size_t const join_bytes = sizeof(int) * 3 * State::kJoinWorkgroups * State::kJoinStep * MI355_NUM_QUEUES;
+  size_t const join_bytes = sizeof(int) * State::kTicketsEach * State::kJoinWorkgroups * State::kJoinStep * MI355_NUM_QUEUES;
   MI355_HIP(hipMalloc(reinterpret_cast<void **>(&s.join_tickets), join_bytes));
   MI355_HIP(hipMemset(s.join_tickets, 0, join_bytes));
   s.ready = true;
