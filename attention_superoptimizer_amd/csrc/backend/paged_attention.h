@@ -687,7 +687,8 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
       // Parts i0, i0 + step, .. (n of them), into the first of them or the result; they are asked for together: a trip to the
       // memory that all XCDs share is a microsecond.  A joined part's maximum and sum go beside those it is made of, which
       // other threads may still be reading (level 0 and 2: which of them are read).
-      auto join = [&](int i0, int step, int n, int level, bool final) {
+      auto join_by = [&](int i0, int step, int n, int level, bool final, auto at_once) {
+        constexpr int kBatch = decltype(at_once)::value;
         constexpr int kItems = RG > 1 ? 2 : 1;
         int const items = rows * (DP / 4);
         for (int first_item = tid; first_item < items; first_item += kItems * kThreads) {
@@ -703,10 +704,10 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
             all_sum[k] = 0.0f;
             x[k] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
           }
-          for (int j0 = 0; j0 < n; j0 += kAtOnce) {
-            uint64_t a[kItems][kAtOnce], b[kItems][kAtOnce], ms[kItems][kAtOnce];
+          for (int j0 = 0; j0 < n; j0 += kBatch) {
+            uint64_t a[kItems][kBatch], b[kItems][kBatch], ms[kItems][kBatch];
 #pragma unroll
-            for (int j = 0; j < kAtOnce; j++) {
+            for (int j = 0; j < kBatch; j++) {
               float const *const from = slot(i0 + (j0 + j < n ? j0 + j : n - 1) * step);
 #pragma unroll
               for (int k = 0; k < kItems; k++) {
@@ -716,14 +717,14 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
               }
             }
 #pragma unroll
-            for (int j = 0; j < kAtOnce; j++) {  // (read whether they count or not: under the condition each is a trip of its own)
+            for (int j = 0; j < kBatch; j++) {  // (read whether they count or not: under the condition each is a trip of its own)
 #pragma unroll
               for (int k = 0; k < kItems; k++) {
                 asm volatile("" : "+v"(a[k][j]), "+v"(b[k][j]), "+v"(ms[k][j]));
               }
             }
 #pragma unroll
-            for (int j = 0; j < kAtOnce; j++) {
+            for (int j = 0; j < kBatch; j++) {
               if (j0 + j < n) {
 #pragma unroll
                 for (int k = 0; k < kItems; k++) {
@@ -750,6 +751,15 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
               }
             }
           }
+        }
+      };
+      auto join = [&](int i0, int step, int n, int level, bool final) {  // (what is asked for past the last part is read all the same)
+        if (n <= 2) {
+          join_by(i0, step, n, level, final, std::integral_constant<int, 2>());
+        } else if (n <= 4) {
+          join_by(i0, step, n, level, final, std::integral_constant<int, 4>());
+        } else {
+          join_by(i0, step, n, level, final, std::integral_constant<int, kAtOnce>());
         }
       };
       // in one, two or three levels of groups of up to kAtOnce: a compute unit reads what others wrote at a few bytes a cycle
