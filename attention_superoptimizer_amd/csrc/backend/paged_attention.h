@@ -364,6 +364,9 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
         acc[r][d] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
       }
     }
+    // The greatest weight is 2^bias.  2^15 keeps small ones in two words of fp16, and its sums are far from the end of 32 bits.
+    // bf16 values reach that end themselves: n weights of at most 2^bias < 1 / 2n add up to less than a half.
+    float const bias = std::is_same<T, _Float16>::value ? 15.0f : (float)(__builtin_clz((unsigned)(span.to - span.first) | 1u) - 33);
     uint64_t const k_base = reinterpret_cast<uint64_t>(P.k) + 16ull * kv * P.head_step, v_base = reinterpret_cast<uint64_t>(P.v) + 16ull * kv * P.head_step;
 
     // as many units at a time as the page numbers in LDS cover
@@ -456,8 +459,8 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
           load(k_base, k_lds, Keys{});
         }
 
-        // weights, times 2^15 so that fp16 keeps small ones: two numbers of the value's type each -- one alone would put as
-        // much error into the result as rounding that does
+        // weights, as two numbers of the value's type each -- one alone would put as much error into the result as rounding
+        // that does
         bool const whole = is_there == ~0u && key >= all_least && key + kTile <= all_limit;
         uintx4 p[RG], rest[RG];
 #pragma unroll
@@ -488,7 +491,7 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
               acc[r][d] *= less;
             }
           }
-          float const base = m[r] == -INFINITY ? 0.0f : 15.0f - m[r] * P.scale;
+          float const base = m[r] == -INFINITY ? 0.0f : bias - m[r] * P.scale;
 #pragma unroll
           for (int e = 0; e < 8; e += 2) {
             float const w0 = exp2_fast(__builtin_fmaf(x[e], P.scale, base)), w1 = exp2_fast(__builtin_fmaf(x[e + 1], P.scale, base));
