@@ -142,19 +142,25 @@ __device__ __forceinline__ float over_groups(float x, Op op) {
 }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Two weights as two numbers of the value's type each, of which the second is what cutting the first short lost.
+// Two weights as two numbers of the value's type each, of which the second is what cutting the first short lost and a small
+// part of the first beside it, so that it is not zero: zero times an infinite value would be NaN where the sum is infinite.
+// All weights grow by that part alike (divided out at the end) but for what is cut off, a 2^-10 (2^-7) of one at most.
+template <class T>
+constexpr float kPart = std::is_same<T, _Float16>::value ? 0x1p-8f : 0x1p-12f;
 __device__ __forceinline__ void split(float w0, float w1, uint32_t &first, uint32_t &rest, _Float16) {
+  constexpr float back = kPart<_Float16> - 1.0f;
   auto const cut = __builtin_amdgcn_cvt_pkrtz(w0, w1);
-  auto const less = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(-1.0f, static_cast<float>(cut[0]), w0), __builtin_fmaf(-1.0f, static_cast<float>(cut[1]), w1));
+  auto const less = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(back, static_cast<float>(cut[0]), w0), __builtin_fmaf(back, static_cast<float>(cut[1]), w1));
   first = __builtin_bit_cast(uint32_t, cut);
   rest = __builtin_bit_cast(uint32_t, less);
 }
 __device__ __forceinline__ void split(float w0, float w1, uint32_t &first, uint32_t &rest, __bf16) {
+  constexpr float back = kPart<__bf16> - 1.0f;
   uint32_t const b0 = __builtin_bit_cast(uint32_t, w0), b1 = __builtin_bit_cast(uint32_t, w1);
   first = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
   typedef __bf16 pair __attribute__((ext_vector_type(2)));
-  pair const less = {static_cast<__bf16>(w0 - __builtin_bit_cast(float, b0 & 0xffff0000u)),
-                     static_cast<__bf16>(w1 - __builtin_bit_cast(float, b1 & 0xffff0000u))};
+  pair const less = {static_cast<__bf16>(__builtin_fmaf(back, __builtin_bit_cast(float, b0 & 0xffff0000u), w0)),
+                     static_cast<__bf16>(__builtin_fmaf(back, __builtin_bit_cast(float, b1 & 0xffff0000u), w1))};
   rest = __builtin_bit_cast(uint32_t, less);
 }
 
@@ -603,7 +609,7 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
     int const rows = R - row0 < 16 * RG ? R - row0 : 16 * RG;
     bool const alone = units == span.units;
     float *const mine = P.parts + (2 * (long long)me + (first == 0 ? 1 : 0)) * part_floats<DP, RG>();
-    auto of_sum = [](float all) { return all == 0.0f ? 0.0f : 1.0f / all; };
+    auto of_sum = [](float all) { return all == 0.0f ? 0.0f : 1.0f / (1.0f + kPart<T>) / all; };
     T *const out = static_cast<T *>(P.out) + (long long)sequence * P.new_tokens * P.out_stride + (long long)kv * P.group * P.head_dim;
     auto store_row = [&](int row, int d, floatx4 x, float by) {  // row of the head, columns d .. d + 3
       if (d < P.head_dim) {

@@ -304,7 +304,8 @@ class KNGraph:
         the keys before length - (new - 1 - t), of these the last `window` if that is not 0; a row that sees none, or
         only scores of minus infinity, is zeros.  Query head h reads key-value head h // (q_heads // kv_heads).  A page
         number outside the cache holds no keys, a length past the table counts as the table's.  What lies in places that a
-        row does not see never reaches it; a seen value that is no number leaves its column none.  scale: 1 /
+        row does not see never reaches it; a seen value that is infinite makes its column infinite, NaN beside one of the
+        other sign (either, where its weight is below 2^-30 of the row's greatest), a NaN makes it NaN.  scale: 1 /
         sqrt(head_dim) if not given."""
         if scale is None:
             scale = float(k_cache.dims[-1]) ** -0.5

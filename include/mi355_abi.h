@@ -467,7 +467,8 @@ int mi355_rotary_append(void const *q, long long q_stride, void const *k, long l
  * the pages table[sequence][0 .. table_width - 1] names: new token t sees the keys before L = lengths[sequence] -
  * (new_tokens - 1 - t), of these the last `window` where that is not 0.  A row without keys, or with scores of minus
  * infinity only, is zeros; a page number outside the cache holds no keys; a length past the table counts as the table's.
- * Values in places that a row does not see never reach it; a seen one that is no number leaves its column none.  Head sizes
+ * Values in places that a row does not see never reach it.  A seen one that is infinite makes its column infinite, NaN beside one of
+ * the other sign (where its weight is below 2^-30 of the row's greatest, either); a NaN makes it NaN.  Head sizes
  * are multiples of 8 up to MI355_MAX_PAGED_HEAD_DIM, q_heads one of kv_heads, strides multiples of 8, q, out, k and v 16-byte
  * aligned (a cache whose heads begin at multiples of 128 bytes is read up to a quarter faster), a table covers up to 2^30
  * keys, new_tokens * q_heads is up to 2^29, q_heads * head_dim below 2^31, out overlaps nothing that is read. */

@@ -53,7 +53,9 @@ public:
 // [sequences], the new tokens (whose keys are in the cache already) among them: new token t sees the keys before
 // L = length - (new - 1 - t), of these the last `window` where that is not 0.  Query head h reads key-value head
 // h / (q_heads / kv_heads).  A row that sees no key, or only scores of minus infinity, is zeros; a page number outside the cache holds no keys; a length
-// past the table counts as the table's.
+// past the table counts as the table's.  What lies in places that a row does not see never reaches it; a seen value that is
+// infinite makes its column infinite, NaN beside one of the other sign (either, where its weight is below 2^-30 of the row's
+// greatest); a NaN makes it NaN.
 class KNPagedAttentionOp : public KNDecodingOp {
 public:
   KNPagedAttentionOp(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table,
