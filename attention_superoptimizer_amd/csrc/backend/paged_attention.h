@@ -5,8 +5,8 @@
 //
 // Every key and value is read once for all rows of its head (query heads of the group x new tokens), so the bytes of
 // the cache bound a long call and the chain of trips to memory a short one.  What follows from that:
-// * the work is cut into units of 128 keys (32 a wavefront, of which a workgroup has one, four or eight) of one sequence and key-value
-//   head.  Every head goes in equal parts to as many workgroups as its share of the chip is, or, where heads are more or
+// * the work is cut into units of 32, 128 or 256 keys (32 a wavefront, of which a workgroup has one, four or eight) of one sequence and
+//   key-value head.  Every head goes in equal parts to as many workgroups as its share of the chip is, or, where heads are more or
 //   shorter than that, units are dealt in equal runs that go on from one head to the next.  The parts of a head are joined
 //   by the last of its workgroups (a ticket), in the order of the keys; more than eight in levels.
 // * a wavefront has 32 keys at a time and streams them from the pages straight into LDS of its own: no barrier in the
@@ -18,6 +18,7 @@
 
 #include "common.h"
 #include "mi355_kernels/kernarg.h"
+#include "mi355_kernels/paged_units.h"
 
 #include <climits>
 #include <cmath>
@@ -26,7 +27,6 @@
 namespace mi355 {
 namespace paged {
 
-constexpr int kTile = 32;                 // keys of a wavefront at a time
 template <int WAVES>
 constexpr int kIdsOf = WAVES == 1 ? 256 : 1024;  // page numbers of a run that a workgroup holds in LDS
 constexpr int kAtOnce = 8;                // parts that a thread reads together; more are joined in levels
@@ -849,7 +849,7 @@ int launch_group(PagedParams const &P, int kv_heads, bool passing) {
     long long const heads = (long long)P.sequences * kv_heads * ((P.new_tokens * P.group + 16 * RG - 1) / (16 * RG));
     long long const keys = (long long)P.table_width * P.page_size, units = heads * ((keys + 4 * kTile - 1) / (4 * kTile));
     if constexpr (RG == 1) {
-      if (heads >= 2048 && keys <= 512) {
+      if (one_wavefront(heads, P.new_tokens * P.group, keys)) {
         return passing ? launch_paged<T, DP, RG, 1, true>(P, kv_heads) : launch_paged<T, DP, RG, 1, false>(P, kv_heads);
       }
     }

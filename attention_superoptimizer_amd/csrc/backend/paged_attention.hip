@@ -96,11 +96,11 @@ extern "C" int mi355_paged_attention(void const *q, long long q_stride, void *ou
   long long const slots = (long long)sequences * keys < (long long)c.pages * c.page_size ? (long long)sequences * keys : (long long)c.pages * c.page_size;
   bool const passing = 4 * slots * c.kv_heads * c.head_dim > 192LL << 20;
   // units are counted in 32 bits: a batch with more of them goes in slices of sequences
-  long long const per_sequence = (long long)c.kv_heads * ((long long)new_tokens * P.group / 16 + 1) * (keys / (4 * kTile) + 2);
-  if (per_sequence > INT_MAX / 4) {
+  long long const rows = (long long)new_tokens * P.group;
+  if (too_many_units(c.kv_heads, rows, keys)) {
     return fail(MI355_ERR_UNSUPPORTED, "mi355_paged_attention: %d new tokens of %d heads over %lld keys", new_tokens, q_heads, keys);
   }
-  long long const slice = INT_MAX / 2 / per_sequence;
+  long long const slice = sequences_at_once(c.kv_heads, rows, keys);
   for (long long at = 0; at < sequences; at += slice) {
     P.sequences = (int)(sequences - at < slice ? sequences - at : slice);
     P.q = static_cast<char const *>(q) + 2 * at * new_tokens * q_stride;

@@ -1,6 +1,7 @@
 // Operators of a decoding step (include/mirage/kernel/decoding.h): what they take, their results' tensors, and the
 // calls of the C ABI that run them.
 #include "mi355_abi.h"
+#include "mi355_kernels/paged_units.h"
 #include "mirage/kernel/device_memory_manager.h"
 #include "mirage/kernel/graph.h"
 #include "mirage/utils/hip_types.h"
@@ -155,7 +156,7 @@ bool attention_ok(DTensor const &q, DTensor const &k, DTensor const &v, DTensor 
   long long const new_tokens = table.num_dims == 2 && positive(table) ? q.dim[0] / table.dim[0] : 0;
   long long const keys = table.num_dims == 2 ? (long long)table.dim[1] * c.page_size : 0;
   if (new_tokens * heads > 1 << 29 || keys > 1 << 30 || (long long)heads * c.head_dim > INT_MAX || (unsigned long long)k.num_elements() / 8 >= UINT_MAX ||
-      c.kv_heads * (new_tokens * (heads / c.kv_heads) / 16 + 1) * (keys / 128 + 2) > INT_MAX / 4) {
+      mi355::paged::too_many_units(c.kv_heads, new_tokens * (heads / c.kv_heads), keys)) {
     return false;
   }
   return positive(q) && table.num_dims == 2 && positive(table) && table.data_type == DT_INT32 && row_major(table) && has_dims(lengths, {table.dim[0]}) &&
