@@ -60,6 +60,23 @@ std::vector<DTensor> graph_outputs(kernel::Graph const &g) {
   return outs;
 }
 
+static bool has_fingerprint(KNOperator const *op) {
+  if (!kernel::is_decoding_op(op->op_type)) {
+    return true;
+  }
+  std::fprintf(stderr, "mirage: %s has no fingerprint\n", mirage::type::to_string(op->op_type));
+  return false;
+}
+
+bool has_fingerprints(kernel::Graph const &g) {
+  for (KNOperator const *op : g.operators) {
+    if (!has_fingerprint(op)) {
+      return false;
+    }
+  }
+  return true;
+}
+
 static void account(KNOperator const *op, VerifyStats *stats) {
   if (stats == nullptr) {
     return;
@@ -125,6 +142,7 @@ static void fill_inputs(std::vector<kernel::Graph const *> const &graphs, uint64
 }
 
 void fingerprint_graph(kernel::Graph const &g, uint64_t input_seed, VerifyStats *stats) {
+  MIRAGE_CHECK(has_fingerprints(g), "fingerprint_graph: an operator has no fingerprint");
   fill_inputs({&g}, input_seed);
   for (KNOperator *op : g.operators) {
     account(op, stats);
@@ -514,6 +532,14 @@ void set_verify_queues_per_batch(int queues) {
 VerifyTicket *verify_batch_begin(std::vector<kernel::Graph *> const &candidates,
                                  std::vector<DTensor> const &reference_outputs,
                                  uint64_t input_seed, kernel::Graph *reference_to_fingerprint) {
+  bool all = reference_to_fingerprint == nullptr || has_fingerprints(*reference_to_fingerprint);
+  for (kernel::Graph const *g : candidates) {
+    all = all && has_fingerprints(*g);
+  }
+  for (DTensor const &t : reference_outputs) {
+    all = all && (t.owner_op == nullptr || has_fingerprint(t.owner_op));
+  }
+  MIRAGE_CHECK(all, "verify_batch: an operator has no fingerprint");
   kernel::require_device("verify_batch");
   std::unique_ptr<VerifyTicket> t(new VerifyTicket);
   t->t_begin = std::chrono::steady_clock::now();
@@ -713,16 +739,9 @@ static void export_stats(mirage::search::VerifyStats const &s, mirage_verify_sta
   }
 }
 
-// Whether every operator of the graph has a fingerprint (decoding.h: some have none).  The calls below refuse one
-// that has not: its verdict would be about values nobody computed.
+// The calls below return an error for a graph that the functions they are for abort on.
 static bool has_fingerprints(void const *graph) {
-  for (mirage::kernel::KNOperator const *op : static_cast<mirage::kernel::Graph const *>(graph)->operators) {
-    if (mirage::kernel::is_decoding_op(op->op_type)) {
-      std::fprintf(stderr, "mirage: %s has no fingerprint\n", mirage::type::to_string(op->op_type));
-      return false;
-    }
-  }
-  return true;
+  return mirage::search::has_fingerprints(*static_cast<mirage::kernel::Graph const *>(graph));
 }
 static bool have_fingerprints(void *const *graphs, int n, void const *reference) {
   bool all = has_fingerprints(reference);

@@ -21,6 +21,11 @@ namespace search {
 // (search.cc:580-593: `num_consumers[i] == 0`).
 std::vector<mirage::kernel::DTensor> graph_outputs(mirage::kernel::Graph const &g);
 
+// Whether every operator of `g` has a fingerprint (those of a decoding step, kernel/decoding.h, have none; one that
+// has not is named on stderr).  The functions below abort on a graph of which this is false, as on outputs of such
+// an operator: their verdict would be about values nobody computed.
+bool has_fingerprints(mirage::kernel::Graph const &g);
+
 struct VerifyStats {
   int kernel_ops = 0;         // operators fingerprinted (inputs included)
   int customized_ops = 0;     // of which customized
