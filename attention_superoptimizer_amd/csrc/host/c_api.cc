@@ -19,8 +19,9 @@ using kernel::KNOperator;
 
 namespace mirage {
 namespace kernel {
-void execute_once(KNOperator *op);
-void execute_all(Graph const &graph);
+char const *without_kernel(KNOperator const &op);
+char const *execute_once(KNOperator *op);
+char const *execute_all(Graph const &graph, KNOperator const **missing);
 }
 }  // namespace mirage
 
@@ -145,15 +146,23 @@ float mirage_op_profile(void *g, int idx) {
   return r.run_time;
 }
 
-int mirage_op_execute(void *g, int idx) {
-  kernel::execute_once(static_cast<kernel::Graph *>(g)->operators.at(idx));
-  return 0;
+static int refused(KNOperator const *op, char const *why) {
+  std::fprintf(stderr, "mirage: %s: %s\n", type::to_string(op->op_type), why);
+  return -1;
 }
 
-// every operator in order
+// -1, and nothing run, where no kernel computes what a tensor is declared as (its type, a storage order)
+int mirage_op_execute(void *g, int idx) {
+  KNOperator *op = static_cast<kernel::Graph *>(g)->operators.at(idx);
+  char const *const why = kernel::execute_once(op);
+  return why == nullptr ? 0 : refused(op, why);
+}
+
+// every operator in order; -1 as above
 int mirage_graph_execute(void *g) {
-  kernel::execute_all(*static_cast<kernel::Graph *>(g));
-  return 0;
+  KNOperator const *missing = nullptr;
+  char const *const why = kernel::execute_all(*static_cast<kernel::Graph *>(g), &missing);
+  return why == nullptr ? 0 : refused(missing, why);
 }
 
 // the lowered program of a customized op, as handed to the backend
@@ -230,8 +239,14 @@ int mirage_tensor_same_fingerprint(void *a, void *b) {
   return static_cast<DTensor *>(a)->has_same_fingerprint(*static_cast<DTensor *>(b)) ? 1 : 0;
 }
 
-// Graph::generate_hip_program
+// Graph::generate_hip_program; -1 where a customized operator has values of another type than its kernels'
 int mirage_graph_generate_hip_program(void *g, char const *path) {
+  for (KNOperator const *op : static_cast<kernel::Graph *>(g)->operators) {
+    char const *const why = op->op_type == type::KN_CUSTOMIZED_OP ? kernel::without_kernel(*op) : nullptr;
+    if (why != nullptr) {
+      return refused(op, why);
+    }
+  }
   static_cast<kernel::Graph *>(g)->generate_hip_program(path);
   return 0;
 }

@@ -18,6 +18,8 @@ using namespace mirage::type;
 
 #define MI355_CALL(expr) MIRAGE_CHECK((expr) == MI355_OK, mi355_last_error())
 
+char const *without_kernel(KNOperator const &op);  // (kernel_device.cc)
+
 namespace {
 
 bool row_major(DTensor const &t) { return t.layout == mirage::layout::DmemRowMajor; }
@@ -217,14 +219,11 @@ KNDecodingOp::operator json() const {
 }
 
 bool KNDecodingOp::profile(ProfileResult &result) {
-  require_device("KNDecodingOp::profile");
-  for (auto const *tensors : {&input_tensors, &output_tensors}) {
-    for (DTensor const &t : *tensors) {
-      if (!row_major(t)) {
-        return false;
-      }
-    }
+  if (without_kernel(*this) != nullptr) {
+    result = ProfileResult::infinity();
+    return false;
   }
+  require_device("KNDecodingOp::profile");
   int const iters = 16;
   run();
   MI355_CALL(mi355_timer_start());

@@ -24,6 +24,37 @@ using namespace mirage::type;
 
 #define MI355_CALL(expr) MIRAGE_CHECK((expr) == MI355_OK, mi355_last_error())
 
+// ---- what has no kernel --------------------------------------------------------------
+// Null, or why the values of `op` cannot be computed as its tensors are declared: the operators of a decoding step have
+// types of their own and row-major tensors (a caller may have declared them otherwise since), all others compute fp16.
+// Fingerprints know no type, so such operators can be built.
+char const *without_kernel(KNOperator const &op) {
+  if (is_decoding_op(op.op_type)) {
+    for (auto const *tensors : {&op.input_tensors, &op.output_tensors}) {
+      for (DTensor const &t : *tensors) {
+        if (t.layout != mirage::layout::DmemRowMajor) {
+          return "an operator of a decoding step takes row-major tensors";
+        }
+      }
+    }
+    return nullptr;
+  }
+  for (DTensor const &t : op.input_tensors) {
+    if (t.data_type != DT_FLOAT16) {
+      return "the operator computes fp16 values, of fp16 inputs";
+    }
+  }
+  return nullptr;
+}
+
+static bool no_profile(KNOperator const &op, ProfileResult &result) {
+  if (without_kernel(op) == nullptr) {
+    return false;
+  }
+  result = ProfileResult::infinity();
+  return true;
+}
+
 // ---- compare (reference src/kernel/cuda/device_tensor_kernel.cu:22-53) ---------------
 bool DTensor::has_same_fingerprint(DTensor const &ref) const {
   if (data_type != ref.data_type || layout != ref.layout || num_dims != ref.num_dims) {
@@ -171,6 +202,9 @@ static void on_row_major(std::vector<DTensor> const &inputs, DTensor const &outp
 }
 
 bool KNMatmulOp::profile(ProfileResult &result) {
+  if (no_profile(*this, result)) {
+    return false;
+  }
   require_device("KNMatmulOp::profile");
   int batch, m, n, k;
   matmul_extents(input_tensors[0], input_tensors[1], batch, m, n, k);
@@ -213,6 +247,9 @@ static void run_unary(mirage::type::KNOperatorType type, std::vector<DTensor> co
 }
 
 bool KNElementUnaryOp::profile(ProfileResult &result) {
+  if (no_profile(*this, result)) {
+    return false;
+  }
   require_device("KNElementUnaryOp::profile");
   size_t const n = input_tensors[0].num_elements();
   int const iters = ProfileResult::NUM_ITERATIONS;
@@ -237,6 +274,9 @@ bool KNElementUnaryOp::fingerprint(void) {
 
 // ---- element-wise binary (reference src/kernel/cuda/element_binary_kernel.cu:53-199) -----
 bool KNElementBinaryOp::profile(ProfileResult &result) {
+  if (no_profile(*this, result)) {
+    return false;
+  }
   require_device("KNElementBinaryOp::profile");
   DTensor const &a = input_tensors[0], &b = input_tensors[1], &o = output_tensors[0];
   int const iters = 16;
@@ -275,6 +315,9 @@ static void reduction_strides(DTensor const &in, DTensor const &out, int dim, in
 }
 
 bool KNReductionOp::profile(ProfileResult &result) {
+  if (no_profile(*this, result)) {
+    return false;
+  }
   require_device("KNReductionOp::profile");
   int factor, is, os;
   reduction_strides(input_tensors[0], output_tensors[0], reduction_dim_idx, factor, is, os);
@@ -408,11 +451,17 @@ void KNCustomizedOp::launch(bool fingerprint) {
 }
 
 void KNCustomizedOp::run() {
+  char const *const why = without_kernel(*this);
+  MIRAGE_CHECK(why == nullptr, why);
   require_device("KNCustomizedOp::run");
   launch(false);
 }
 
 void KNCustomizedOp::run_with(KNCustomizedOp &next) {
+  for (KNOperator const *op : {this, &next}) {
+    char const *const why = without_kernel(*op);
+    MIRAGE_CHECK(why == nullptr, why);
+  }
   require_device("KNCustomizedOp::run_with");
   LoweredOp const l = lower_unchecked(*this, false), n = lower_unchecked(next, false);
   static_assert(sizeof(kept_two) / sizeof(kept_two[0]) == MI355_NUM_QUEUES, "per queue");
@@ -430,6 +479,9 @@ void KNCustomizedOp::run_with(KNCustomizedOp &next) {
 }
 
 bool KNCustomizedOp::profile(ProfileResult &result) {
+  if (no_profile(*this, result)) {
+    return false;
+  }
   require_device("KNCustomizedOp::profile");
   LoweredOp l = lower(*this, false);
   float ms = 0.0f;
@@ -483,6 +535,8 @@ void Graph::generate_hip_program(char const *file_path) {
     if (op->op_type != mirage::type::KN_CUSTOMIZED_OP) {
       continue;  // as the reference: only customized operators are emitted
     }
+    char const *const why = without_kernel(*op);
+    MIRAGE_CHECK(why == nullptr, why);
     LoweredOp l = lower(*static_cast<KNCustomizedOp *>(op), false);
     std::string const name = "graphdef_kernel_" + std::to_string(kernels++);
     long long const n = mi355_emit_hip_kernel(&l.plan, name.c_str(), 0, nullptr, 0);
@@ -578,7 +632,11 @@ int main() {
 namespace mirage {
 namespace kernel {
 
-void execute_once(KNOperator *op) {
+// (null, or why the operator cannot be executed)
+char const *execute_once(KNOperator *op) {
+  if (char const *why = without_kernel(*op)) {
+    return why;
+  }
   require_device("execute_once");
   using namespace mirage::type;
   switch (op->op_type) {
@@ -631,6 +689,7 @@ void execute_once(KNOperator *op) {
     default:
       MIRAGE_CHECK(false, "operator cannot be executed");
   }
+  return nullptr;
 }
 
 // ---- a whole graph: neighbouring kernel-level operators that one launch can run ------------------
@@ -831,9 +890,16 @@ static size_t run_two_matmuls(std::vector<KNOperator *> const &ops, size_t i) {
   return taken != 0 ? at - i : 0;
 }
 
-void execute_all(Graph const &graph) {
-  require_device("execute_all");
+// (null, or why `missing`, one of its operators, cannot be executed: then none has been)
+char const *execute_all(Graph const &graph, KNOperator const **missing) {
   std::vector<KNOperator *> const &ops = graph.operators;
+  for (KNOperator const *op : ops) {
+    if (char const *why = without_kernel(*op)) {
+      *missing = op;
+      return why;
+    }
+  }
+  require_device("execute_all");
   size_t const n = ops.size();
   auto softmax_at = [&](size_t i) {
     return i + 2 < n && is_softmax_rows(ops[i], ops[i + 1], ops[i + 2]) && !column_major(ops[i]->input_tensors[0]) &&
@@ -857,6 +923,7 @@ void execute_all(Graph const &graph) {
       i += 1;
     }
   }
+  return nullptr;
 }
 
 }  // namespace kernel

@@ -359,8 +359,10 @@ class KNGraph:
         assert self._rt.mirage_op_execute(self._g, idx) == 0
 
     def execute_all(self) -> None:
-        """One fp16 run of every operator, in order (one call into the runtime: a ctypes call per
-        operator is a microsecond each)."""
+        """One run of every operator, in order (one call into the runtime: a ctypes call per
+        operator is a microsecond each).  Matmuls, element-wise operators, reductions and customized
+        operators compute fp16 values; with inputs of another type nothing is run (an AssertionError,
+        the reason on stderr), and `profile` gives them the 1000 ms of what has no kernel."""
         assert self._rt.mirage_graph_execute(self._g) == 0
 
     def profile(self, idx: int) -> float:
