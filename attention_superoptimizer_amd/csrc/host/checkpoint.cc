@@ -82,13 +82,16 @@ Checkpoint load_checkpoint_file(std::string const &path) {
 
 GraphProfile profile_graph(mirage::kernel::Graph &g) {
   GraphProfile out;
+  bool const kept = g.keeps_inputs();
   for (auto *op : g.operators) {
     op->fingerprint();
   }
   for (auto *op : g.operators) {
     ProfileResult r;
     r.run_time = 0.0f;
-    op->profile(r);
+    if (!kept || op->op_type != mirage::type::KN_INPUT_OP) {
+      op->profile(r);
+    }
     out.op_ms.push_back(r.run_time);
     out.run_time += r.run_time;
   }

@@ -209,6 +209,15 @@ DTensor push(std::vector<KNOperator *> &ops, KNOperator *op, char const *what) {
 
 bool is_decoding_op(KNOperatorType type) { return type >= KN_ROTARY_OP && type <= KN_VERIFY_DRAFTS_OP; }
 
+bool Graph::keeps_inputs() const {
+  for (KNOperator const *op : operators) {
+    if (is_decoding_op(op->op_type)) {
+      return true;
+    }
+  }
+  return false;
+}
+
 KNDecodingOp::KNDecodingOp(KNOperatorType type, std::vector<DTensor> inputs) : KNOperator(type, std::move(inputs)) {}
 KNDecodingOp::~KNDecodingOp() { release_outputs(); }
 

@@ -75,7 +75,7 @@ bool DTensor::has_same_fingerprint(DTensor const &ref) const {
 bool KNInputOp::profile(ProfileResult &profile) {
   require_device("KNInputOp::profile");
   DTensor const &t = output_tensors[0];
-  if (t.data_type != DT_FLOAT16) {  // (page tables, positions, probabilities: they keep what the caller wrote)
+  if (t.data_type != DT_FLOAT16) {  // (no operator that computes from filled inputs takes other types)
     profile.run_time = 0.0f;
     return true;
   }

@@ -203,6 +203,8 @@ struct Searcher {
     float ms;
     if (cfg.cost) {
       ms = cfg.cost(op);
+    } else if (op->op_type == KN_INPUT_OP && g.keeps_inputs()) {
+      ms = 0.0f;
     } else {
       ProfileResult r;
       bool const ran = op->profile(r);

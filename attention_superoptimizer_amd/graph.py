@@ -366,13 +366,14 @@ class KNGraph:
         assert self._rt.mirage_graph_execute(self._g) == 0
 
     def profile(self, idx: int) -> float:
-        """Mean milliseconds per launch (reference profile() protocol)."""
+        """Mean milliseconds per launch (reference profile() protocol).  Inputs are filled with a
+        pattern, but for those of a graph with operators of a decoding step, which keep their values."""
         return float(self._rt.mirage_op_profile(self._g, idx))
 
     def profile_all(self):
         """What the reference's cpp_examples/profile.cc does with a graph (:25-34):
-        fingerprint() of every operator, then profile() of every operator.  Returns
-        (sum of the mean milliseconds per launch, per-operator list)."""
+        fingerprint() of every operator, then profile() of every operator (which fills inputs, or
+        keeps them, as `profile`).  Returns (sum of the mean milliseconds per launch, per-operator list)."""
         n = self.num_operators
         per_op = (ctypes.c_float * n)()
         total = float(self._rt.mirage_graph_profile(self._g, per_op, n))

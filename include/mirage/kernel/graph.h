@@ -75,6 +75,10 @@ public:
   KNOperator *create_verify_drafts_op(DTensor const &target, DTensor const *draft, DTensor const &tokens,
                                       DTensor const &uniforms);
 
+  // Whether the graph has an operator of a decoding step.  Its inputs are then what a program serves from -- caches,
+  // page tables, weights -- and profiles and layout searches leave them as they are (inputs of others are filled).
+  bool keeps_inputs() const;
+
   // Writes a self-contained HIP program for gfx950: one specialised kernel per
   // customized operator, a launcher over all of them and a main() that fills the
   // tensors with random values and times the launcher (the role of the reference's

@@ -46,7 +46,8 @@ struct GraphProfile {
 };
 
 // cpp_examples/profile.cc:25-34: fingerprint() of every operator, then profile() of every
-// operator (ProfileResult's 1024 + 1024 launches each), run times summed.
+// operator (ProfileResult's 1024 + 1024 launches each), run times summed.  Inputs are filled first, but for a graph
+// that keeps them.
 GraphProfile profile_graph(mirage::kernel::Graph &g);
 
 }  // namespace search
