@@ -262,8 +262,9 @@ size_t mirage_get_smem_budget(void) { return threadblock::Graph::smem_budget(); 
 int mirage_device_ready(void) {
   return kernel::DeviceMemoryManager::get_instance()->device_ready ? 1 : 0;
 }
+// bytes of the arena's total that are taken
 long long mirage_arena_offset(void) {
-  return (long long)kernel::DeviceMemoryManager::get_instance()->offset;
+  return (long long)kernel::DeviceMemoryManager::get_instance()->used();
 }
 long long mirage_arena_total(void) {
   return (long long)kernel::DeviceMemoryManager::get_instance()->total_size;

@@ -53,11 +53,10 @@ bool room_for(std::initializer_list<size_t> data_bytes, std::initializer_list<si
   size_t need = 0;
   for (auto const &list : {data_bytes, fingerprint_bytes}) {
     for (size_t b : list) {
-      need += (b + 15) / 16 * 16 + 256;  // (a large tensor may skip to a cache line)
+      need += (b + 15) / 16 * 16;
     }
   }
-  DeviceMemoryManager *dmm = DeviceMemoryManager::get_instance();
-  return need <= dmm->total_size - (size_t)dmm->offset;
+  return DeviceMemoryManager::get_instance()->has_room(need);
 }
 bool room_for(DTensor const &t) { return room_for({t.data_size()}, {t.fingerprint_size()}); }
 

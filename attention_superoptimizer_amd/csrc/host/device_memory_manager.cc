@@ -13,17 +13,21 @@ namespace kernel {
 DeviceMemoryManager *DeviceMemoryManager::singleton = nullptr;
 
 static size_t round16(size_t n) { return (n + 15) / 16 * 16; }
-static constexpr size_t kLine = 256, kLinesFrom = 1 << 20;  // two cache lines; tensors of so many bytes
+// A tensor of a megabyte and more begins at two cache lines: attention over 537 MB of cached keys and values whose rows lie
+// across lines takes 118 us, 95 from their beginning.  What that skips (given back with the tensor) lies in a margin of the
+// allocation beside the arena's size, room for as many such tensors as fit it.
+static constexpr size_t kLine = 256, kLinesFrom = 1 << 20;
+static size_t margin_of(size_t total) { return total / kLinesFrom * kLine; }
 
 DeviceMemoryManager::DeviceMemoryManager()
-    : base_ptr(nullptr), offset(0), total_size((size_t)10 * 1024 * 1024 * 1024),
+    : base_ptr(nullptr), offset(0), skipped(0), total_size((size_t)10 * 1024 * 1024 * 1024),
       exp_lookup_table(nullptr), div_p_lookup_table(nullptr), div_q_lookup_table(nullptr),
       device_ready(false) {
   if (char const *env = std::getenv("MIRAGE_ARENA_BYTES")) {
     total_size = std::strtoull(env, nullptr, 10);
   }
   void *base = nullptr;
-  int rc = mi355_init(total_size, &base);
+  int rc = mi355_init(total_size + margin_of(total_size), &base);
   if (rc == MI355_OK) {
     base_ptr = static_cast<char *>(base);
     void const *e = nullptr, *p = nullptr, *q = nullptr;
@@ -53,15 +57,11 @@ DeviceMemoryManager::~DeviceMemoryManager() {
 bool DeviceMemoryManager::allocate(DTensor &tensor, bool allocate_fingerprint) {
   MIRAGE_CHECK(offset % 16 == 0, "arena offset lost its alignment");
   size_t bytes = round16(tensor.data_size());
-  // A large tensor begins with a cache line, where there is room for what that skips (given back with the tensor): attention over
-  // 537 MB of cached keys and values whose rows lie across lines takes 118 us, 95 from their beginning.
-  size_t skipped = bytes >= kLinesFrom ? (kLine - reinterpret_cast<uintptr_t>(base_ptr + offset) % kLine) % kLine : 0;
-  if (offset + skipped + bytes + (allocate_fingerprint ? round16(tensor.fingerprint_size()) : 0) > total_size) {
-    skipped = 0;
-  }
-  offset += skipped;
+  size_t const skip = bytes >= kLinesFrom ? (kLine - reinterpret_cast<uintptr_t>(base_ptr + offset) % kLine) % kLine : 0;
+  offset += skip;
+  skipped += skip;
   tensor.data_ptr = base_ptr + offset;
-  allocated_tensors.push_back({tensor.data_ptr, skipped + bytes});
+  allocated_tensors.push_back({tensor.data_ptr, bytes});
   offset += bytes;
   tensor.fp_ptr = nullptr;
   if (allocate_fingerprint) {
@@ -70,7 +70,7 @@ bool DeviceMemoryManager::allocate(DTensor &tensor, bool allocate_fingerprint) {
     allocated_tensors.push_back({tensor.fp_ptr, bytes});
     offset += bytes;
   }
-  MIRAGE_CHECK((size_t)offset <= total_size, "device arena exhausted");
+  MIRAGE_CHECK(has_room(0), "device arena exhausted");
   return true;
 }
 
@@ -86,6 +86,11 @@ bool DeviceMemoryManager::free(DTensor &tensor) {
                "tensors must be freed in reverse allocation order");
   offset -= allocated_tensors.back().second;
   allocated_tensors.pop_back();
+  // what was skipped before it: back to the end of the tensor below
+  char const *const end = allocated_tensors.empty() ? base_ptr : static_cast<char *>(allocated_tensors.back().first) + allocated_tensors.back().second;
+  size_t const skip = (size_t)(base_ptr + offset - end);
+  offset -= skip;
+  skipped -= skip;
   return true;
 }
 

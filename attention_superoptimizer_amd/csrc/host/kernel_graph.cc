@@ -32,8 +32,7 @@ void KNOperator::release_outputs() {
 }
 
 static bool arena_has_room(size_t bytes) {
-  DeviceMemoryManager *dmm = DeviceMemoryManager::get_instance();
-  return (size_t)dmm->offset + bytes <= dmm->total_size;
+  return DeviceMemoryManager::get_instance()->has_room(bytes);
 }
 
 static void adopt_output(KNOperator *op, DTensor &t) {

@@ -1,7 +1,8 @@
 // Process-wide device arena (reference include/mirage/kernel/device_memory_manager.h:28-53):
 // one allocation made by the backend at first use, handed out by a bump pointer
 // and returned strictly last-in-first-out.  Every tensor gets a data buffer and
-// a fingerprint buffer, each rounded to 16 bytes.  Default size 10 GiB
+// a fingerprint buffer, each rounded to 16 bytes; data of a megabyte and more begins
+// at a multiple of 256 bytes, which takes nothing of the arena's size.  Default size 10 GiB
 // (environment MIRAGE_ARENA_BYTES overrides).  With MIRAGE_HOST_ONLY=1 and no
 // GPU the manager hands out addresses only, so graph construction and plan
 // lowering can be exercised on a CPU-only machine; any device work then aborts.
@@ -23,9 +24,12 @@ public:
   bool allocate(DTensor &tensor, bool allocate_fingerprint = true);
   bool free(DTensor &tensor);
   static DeviceMemoryManager *get_instance();
+  size_t used() const { return (size_t)offset - skipped; }
+  bool has_room(size_t bytes) const { return used() <= total_size && bytes <= total_size - used(); }
 
   char *base_ptr;
   off_t offset;
+  size_t skipped;  // of offset, what the beginnings of large tensors skipped
   size_t total_size;
   std::vector<std::pair<void *, size_t>> allocated_tensors;
   // device copies of the fingerprint lookup tables (owned by the backend)
