@@ -839,7 +839,11 @@ int launch_paged(PagedParams P, int kv_heads) {
 // to read, or all of them more than the caches keep: measured (us, four and eight) 99.7 and 95.7 of 1 sequence x 8 heads x
 // 131072 keys, 98.7 and 94.7 of 64 x 8 x 4096, 12.8 and 11.2 of 4 x 8 x 2000, 47.3 and 38.3 of 16 x 4 x 8192 with 32 rows; against it
 // 8.8 and 10.4 of 8 x 8 x 500, 32.9 and 38.9 of 128 x 8 x 500, 31.6 and 34.8 of 16 x 8 x 4096, 181 and 222 of 1024 x 8 x 400, and heads
-// of 64, of which less is on its way: 37.9 and 41.0 of 47 x 5 x 6280.
+// of 64, of which less is on its way: 37.9 and 41.0 of 47 x 5 x 6280.  With 17 - 48 rows more heads gain, the fewer their keys are
+// (us, four and eight, 40 rows of heads of 64): 25.7 and 20.8 of 32 heads x up to 8000 keys, 54.9 and 52.4 of 48 x 30000, 24.8 and 17.9 of
+// 96 x 2500, 15.0 and 13.0 of 256 x 500; against it 32.8 and 49.4 of 96 x 8000, 26.2 and 36.9 of 128 x 4000, 21.3 and 31.0 of 256 x 1500,
+// 21.6 and 25.4 of 384 x 500.  With 20 rows of heads of 128 the limits lie where these do: 31.2 and 27.7 of 96 x 4000, 17.7 and 15.4 of
+// 256 x 500; 37.3 and 40.7 of 128 x 4000, 28.6 and 33.5 of 256 x 1500.
 // Eight workgroups of one wavefront for thousands of heads that are short: no wavefront waits for another at a head's end (four
 // and one: 93 and 74 us of 1024 sequences x 8 heads x 100 keys, 355 and 244 of 4096 x 8 x 100, 181 and 177 of 1024 x 8 x 400;
 // against it 98 and 104 of 64 x 8 x 4096, 33.4 and 33.2 of 128 x 8 x 500, 7.7 and 11.4 of 64 x 8 x 100).
@@ -858,7 +862,8 @@ int launch_group(PagedParams const &P, int kv_heads, bool passing) {
         return launch_paged<T, DP, RG, (DP <= 64 ? 4 : 8), true>(P, kv_heads);
       }
     }
-    if (heads <= (RG == 1 ? 96 : 256) && units >= 512) {
+    bool const few = RG == 1 ? heads <= 96 : heads <= 48 || (heads <= 256 && heads * units <= 300 << 10);
+    if (few && units >= 512) {
       return launch_paged<T, DP, RG, 8, false>(P, kv_heads);
     }
   }
