@@ -144,6 +144,9 @@ int rotary(RotaryParams const &P, int interleaved, int type) {
     return fail(MI355_ERR_INVALID, "rotary: a stride below zero, or results of %d heads of %d that lie %lld apart", P.q_heads, P.head_dim,
                 P.out_stride);
   }
+  if (P.src[0] == P.q_out && P.src_stride[0] != P.out_stride && P.tokens > 1) {  // a token's results would lie on another's queries
+    return fail(MI355_ERR_INVALID, "rotary: in place the strides are the same, not %lld and %lld", P.src_stride[0], P.out_stride);
+  }
   if (type != MI355_TYPE_F16 && type != MI355_TYPE_BF16) {
     return fail(MI355_ERR_UNSUPPORTED, "rotary: type %d", type);
   }
@@ -164,9 +167,6 @@ using namespace mi355;
 extern "C" int mi355_rotary(void const *x, long long x_stride, void *y, long long y_stride, int const *positions,
                             double const *angles, int tokens, int heads, int head_dim, int pairs, int interleaved, int type) {
   MI355_REQUIRE_INIT();
-  if (x == y && x_stride != y_stride) {
-    return fail(MI355_ERR_INVALID, "mi355_rotary: in place the strides are the same");
-  }
   RotaryParams P{};
   P.src[0] = x;
   P.src_stride[0] = x_stride;

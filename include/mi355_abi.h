@@ -454,11 +454,11 @@ typedef struct mi355_paged_cache {
 /* y = x with rotary positions, `heads` heads of head_dim elements in a row for every token, tokens x_stride and
  * y_stride apart: pair i < pairs of a head, elements (i, i + pairs) or, interleaved, (2i, 2i + 1), is turned by
  * positions[token] * angles[i] radians (computed in 64 bits) and scaled by angles[pairs + i]; the rest is copied.  y may
- * be x with the same stride.  Up to MI355_MAX_ROTARY_PAIRS pairs and 2^30 elements a token. */
+ * be x with the same stride, and else overlaps nothing that is read.  Up to MI355_MAX_ROTARY_PAIRS pairs and 2^30 elements a token. */
 int mi355_rotary(void const *x, long long x_stride, void *y, long long y_stride, int const *positions, double const *angles,
                  int tokens, int heads, int head_dim, int pairs, int interleaved, int type);
 /* The same for q_heads heads of q (results in q_out) and the cache's kv_heads heads of k, which go into the cache at
- * slots[token] = page * page_size + place, the values v beside them as they are.  A slot that is negative or past the
+ * slots[token] = page * page_size + place, the values v beside them as they are.  q_out may be q with the same stride.  A slot that is negative or past the
  * cache stores nothing.  Slots of one call differ (of one named twice, any element may come from either token). */
 int mi355_rotary_append(void const *q, long long q_stride, void const *k, long long k_stride, void const *v, long long v_stride,
                         void *q_out, long long out_stride, int const *positions, double const *angles, int const *slots,
