@@ -11,6 +11,7 @@
 // again.  Sums are added in an order that does not depend on who comes last.  Bound by HBM for a batch (64 sequences x 131072
 // fp32, 67 MB: 16 us, 4.2 TB/s), by the chain of trips for one sequence (5.4 us).
 #include "common.h"
+#include "slices.h"
 
 #include <climits>
 #include <cmath>
@@ -295,19 +296,18 @@ int launch_rounds(VerifyParams P, int sequences, int most) {
   if (slice == 0) {
     return fail(MI355_ERR_UNSUPPORTED, "mi355_verify_drafts: a vocabulary of %d", P.vocabulary);
   }
-  for (int at = 0; at < sequences; at += slice) {
+  return in_slices(sequences, slice, [&](long long at, long long count) -> int {
     VerifyParams Q = P;
-    int const count = sequences - at < slice ? sequences - at : slice;
-    Q.target = static_cast<T const *>(P.target) + (long long)at * (P.drafts + 1) * P.vocabulary;
-    Q.draft = P.draft != nullptr ? static_cast<T const *>(P.draft) + (long long)at * P.drafts * P.vocabulary : nullptr;
-    Q.tokens = P.tokens + (long long)at * P.drafts;
-    Q.uniforms = P.uniforms + (long long)at * (P.drafts + 1);
+    Q.target = static_cast<T const *>(P.target) + at * (P.drafts + 1) * P.vocabulary;
+    Q.draft = P.draft != nullptr ? static_cast<T const *>(P.draft) + at * P.drafts * P.vocabulary : nullptr;
+    Q.tokens = P.tokens + at * P.drafts;
+    Q.uniforms = P.uniforms + at * (P.drafts + 1);
     Q.accepted = P.accepted + at;
-    Q.out = P.out + (long long)at * (P.drafts + 1);
+    Q.out = P.out + at * (P.drafts + 1);
     MI355_HIP(launch_kernel(verify_drafts_kernel<T, ROUNDS>, dim3((unsigned)workgroups(), (unsigned)count), dim3(kThreads), 0,
                             state().stream(), Q));
-  }
-  return MI355_OK;
+    return MI355_OK;
+  });
 }
 
 // Strips of one round where all of them together are at most two workgroups a compute unit: the last workgroup then has
