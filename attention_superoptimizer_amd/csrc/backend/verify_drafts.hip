@@ -334,6 +334,9 @@ extern "C" int mi355_verify_drafts(void const *target, void const *draft, int co
   if (type != MI355_TYPE_F16 && type != MI355_TYPE_BF16 && type != MI355_TYPE_F32) {
     return fail(MI355_ERR_UNSUPPORTED, "mi355_verify_drafts: type %d", type);
   }
+  if (drafts > INT_MAX / 2) {  // (a wavefront goes through them in steps of 64, counted by an int)
+    return fail(MI355_ERR_UNSUPPORTED, "mi355_verify_drafts: %d drafts", drafts);
+  }
   if (sequences == 0) {
     return MI355_OK;
   }

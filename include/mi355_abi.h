@@ -482,7 +482,7 @@ int mi355_paged_attention(void const *q, long long q_stride, void *out, long lon
  * weights passes that share of their total -- and -1 behind it.  The weights: target, less draft and not below zero
  * (certain: without the token) where a draft was refused, unless that leaves nothing; without any weight the token is
  * -1.  target [sequences][drafts + 1][vocabulary], draft [sequences][drafts][vocabulary], fp16, bf16 or fp32; sums and
- * comparisons in 64 bits. */
+ * comparisons in 64 bits.  Up to 2^30 - 1 drafts. */
 int mi355_verify_drafts(void const *target, void const *draft, int const *tokens, float const *uniforms, int *accepted, int *out,
                         int sequences, int drafts, int vocabulary, int type);
 
