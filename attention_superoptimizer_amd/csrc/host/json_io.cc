@@ -9,6 +9,8 @@
 
 #include "mirage/utils/hip_types.h"
 
+#include <algorithm>
+#include <climits>
 #include <cmath>
 #include <cstdio>
 #include <memory>
@@ -720,7 +722,8 @@ void from_json(json const &j, Graph &g) {
                                          jop.at("heads_first").as_bool());
         } else if (op_type == KN_PAGED_ATTENTION_OP) {
           op = g.create_paged_attention_op(in(0), in(1), in(2), in(3), in(4), (float)jop.at("scale").as_double(),
-                                           (int)jop.at("window").as_int(), jop.at("heads_first").as_bool());
+                                           (int)std::max(-1LL, std::min(jop.at("window").as_int(), (long long)INT_MAX)),
+                                           jop.at("heads_first").as_bool());
         } else {
           bool const certain = ins.size() == 3;
           op = g.create_verify_drafts_op(in(0), certain ? nullptr : &in(1), in(certain ? 1 : 2), in(certain ? 2 : 3));

@@ -309,8 +309,9 @@ class KNGraph:
         sqrt(head_dim) if not given."""
         if scale is None:
             scale = float(k_cache.dims[-1]) ** -0.5
+        window = max(-1, min(int(window), 2 ** 31 - 1))  # (ctypes would take its lowest 32 bits)
         return self._wrap(self._rt.mirage_graph_paged_attention(self._g, q._h, k_cache._h, v_cache._h, table._h, lengths._h,
-                                                                scale, int(window), int(heads_first)), "paged_attention")
+                                                                scale, window, int(heads_first)), "paged_attention")
 
     def verify_drafts(self, target: DTensor, draft: Optional[DTensor], tokens: DTensor, uniforms: DTensor):
         """Which drafted tokens the target's probabilities keep, and the one after them: (accepted [sequences], tokens
