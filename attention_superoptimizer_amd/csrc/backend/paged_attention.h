@@ -193,7 +193,9 @@ __device__ __forceinline__ int wave_upto(int x) {
   return x;
 }
 
-// Parts go through the memory that all XCDs share: device-scope stores and loads, which pass by this XCD's L2.
+// Parts go through the memory that all XCDs share: device-scope stores and loads (sc1 on each), which pass by this XCD's L2.
+// The join depends on that for every access to a part, not on fences: parts lie where those of earlier launches did, and
+// a load that this XCD's L2 may serve finds what was there then.  The ticket is taken when the stores have arrived (vmcnt).
 __device__ __forceinline__ void store_shared(float *p, float a, float b) {
   uint64_t const both = (uint64_t)__builtin_bit_cast(uint32_t, a) | (uint64_t)__builtin_bit_cast(uint32_t, b) << 32;
   __hip_atomic_store((__attribute__((address_space(1))) uint64_t *)(uint64_t *)p, both, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
