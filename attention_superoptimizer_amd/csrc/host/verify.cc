@@ -529,17 +529,10 @@ void set_verify_queues_per_batch(int queues) {
   g_queues_per_batch = std::max(1, std::min(queues, (int)MI355_NUM_QUEUES));
 }
 
-VerifyTicket *verify_batch_begin(std::vector<kernel::Graph *> const &candidates,
+// of graphs whose operators all have fingerprints (asked once: of a thousand candidates it shows)
+static VerifyTicket *begin_batch(std::vector<kernel::Graph *> const &candidates,
                                  std::vector<DTensor> const &reference_outputs,
                                  uint64_t input_seed, kernel::Graph *reference_to_fingerprint) {
-  bool all = reference_to_fingerprint == nullptr || has_fingerprints(*reference_to_fingerprint);
-  for (kernel::Graph const *g : candidates) {
-    all = all && has_fingerprints(*g);
-  }
-  for (DTensor const &t : reference_outputs) {
-    all = all && (t.owner_op == nullptr || has_fingerprint(t.owner_op));
-  }
-  MIRAGE_CHECK(all, "verify_batch: an operator has no fingerprint");
   kernel::require_device("verify_batch");
   std::unique_ptr<VerifyTicket> t(new VerifyTicket);
   t->t_begin = std::chrono::steady_clock::now();
@@ -709,6 +702,20 @@ void verify_batch_end(VerifyTicket *ticket, std::vector<uint8_t> &equal, VerifyS
   }
 }
 
+VerifyTicket *verify_batch_begin(std::vector<kernel::Graph *> const &candidates,
+                                 std::vector<DTensor> const &reference_outputs,
+                                 uint64_t input_seed, kernel::Graph *reference_to_fingerprint) {
+  bool all = reference_to_fingerprint == nullptr || has_fingerprints(*reference_to_fingerprint);
+  for (kernel::Graph const *g : candidates) {
+    all = all && has_fingerprints(*g);
+  }
+  for (DTensor const &t : reference_outputs) {
+    all = all && (t.owner_op == nullptr || has_fingerprint(t.owner_op));
+  }
+  MIRAGE_CHECK(all, "verify_batch: an operator has no fingerprint");
+  return begin_batch(candidates, reference_outputs, input_seed, reference_to_fingerprint);
+}
+
 void verify_batch(std::vector<kernel::Graph *> const &candidates,
                   std::vector<DTensor> const &reference_outputs, uint64_t input_seed,
                   std::vector<uint8_t> &equal, VerifyStats *stats) {
@@ -778,8 +785,8 @@ void *mirage_verify_batch_begin(void *const *candidates, int n, void *reference,
     c[i] = static_cast<mirage::kernel::Graph *>(candidates[i]);
   }
   mirage::kernel::Graph *ref = static_cast<mirage::kernel::Graph *>(reference);
-  return mirage::search::verify_batch_begin(c, mirage::search::graph_outputs(*ref), input_seed,
-                                            fingerprint_reference ? ref : nullptr);
+  return mirage::search::begin_batch(c, mirage::search::graph_outputs(*ref), input_seed,
+                                     fingerprint_reference ? ref : nullptr);
 }
 
 // The bookkeeping of slot ranges and mark pairs by itself (no device): a scratch instance for
@@ -821,7 +828,7 @@ int mirage_verify_batch(void *const *candidates, int n, void *reference,
       mirage::search::graph_outputs(*static_cast<mirage::kernel::Graph *>(reference));
   std::vector<uint8_t> eq;
   mirage::search::VerifyStats s;
-  mirage::search::verify_batch(c, ref, input_seed, eq, &s);
+  mirage::search::verify_batch_end(mirage::search::begin_batch(c, ref, input_seed, nullptr), eq, &s);
   for (int i = 0; i < n; i++) {
     equal[i] = eq[i];
   }
