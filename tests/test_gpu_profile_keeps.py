@@ -24,7 +24,8 @@ def test_a_profile_keeps_the_caches(rt, kind):
         kept = [qkv, k, v, positions, slots, angles, table, lengths, q, o]
         want = [read(t) for t in kept]
         total, each = g.profile_all()
-        assert len(each) == g.num_operators and min(each[-2:]) > 0 and total >= sum(each[-2:])
+        assert len(each) == g.num_operators and min(each[-2:]) > 0
+        assert abs(total - sum(each[-2:])) <= 2.0 ** -24 * total  # (one addition in 32 bits: off by half a step of its result at most)
         for t, w in zip(kept, want):
             np.testing.assert_array_equal(read(t), w)
         for i in range(g.num_operators):
