@@ -148,6 +148,10 @@ ABI = {
     "mi355_paged_attention": (_ci, [_vp, _ll, _vp, _ll, ctypes.POINTER(Mi355PagedCache), _vp, _ci, _vp, _ci, _ci, _ci,
                                     ctypes.c_float, _ci]),
     "mi355_verify_drafts": (_ci, [_vp] * 6 + [_ci] * 4),
+    "mi355_tree_attention": (_ci, [_vp, _ll, _vp, _ll, ctypes.POINTER(Mi355PagedCache), _vp, _ci, _vp, _vp, _ci, _ci, _ci, ctypes.c_float]),
+    "mi355_window_attention": (_ci, [_vp, _ll, _vp, _ll, ctypes.POINTER(Mi355PagedCache), _vp, _ci, _vp, _vp, _ci, _ci, _ci,
+                                     ctypes.c_float, _ci, _ci]),
+    "mi355_log_probabilities": (_ci, [_vp, _ll] + [_vp] * 5 + [_ci] * 4 + [ctypes.c_float, _ci]),
     "mi355_emit_hip_preamble": (ctypes.c_char_p, []),
     "mi355_emit_hip_kernel": (ctypes.c_longlong, [_pplan, ctypes.c_char_p, _ci, ctypes.c_char_p,
                                                   ctypes.c_longlong]),
@@ -180,6 +184,9 @@ FACADE = {
     "mirage_graph_rotary_append": (_vp, [_vp] * 7 + [_ci] * 2),
     "mirage_graph_paged_attention": (_vp, [_vp] * 6 + [ctypes.c_float, _ci, _ci]),
     "mirage_graph_verify_drafts": (_ci, [_vp] * 5 + [_pvp]),
+    "mirage_graph_tree_attention": (_vp, [_vp] * 7 + [ctypes.c_float, _ci]),
+    "mirage_graph_window_attention": (_vp, [_vp] * 7 + [ctypes.c_float, _ci, _ci, _ci]),
+    "mirage_graph_log_probabilities": (_ci, [_vp] * 3 + [_ci, ctypes.c_float, _pvp]),
     "mirage_graph_pop_operator": (_ci, [_vp]),
     "mirage_op_type": (_ci, [_vp, _ci]),
     "mirage_op_num_outputs": (_ci, [_vp, _ci]),

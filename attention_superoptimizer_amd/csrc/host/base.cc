@@ -57,6 +57,9 @@ char const *to_string(KNOperatorType t) {
     case KN_ROTARY_APPEND_OP: return "kn_rotary_append_op";
     case KN_PAGED_ATTENTION_OP: return "kn_paged_attention_op";
     case KN_VERIFY_DRAFTS_OP: return "kn_verify_drafts_op";
+    case KN_TREE_ATTENTION_OP: return "kn_tree_attention_op";
+    case KN_WINDOW_ATTENTION_OP: return "kn_window_attention_op";
+    case KN_LOG_PROBABILITIES_OP: return "kn_log_probabilities_op";
     case KN_CUSTOMIZED_OP: return "kn_customized_op";
     default: return "kn_unkown";
   }

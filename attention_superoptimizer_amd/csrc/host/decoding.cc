@@ -1,6 +1,7 @@
 // Operators of a decoding step (include/mirage/kernel/decoding.h): what they take, their results' tensors, and the
 // calls of the C ABI that run them.
 #include "mi355_abi.h"
+#include "mi355_kernels/attention_blocks_units.h"
 #include "mi355_kernels/paged_units.h"
 #include "mirage/kernel/device_memory_manager.h"
 #include "mirage/kernel/graph.h"
@@ -183,6 +184,60 @@ bool verify_ok(DTensor const &target, DTensor const *draft, DTensor const &token
          has_dims(uniforms, {sequences, drafts + 1}) && uniforms.data_type == DT_FLOAT32 && row_major(uniforms);
 }
 
+// What paged caches, a table and lengths of `sequences` sequences have to be for attention of q, whose heads it gives; 0: infeasible.
+int cached_heads(DTensor const &q, DTensor const &k, DTensor const &v, DTensor const &table, DTensor const &lengths, float scale,
+                 bool heads_first) {
+  if (!caches_ok(k, v, heads_first) || q.data_type != k.data_type || !row_major(q) || !positive(q) || !std::isfinite(scale) ||
+      table.num_dims != 2 || !positive(table) || table.data_type != DT_INT32 || !row_major(table) || !has_dims(lengths, {table.dim[0]}) ||
+      lengths.data_type != DT_INT32 || !row_major(lengths)) {
+    return 0;
+  }
+  CacheShape const c(k, heads_first);
+  int const heads = heads_in(q, c.head_dim);
+  if (heads == 0 || heads % c.kv_heads != 0 || c.head_dim % 8 != 0 || c.head_dim > MI355_MAX_PAGED_HEAD_DIM ||
+      (long long)heads * c.head_dim > INT_MAX || (long long)table.dim[1] * c.page_size > 1 << 30 ||
+      (unsigned long long)k.num_elements() / 8 >= UINT_MAX) {
+    return 0;
+  }
+  return heads;
+}
+
+bool tree_ok(DTensor const &q, DTensor const &k, DTensor const &v, DTensor const &table, DTensor const &lengths, DTensor const &parents,
+             float scale, bool heads_first) {
+  int const heads = cached_heads(q, k, v, table, lengths, scale, heads_first);
+  return heads > 0 && parents.num_dims == 2 && positive(parents) && parents.dim[0] == table.dim[0] && parents.dim[1] <= MI355_MAX_TREE_NODES &&
+         parents.data_type == DT_INT32 && row_major(parents) && (long long)parents.dim[0] * parents.dim[1] == q.dim[0] &&
+         mi355::blocks::fit(q.dim[0], heads / CacheShape(k, heads_first).kv_heads, CacheShape(k, heads_first).kv_heads, table.dim[0]);
+}
+
+bool window_ok(DTensor const &q, DTensor const &k, DTensor const &v, DTensor const &table, DTensor const &lengths, DTensor const *starts,
+               float scale, int window, int sinks, bool heads_first) {
+  int const heads = cached_heads(q, k, v, table, lengths, scale, heads_first);
+  bool const rows = starts == nullptr ? heads > 0 && q.dim[0] % table.dim[0] == 0
+                                      : heads > 0 && table.dim[0] < INT_MAX && has_dims(*starts, {table.dim[0] + 1}) &&
+                                            starts->data_type == DT_INT32 && row_major(*starts);
+  return rows && window >= 0 && sinks >= 0 &&
+         mi355::blocks::fit(q.dim[0], heads / CacheShape(k, heads_first).kv_heads, CacheShape(k, heads_first).kv_heads, table.dim[0]);
+}
+
+std::vector<DTensor> window_inputs(DTensor const &q, DTensor const &k, DTensor const &v, DTensor const &table, DTensor const &lengths,
+                                   DTensor const *starts) {
+  std::vector<DTensor> in{q, k, v, table, lengths};
+  if (starts != nullptr) {
+    in.push_back(*starts);
+  }
+  return in;
+}
+
+long long log_rows(DTensor const &logits) { return logits.num_dims == 3 ? (long long)logits.dim[0] * logits.dim[1] : logits.dim[0]; }
+
+bool log_ok(DTensor const &logits, DTensor const &tokens, int top, float scale) {
+  return (logits.num_dims == 2 || logits.num_dims == 3) && positive(logits) && (half_type(logits) || logits.data_type == DT_FLOAT32) &&
+         row_major(logits) && log_rows(logits) <= INT_MAX && (tokens.num_dims == 1 || tokens.num_dims == 2) && positive(tokens) &&
+         tokens.dim[0] == log_rows(logits) && tokens.data_type == DT_INT32 && row_major(tokens) && top >= 0 && top <= MI355_MAX_TOP &&
+         scale > 0.0f && std::isfinite(scale) && logits.dim[logits.num_dims - 1] <= MI355_MAX_VOCABULARY;
+}
+
 std::vector<DTensor> verify_inputs(DTensor const &target, DTensor const *draft, DTensor const &tokens, DTensor const &uniforms) {
   std::vector<DTensor> in{target};
   if (draft != nullptr) {
@@ -206,7 +261,7 @@ DTensor push(std::vector<KNOperator *> &ops, KNOperator *op, char const *what) {
 
 }  // namespace
 
-bool is_decoding_op(KNOperatorType type) { return type >= KN_ROTARY_OP && type <= KN_VERIFY_DRAFTS_OP; }
+bool is_decoding_op(KNOperatorType type) { return type >= KN_ROTARY_OP && type <= KN_LOG_PROBABILITIES_OP; }
 
 bool Graph::keeps_inputs() const {
   for (KNOperator const *op : operators) {
@@ -371,6 +426,113 @@ void KNVerifyDraftsOp::run() const {
                                  tokens.dim[0], tokens.dim[1], target.dim[target.num_dims - 1], target.data_type));
 }
 
+// ---- tree_attention -----------------------------------------------------------------------------
+KNOperator *Graph::create_tree_attention_op(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table,
+                                            DTensor const &lengths, DTensor const &parents, float scale, bool heads_first) {
+  return tree_ok(q, k_cache, v_cache, table, lengths, parents, scale, heads_first) && room_for(q)
+             ? new KNTreeAttentionOp(q, k_cache, v_cache, table, lengths, parents, scale, heads_first)
+             : nullptr;
+}
+
+DTensor Graph::tree_attention(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table,
+                              DTensor const &lengths, DTensor const &parents, float scale, bool heads_first) {
+  return push(operators, create_tree_attention_op(q, k_cache, v_cache, table, lengths, parents, scale, heads_first),
+              "infeasible tree_attention");
+}
+
+KNTreeAttentionOp::KNTreeAttentionOp(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table,
+                                     DTensor const &lengths, DTensor const &parents, float _scale, bool _heads_first)
+    : KNDecodingOp(KN_TREE_ATTENTION_OP, {q, k_cache, v_cache, table, lengths, parents}), scale(_scale), heads_first(_heads_first) {
+  MIRAGE_CHECK(tree_ok(q, k_cache, v_cache, table, lengths, parents, scale, heads_first), "tree_attention operands do not agree");
+  adopt(this, queries_of(q, heads_in(q, k_cache.dim[3]), k_cache.dim[3]));
+}
+
+void KNTreeAttentionOp::run() const {
+  DTensor const &q = input_tensors[0], &table = input_tensors[3], &parents = input_tensors[5];
+  mi355_paged_cache const cache = cache_of(input_tensors[1], input_tensors[2], heads_first);
+  int const q_heads = heads_in(q, cache.head_dim);
+  long long const stride = (long long)q_heads * cache.head_dim;
+  MI355_CALL(mi355_tree_attention(q.data_ptr, stride, output_tensors[0].data_ptr, stride, &cache,
+                                  static_cast<int const *>(table.data_ptr), table.dim[1],
+                                  static_cast<int const *>(input_tensors[4].data_ptr), static_cast<int const *>(parents.data_ptr),
+                                  parents.dim[0], parents.dim[1], q_heads, scale));
+}
+
+// ---- window_attention ---------------------------------------------------------------------------
+KNOperator *Graph::create_window_attention_op(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table,
+                                              DTensor const &lengths, DTensor const *starts, float scale, int window, int sinks,
+                                              bool heads_first) {
+  return window_ok(q, k_cache, v_cache, table, lengths, starts, scale, window, sinks, heads_first) && room_for(q)
+             ? new KNWindowAttentionOp(q, k_cache, v_cache, table, lengths, starts, scale, window, sinks, heads_first)
+             : nullptr;
+}
+
+DTensor Graph::window_attention(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table,
+                                DTensor const &lengths, DTensor const *starts, float scale, int window, int sinks, bool heads_first) {
+  return push(operators, create_window_attention_op(q, k_cache, v_cache, table, lengths, starts, scale, window, sinks, heads_first),
+              "infeasible window_attention");
+}
+
+KNWindowAttentionOp::KNWindowAttentionOp(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table,
+                                         DTensor const &lengths, DTensor const *starts, float _scale, int _window, int _sinks,
+                                         bool _heads_first)
+    : KNDecodingOp(KN_WINDOW_ATTENTION_OP, window_inputs(q, k_cache, v_cache, table, lengths, starts)), scale(_scale), window(_window),
+      sinks(_sinks), heads_first(_heads_first) {
+  MIRAGE_CHECK(window_ok(q, k_cache, v_cache, table, lengths, starts, scale, window, sinks, heads_first),
+               "window_attention operands do not agree");
+  adopt(this, queries_of(q, heads_in(q, k_cache.dim[3]), k_cache.dim[3]));
+}
+
+void KNWindowAttentionOp::run() const {
+  DTensor const &q = input_tensors[0], &table = input_tensors[3];
+  mi355_paged_cache const cache = cache_of(input_tensors[1], input_tensors[2], heads_first);
+  int const q_heads = heads_in(q, cache.head_dim);
+  long long const stride = (long long)q_heads * cache.head_dim;
+  int const *const starts = input_tensors.size() > 5 ? static_cast<int const *>(input_tensors[5].data_ptr) : nullptr;
+  MI355_CALL(mi355_window_attention(q.data_ptr, stride, output_tensors[0].data_ptr, stride, &cache,
+                                    static_cast<int const *>(table.data_ptr), table.dim[1],
+                                    static_cast<int const *>(input_tensors[4].data_ptr), starts, table.dim[0], q.dim[0], q_heads, scale,
+                                    window, sinks));
+}
+
+// ---- log_probabilities ----------------------------------------------------------------------------
+KNOperator *Graph::create_log_probabilities_op(DTensor const &logits, DTensor const &tokens, int top, float scale) {
+  if (!log_ok(logits, tokens, top, scale)) {
+    return nullptr;
+  }
+  size_t const rows = (size_t)tokens.dim[0], given = tokens.num_elements(), best = rows * (size_t)top;
+  return room_for({4 * given, 4 * rows, 4 * best, 4 * best}, {2 * given, 2 * rows, 2 * best, 2 * best})
+             ? new KNLogProbabilitiesOp(logits, tokens, top, scale)
+             : nullptr;
+}
+
+std::vector<DTensor> Graph::log_probabilities(DTensor const &logits, DTensor const &tokens, int top, float scale) {
+  push(operators, create_log_probabilities_op(logits, tokens, top, scale), "infeasible log_probabilities");
+  return operators.back()->output_tensors;
+}
+
+KNLogProbabilitiesOp::KNLogProbabilitiesOp(DTensor const &logits, DTensor const &tokens, int _top, float _scale)
+    : KNDecodingOp(KN_LOG_PROBABILITIES_OP, {logits, tokens}), top(_top), scale(_scale) {
+  MIRAGE_CHECK(log_ok(logits, tokens, top, scale), "log_probabilities operands do not agree");
+  int const rows = tokens.dim[0];
+  adopt(this, tokens.num_dims == 1 ? tensor_of({rows}, DT_FLOAT32) : tensor_of({rows, tokens.dim[1]}, DT_FLOAT32));
+  adopt(this, tensor_of({rows}, DT_FLOAT32));
+  if (top > 0) {
+    adopt(this, tensor_of({rows, top}, DT_FLOAT32));
+    adopt(this, tensor_of({rows, top}, DT_INT32));
+  }
+}
+
+void KNLogProbabilitiesOp::run() const {
+  DTensor const &logits = input_tensors[0], &tokens = input_tensors[1];
+  int const vocabulary = logits.dim[logits.num_dims - 1];
+  MI355_CALL(mi355_log_probabilities(logits.data_ptr, vocabulary, static_cast<int const *>(tokens.data_ptr),
+                                     static_cast<float *>(output_tensors[0].data_ptr), static_cast<float *>(output_tensors[1].data_ptr),
+                                     top > 0 ? static_cast<float *>(output_tensors[2].data_ptr) : nullptr,
+                                     top > 0 ? static_cast<int *>(output_tensors[3].data_ptr) : nullptr, tokens.dim[0],
+                                     tokens.num_dims == 1 ? 1 : tokens.dim[1], top, vocabulary, scale, logits.data_type));
+}
+
 }  // namespace kernel
 }  // namespace mirage
 
@@ -418,6 +580,34 @@ int mirage_graph_verify_drafts(void *g, void *target, void *draft, void *tokens,
   outputs[0] = &G->operators.back()->output_tensors[0];
   outputs[1] = &G->operators.back()->output_tensors[1];
   return 0;
+}
+
+void *mirage_graph_tree_attention(void *g, void *q, void *k_cache, void *v_cache, void *table, void *lengths, void *parents, float scale,
+                                  int heads_first) {
+  auto *G = static_cast<Graph *>(g);
+  return keep(G, G->create_tree_attention_op(at(q), at(k_cache), at(v_cache), at(table), at(lengths), at(parents), scale,
+                                             heads_first != 0));
+}
+
+// starts may be null
+void *mirage_graph_window_attention(void *g, void *q, void *k_cache, void *v_cache, void *table, void *lengths, void *starts, float scale,
+                                    int window, int sinks, int heads_first) {
+  auto *G = static_cast<Graph *>(g);
+  return keep(G, G->create_window_attention_op(at(q), at(k_cache), at(v_cache), at(table), at(lengths),
+                                               static_cast<DTensor const *>(starts), scale, window, sinks, heads_first != 0));
+}
+
+// outputs: log probabilities, entropy and, with top > 0, the top ones' and their tokens; returns how many
+int mirage_graph_log_probabilities(void *g, void *logits, void *tokens, int top, float scale, void **outputs) {
+  auto *G = static_cast<Graph *>(g);
+  if (keep(G, G->create_log_probabilities_op(at(logits), at(tokens), top, scale)) == nullptr) {
+    return -1;
+  }
+  auto &made = G->operators.back()->output_tensors;
+  for (size_t i = 0; i < made.size(); i++) {
+    outputs[i] = &made[i];
+  }
+  return (int)made.size();
 }
 
 }  // extern "C"

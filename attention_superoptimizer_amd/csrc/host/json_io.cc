@@ -448,6 +448,9 @@ EnumName const kKnOps[] = {
     {KN_ROTARY_APPEND_OP, "kn_rotary_append_op"},
     {KN_PAGED_ATTENTION_OP, "kn_paged_attention_op"},
     {KN_VERIFY_DRAFTS_OP, "kn_verify_drafts_op"},
+    {KN_TREE_ATTENTION_OP, "kn_tree_attention_op"},
+    {KN_WINDOW_ATTENTION_OP, "kn_window_attention_op"},
+    {KN_LOG_PROBABILITIES_OP, "kn_log_probabilities_op"},
     {KN_CUSTOMIZED_OP, "kn_customized_op"},
 };
 // reference include/mirage/type.h:105-129
@@ -602,6 +605,20 @@ void to_json(json &j, KNOperator const &op) {
     j["scale"] = (double)a.scale;
     j["window"] = a.window;
     j["heads_first"] = a.heads_first;
+  } else if (op.op_type == KN_TREE_ATTENTION_OP) {
+    auto const &a = static_cast<KNTreeAttentionOp const &>(op);
+    j["scale"] = (double)a.scale;
+    j["heads_first"] = a.heads_first;
+  } else if (op.op_type == KN_WINDOW_ATTENTION_OP) {
+    auto const &a = static_cast<KNWindowAttentionOp const &>(op);
+    j["scale"] = (double)a.scale;
+    j["window"] = a.window;
+    j["sinks"] = a.sinks;
+    j["heads_first"] = a.heads_first;
+  } else if (op.op_type == KN_LOG_PROBABILITIES_OP) {
+    auto const &a = static_cast<KNLogProbabilitiesOp const &>(op);
+    j["top"] = a.top;
+    j["scale"] = (double)a.scale;
   }
 }
 
@@ -711,9 +728,15 @@ void from_json(json const &j, Graph &g) {
       case KN_ROTARY_OP:
       case KN_ROTARY_APPEND_OP:
       case KN_PAGED_ATTENTION_OP:
-      case KN_VERIFY_DRAFTS_OP: {
+      case KN_VERIFY_DRAFTS_OP:
+      case KN_TREE_ATTENTION_OP:
+      case KN_WINDOW_ATTENTION_OP:
+      case KN_LOG_PROBABILITIES_OP: {
         json const &ins = jop.at("input_tensors");
         auto in = [&](size_t i) -> DTensor const & { return tensor_of(ins.at(i)); };
+        auto clamped = [&](char const *name) {
+          return (int)std::max(-1LL, std::min(jop.at(name).as_int(), (long long)INT_MAX));
+        };
         KNOperator *op = nullptr;
         if (op_type == KN_ROTARY_OP) {
           op = g.create_rotary_op(in(0), in(1), in(2), jop.at("interleaved").as_bool());
@@ -722,8 +745,16 @@ void from_json(json const &j, Graph &g) {
                                          jop.at("heads_first").as_bool());
         } else if (op_type == KN_PAGED_ATTENTION_OP) {
           op = g.create_paged_attention_op(in(0), in(1), in(2), in(3), in(4), (float)jop.at("scale").as_double(),
-                                           (int)std::max(-1LL, std::min(jop.at("window").as_int(), (long long)INT_MAX)),
-                                           jop.at("heads_first").as_bool());
+                                           clamped("window"), jop.at("heads_first").as_bool());
+        } else if (op_type == KN_TREE_ATTENTION_OP) {
+          op = g.create_tree_attention_op(in(0), in(1), in(2), in(3), in(4), in(5), (float)jop.at("scale").as_double(),
+                                          jop.at("heads_first").as_bool());
+        } else if (op_type == KN_WINDOW_ATTENTION_OP) {
+          op = g.create_window_attention_op(in(0), in(1), in(2), in(3), in(4), ins.size() > 5 ? &in(5) : nullptr,
+                                            (float)jop.at("scale").as_double(), clamped("window"), clamped("sinks"),
+                                            jop.at("heads_first").as_bool());
+        } else if (op_type == KN_LOG_PROBABILITIES_OP) {
+          op = g.create_log_probabilities_op(in(0), in(1), clamped("top"), (float)jop.at("scale").as_double());
         } else {
           bool const certain = ins.size() == 3;
           op = g.create_verify_drafts_op(in(0), certain ? nullptr : &in(1), in(certain ? 1 : 2), in(certain ? 2 : 3));

@@ -684,6 +684,9 @@ char const *execute_once(KNOperator *op) {
     case KN_ROTARY_APPEND_OP:
     case KN_PAGED_ATTENTION_OP:
     case KN_VERIFY_DRAFTS_OP:
+    case KN_TREE_ATTENTION_OP:
+    case KN_WINDOW_ATTENTION_OP:
+    case KN_LOG_PROBABILITIES_OP:
       static_cast<KNDecodingOp *>(op)->run();
       break;
     default:

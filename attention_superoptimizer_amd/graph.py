@@ -327,6 +327,50 @@ class KNGraph:
             raise InfeasibleOperator("verify_drafts")
         return DTensor(outs[0]), DTensor(outs[1])
 
+    def tree_attention(self, q: DTensor, k_cache: DTensor, v_cache: DTensor, table: DTensor, lengths: DTensor, parents: DTensor,
+                       scale: Optional[float] = None, heads_first: bool = False) -> DTensor:
+        """`paged_attention` of a tree of drafted tokens of every sequence: q [sequences * nodes, ..], of which a row sees the
+        keys before the tree, those of its own node and of that one's ancestors.  parents [sequences, nodes] int32, up to 1024
+        nodes: the node that node i follows, one before it; -1: it follows the sequence itself.  lengths count the nodes, whose
+        keys are in the caches already, node i's at place length - nodes + i.  A node with any other parent, or a place below
+        zero, is not there, nor is what follows it: its row is zeros and no row sees its key (mark what fewer drafts leave by
+        -2).  Everything else as in `paged_attention`."""
+        if scale is None:
+            scale = float(k_cache.dims[-1]) ** -0.5
+        return self._wrap(self._rt.mirage_graph_tree_attention(self._g, q._h, k_cache._h, v_cache._h, table._h, lengths._h, parents._h,
+                                                               scale, int(heads_first)), "tree_attention")
+
+    def window_attention(self, q: DTensor, k_cache: DTensor, v_cache: DTensor, table: DTensor, lengths: DTensor, window: int,
+                         sinks: int = 0, starts: Optional[DTensor] = None, scale: Optional[float] = None,
+                         heads_first: bool = False) -> DTensor:
+        """`paged_attention` of single tokens, chunks or whole prompts within a window and to the first `sinks` tokens: new
+        token t of a sequence sees the keys j < L = length - (new - 1 - t) with j >= L - window (window 0: all) or j < sinks.
+        Pages that hold none of them may be given back, their numbers in the table being anything.  q [tokens, q_heads,
+        head_dim] or [tokens, q_heads * head_dim]; without `starts` every sequence has tokens / sequences of them in a row; with
+        starts [sequences + 1] int32, ascending from 0, sequence b has the rows starts[b] to starts[b + 1] - 1, none or any
+        number, and rows of the result from starts[sequences] on are left as they were.  Everything else as in
+        `paged_attention`."""
+        if scale is None:
+            scale = float(k_cache.dims[-1]) ** -0.5
+        window, sinks = (max(-1, min(int(n), 2 ** 31 - 1)) for n in (window, sinks))  # (ctypes would take their lowest 32 bits)
+        return self._wrap(self._rt.mirage_graph_window_attention(self._g, q._h, k_cache._h, v_cache._h, table._h, lengths._h,
+                                                                 None if starts is None else starts._h, scale, window, sinks,
+                                                                 int(heads_first)), "window_attention")
+
+    def log_probabilities(self, logits: DTensor, tokens: DTensor, top: int = 0, scale: float = 1.0):
+        """Of the distribution softmax(scale * logits), logits [rows, vocabulary] or [sequences, tokens, vocabulary], fp16, bf16 or
+        fp32, scale (one over a temperature) above zero: (log probabilities of `tokens`, entropy [rows]) and with top > 0, up to
+        64, (.., .., log probabilities [rows, top], tokens [rows, top]) of the most probable tokens, of equal logits the lower
+        index first.  tokens [rows] or [rows, asked] int32, minus infinity for one outside the vocabulary; numbers are fp32, in
+        natural units.  Tokens whose logit is minus infinity are no alternatives: -1 and minus infinity where there are too few
+        others.  A row of minus infinities alone: log probabilities of minus infinity, entropy 0, no alternatives; one with a NaN
+        or plus infinity: NaN, no alternatives."""
+        outs = (ctypes.c_void_p * 4)()
+        n = self._rt.mirage_graph_log_probabilities(self._g, logits._h, tokens._h, max(-1, min(int(top), 2 ** 31 - 1)), float(scale), outs)
+        if n < 0:
+            raise InfeasibleOperator("log_probabilities")
+        return tuple(DTensor(outs[i]) for i in range(n))
+
     def pop_operator(self) -> None:
         assert self._rt.mirage_graph_pop_operator(self._g) == 0
 

@@ -485,6 +485,35 @@ int mi355_paged_attention(void const *q, long long q_stride, void *out, long lon
  * comparisons in 64 bits.  Up to 2^30 - 1 drafts. */
 int mi355_verify_drafts(void const *target, void const *draft, int const *tokens, float const *uniforms, int *accepted, int *out,
                         int sequences, int drafts, int vocabulary, int type);
+/* mi355_paged_attention for a tree of `nodes` new tokens of each sequence: the row of node i sees the keys before
+ * lengths[sequence] - nodes, its own (at that place + i) and those of its ancestors.  parents[sequence][i] is the node that
+ * node i follows, below i; -1: the sequence itself.  A node with any other parent, or whose place is below zero, is not
+ * there, nor is what follows it: its row is zeros, its key seen by none.  Up to MI355_MAX_TREE_NODES nodes; types, strides,
+ * alignment, and what is out of range or infinite, as there. */
+#define MI355_MAX_TREE_NODES 1024
+int mi355_tree_attention(void const *q, long long q_stride, void *out, long long out_stride, mi355_paged_cache const *cache,
+                         int const *table, int table_width, int const *lengths, int const *parents, int sequences, int nodes,
+                         int q_heads, float scale);
+/* mi355_paged_attention within a window and to the first tokens: new token t of `new` of a sequence sees the keys j < L =
+ * lengths[sequence] - (new - 1 - t) with j >= L - window (any, where window is 0) or j < sinks.  `tokens` rows of q and out;
+ * starts null: tokens / sequences of them, a whole number, for each sequence; else starts[sequence] .. starts[sequence + 1] - 1,
+ * ascending from 0 to at most tokens, none or any number (out of order, rows may be left as they were); rows of out from
+ * starts[sequences] on are left as they were.  Types, strides, alignment, and what is out of range or infinite, as there. */
+int mi355_window_attention(void const *q, long long q_stride, void *out, long long out_stride, mi355_paged_cache const *cache,
+                           int const *table, int table_width, int const *lengths, int const *starts, int sequences, int tokens,
+                           int q_heads, float scale, int window, int sinks);
+/* Of softmax(scale * logits[row]), `vocabulary` logits a row (fp16, bf16 or fp32), rows `stride` elements apart, scale above zero:
+ * log_probs[row][i] of tokens[row][i], i < asked (minus infinity for one outside the vocabulary), entropy[row], and the `top` most
+ * probable tokens, of equal logits the lower index first, in top_tokens[row][..], their log probabilities in top_log_probs.
+ * Natural units; sums in 32 bits.  A logit of minus infinity has no probability and is no top token: -1 and minus infinity where
+ * others are too few.  A row of these alone: minus infinity, entropy 0, no top tokens.  A row with a NaN or plus infinity: NaN and -1.
+ * Up to MI355_MAX_TOP top tokens, a vocabulary of up to MI355_MAX_VOCABULARY; tokens and log_probs may be null where asked is 0,
+ * the top ones where top is. */
+#define MI355_MAX_TOP 64
+#define MI355_MAX_VOCABULARY (1 << 30)
+int mi355_log_probabilities(void const *logits, long long stride, int const *tokens, float *log_probs, float *entropy,
+                            float *top_log_probs, int *top_tokens, int rows, int asked, int top, int vocabulary, float scale,
+                            int type);
 
 /* ---- timing -----------------------------------------------------------------
  * cudaEvent pairs of every profile() in the reference (e.g. matmul_kernel.cu:63-70). */

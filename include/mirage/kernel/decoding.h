@@ -81,5 +81,48 @@ public:
   void run(void) const override;
 };
 
+// Attention of a tree of drafted tokens of every sequence: as paged attention, but of the new tokens a row sees its own node
+// of the tree and that one's ancestors.  parents [sequences, nodes], nodes = new tokens of a sequence, up to 1024: the node
+// that node i follows, one before it; -1: it follows the sequence itself.  The keys of node i are at place
+// length - nodes + i.  A node with any other parent, or a place below zero, is not there, nor is what follows it: its row is
+// zeros and no row sees its key (so fewer drafts are padded).  Values, scores and page numbers that are out of order: as in
+// paged attention.
+class KNTreeAttentionOp : public KNDecodingOp {
+public:
+  KNTreeAttentionOp(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table, DTensor const &lengths,
+                    DTensor const &parents, float scale, bool heads_first);
+  void run(void) const override;
+  float scale;
+  bool heads_first;
+};
+
+// Attention within a window, and to the first tokens of the sequence: as paged attention, but new token t sees the keys j <
+// L = length - (new - 1 - t) with j >= L - window (all, where window is 0) or j < sinks.  One new token of every sequence, whole
+// prompts, or anything between; with starts [sequences + 1], ascending from 0, sequence b's new tokens are the rows starts[b] to
+// starts[b + 1] - 1 of q, and rows from the last of them on are left as they were; without, every sequence has as many.
+class KNWindowAttentionOp : public KNDecodingOp {
+public:
+  KNWindowAttentionOp(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table, DTensor const &lengths,
+                      DTensor const *starts, float scale, int window, int sinks, bool heads_first);
+  void run(void) const override;
+  float scale;
+  int window, sinks;
+  bool heads_first;
+};
+
+// Of logits [rows, vocabulary] (or their first two dimensions as one; fp16, bf16 or DT_FLOAT32), times a scale above zero, as
+// a distribution: the log probabilities of tokens [rows] or [rows, asked] (minus infinity for one outside the vocabulary), of
+// the same shape; its entropy [rows]; and for top > 0 the `top` most probable tokens of every row, of equal logits the lower
+// index first, [rows, top], behind their log probabilities.  Up to 64; a token without probability is none of them: -1, minus
+// infinity.  Everything in natural units, DT_FLOAT32.  A row of minus infinities has log probabilities of minus infinity,
+// entropy zero and no top tokens; one with a NaN or plus infinity NaN for all numbers, and -1.
+class KNLogProbabilitiesOp : public KNDecodingOp {
+public:
+  KNLogProbabilitiesOp(DTensor const &logits, DTensor const &tokens, int top, float scale);
+  void run(void) const override;
+  int top;
+  float scale;
+};
+
 }  // namespace kernel
 }  // namespace mirage

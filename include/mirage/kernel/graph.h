@@ -74,6 +74,17 @@ public:
   std::vector<DTensor> verify_drafts(DTensor const &target, DTensor const *draft, DTensor const &tokens, DTensor const &uniforms);
   KNOperator *create_verify_drafts_op(DTensor const &target, DTensor const *draft, DTensor const &tokens,
                                       DTensor const &uniforms);
+  DTensor tree_attention(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table, DTensor const &lengths,
+                         DTensor const &parents, float scale, bool heads_first = false);
+  KNOperator *create_tree_attention_op(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table,
+                                       DTensor const &lengths, DTensor const &parents, float scale, bool heads_first);
+  DTensor window_attention(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table, DTensor const &lengths,
+                           DTensor const *starts, float scale, int window, int sinks = 0, bool heads_first = false);
+  KNOperator *create_window_attention_op(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table,
+                                         DTensor const &lengths, DTensor const *starts, float scale, int window, int sinks,
+                                         bool heads_first);
+  std::vector<DTensor> log_probabilities(DTensor const &logits, DTensor const &tokens, int top = 0, float scale = 1.0f);
+  KNOperator *create_log_probabilities_op(DTensor const &logits, DTensor const &tokens, int top, float scale);
 
   // Whether the graph has an operator of a decoding step.  Its inputs are then what a program serves from -- caches,
   // page tables, weights -- and profiles and layout searches leave them as they are (inputs of others are filled).

@@ -54,6 +54,9 @@ enum KNOperatorType {
   KN_ROTARY_APPEND_OP = 1013,
   KN_PAGED_ATTENTION_OP = 1014,
   KN_VERIFY_DRAFTS_OP = 1015,
+  KN_TREE_ATTENTION_OP = 1016,
+  KN_WINDOW_ATTENTION_OP = 1017,
+  KN_LOG_PROBABILITIES_OP = 1018,
   KN_CUSTOMIZED_OP = 1999,
 };
 
