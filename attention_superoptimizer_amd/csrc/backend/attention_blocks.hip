@@ -1,6 +1,10 @@
 // Attention of trees and within windows over a paged key-value cache: entry points, and the kernels of fp16 values
 // (attention_blocks.h).
 #include "attention_blocks.h"
+#include "slices.h"
+#ifndef ROWS_LIMIT
+#define ROWS_LIMIT 64
+#endif
 
 namespace mi355 {
 
@@ -68,7 +72,60 @@ int fill(BlockParams &P, char const *name, void const *q, long long q_stride, vo
   return MI355_OK;
 }
 
+// Few rows of a key-value head, as many in every sequence: a head's keys are dealt over workgroups, a wavefront has 32 of them at a time to
+// itself (paged_attention.h), and reading the cache is what counts.
+bool few_rows(BlockParams const &P) {
+  long long const rows = (long long)P.new_tokens * P.group;
+  return P.starts == nullptr && rows <= ROWS_LIMIT && P.new_tokens <= 64 &&
+         !paged::too_many_units(P.kv_heads, rows, (long long)P.table_width * P.page_size);
+}
+
+int launch_few(BlockParams const &B, int type, bool tree) {
+  paged::MaskedParams P{};
+  P.k = B.k;
+  P.v = B.v;
+  P.q_stride = B.q_stride;
+  P.out_stride = B.out_stride;
+  P.page_step = B.page_step;
+  P.token_step = B.token_step;
+  P.head_step = B.head_step;
+  P.parts = static_cast<float *>(state().scratch());
+  P.tickets = state().queue_join_tickets();
+  P.pages = B.pages;
+  P.page_size = B.page_size;
+  P.head_dim = B.head_dim;
+  P.table_width = B.table_width;
+  P.new_tokens = B.new_tokens;
+  P.group = B.group;
+  P.window = B.window;
+  P.page_magic = B.page_magic;
+  P.group_magic = B.group_magic;
+  P.q_keep = B.q_keep;
+  P.q_flip = B.q_flip;
+  P.scale = B.scale;
+  P.sinks = B.sinks;
+  long long const keys = (long long)B.table_width * B.page_size, rows = (long long)B.new_tokens * B.group;
+  long long const seen = B.window != 0 ? (long long)B.window + B.new_tokens - 1 + B.sinks : keys;
+  P.most_keys = (int)(seen < keys ? seen : keys);
+  // loads that pass the caches: as in mi355_paged_attention
+  long long const visible = (long long)B.sequences * P.most_keys, all = (long long)B.pages * B.page_size;
+  bool const passing = 4 * (visible < all ? visible : all) * B.kv_heads * B.head_dim > 192LL << 20;
+  long long const slice = paged::sequences_at_once(B.kv_heads, rows, keys);
+  return in_slices(B.sequences, slice, [&](long long at, long long count) -> int {
+    P.sequences = (int)count;
+    P.q = static_cast<char const *>(B.q) + 2 * at * B.new_tokens * B.q_stride;
+    P.out = static_cast<char *>(B.out) + 2 * at * B.new_tokens * B.out_stride;
+    P.table = B.table + at * B.table_width;
+    P.lengths = B.lengths + at;
+    P.parents = tree ? B.parents + at * B.new_tokens : nullptr;
+    return type == MI355_TYPE_F16 ? paged::launch_masked_f16(P, B.kv_heads, passing, tree) : paged::launch_masked_bf16(P, B.kv_heads, passing, tree);
+  });
+}
+
 int launch(BlockParams &P, int type, bool tree) {
+  if (few_rows(P)) {
+    return launch_few(P, type, tree);
+  }
   P.row_blocks = (int)(((long long)P.new_tokens * P.group + kRows - 1) / kRows);
   return type == MI355_TYPE_F16 ? launch_f16(P, tree) : launch_bf16(P, tree);
 }

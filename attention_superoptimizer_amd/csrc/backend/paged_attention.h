@@ -46,6 +46,20 @@ struct PagedParams {
   float scale;                       // its magnitude, times log2 e: weights are powers of two
 };
 
+// Which keys a row sees: those before its own place (the last `window` of them); with a window also the first of the sequence,
+// which then run on into the window without a gap: key j of the run is key j of the sequence below `kept`, and j + shift from there
+// on; or, in a tree of up to 64 new tokens, those before the tree, its ancestors and itself.
+enum Mask { kPlain, kFirstKeys, kTree };
+struct MaskedParams : PagedParams {
+  int const *parents;
+  int sinks;
+  int most_keys;  // that a sequence's rows see together, at most
+};
+inline long long most_keys_of(PagedParams const &P) { return (long long)P.table_width * P.page_size; }
+inline long long most_keys_of(MaskedParams const &P) { return P.most_keys; }
+template <int MASK>
+using ParamsOf = std::conditional_t<MASK == kPlain, PagedParams, MaskedParams>;
+
 // n / d for 0 <= n < 2^31 - d by magic = 2^32 / d, rounded up (0 for d = 1): one too many at most
 __device__ __forceinline__ int quotient(int n, int d, unsigned magic) {
   int const q = magic == 0 ? n : (int)__umulhi((uint32_t)n, magic);
@@ -56,6 +70,8 @@ inline unsigned magic_of(int d) { return d == 1 ? 0 : (unsigned)(((1ull << 32) +
 // The two units of this operator: the kernels of a type are compiled in one of them each, side by side.
 int launch_f16(PagedParams const &P, int kv_heads, bool passing);
 int launch_bf16(PagedParams const &P, int kv_heads, bool passing);
+int launch_masked_f16(MaskedParams const &P, int kv_heads, bool passing, bool tree);
+int launch_masked_bf16(MaskedParams const &P, int kv_heads, bool passing, bool tree);
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
@@ -168,9 +184,10 @@ struct Span {
   int first, to;  // the keys that any row sees
   int from;       // the tile that the first of them lies in
   int units;     // at least one: a head without keys has its zeros to be written
+  int kept, shift;  // of a run
 };
-template <int UNIT>
-__device__ __forceinline__ Span span_of(PagedParams const &P, int told) {  // of the sequence with that length
+template <int UNIT, int MASK>
+__device__ __forceinline__ Span span_of(ParamsOf<MASK> const &P, int told) {  // of the sequence with that length
   int const most = P.table_width * P.page_size;
   int const length = told < 0 ? 0 : (told < most ? told : most);
   int const first = P.window != 0 ? length - (P.new_tokens - 1) - P.window : 0;  // (no underflow: the host bounds both)
@@ -178,7 +195,14 @@ __device__ __forceinline__ Span span_of(PagedParams const &P, int told) {  // of
   s.first = first > 0 ? first : 0;
   s.from = s.first & ~(kTile - 1);
   s.to = length;
-  s.units = length > s.from ? (length - s.from + UNIT - 1) / UNIT : 1;
+  s.kept = s.shift = 0;
+  if constexpr (MASK == kFirstKeys) {
+    s.kept = P.sinks < s.first ? P.sinks : s.first;
+    s.shift = s.first - s.kept;
+    s.to = length - s.shift;
+    s.first = s.from = 0;
+  }
+  s.units = s.to > s.from ? (s.to - s.from + UNIT - 1) / UNIT : 1;
   return s;
 }
 
@@ -240,9 +264,9 @@ constexpr int per_compute_unit() {
 
 // DP: the head size, rounded up; RG: groups of 16 rows; WAVES: wavefronts of a workgroup; PASSING: keys and values are not to
 // be kept in the caches.
-template <class T, int DP, int RG, int WAVES, bool PASSING>
-__global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVES>() + 3) / 4)) void paged_attention_kernel(PagedParams const P) {
-  fetch_kernel_arguments<sizeof(PagedParams), 1>();  // one trip for all of them
+template <class T, int DP, int RG, int WAVES, bool PASSING, int MASK>
+__global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVES>() + 3) / 4)) void paged_attention_kernel(ParamsOf<MASK> const P) {
+  fetch_kernel_arguments<sizeof(ParamsOf<MASK>), 1>();  // one trip for all of them
   constexpr int kWaves = WAVES, kThreads = 64 * WAVES, kUnit = kTile * WAVES, kIds = kIdsOf<WAVES>;
   constexpr int C = DP / 8, LOADS = kTile * C / 64, KK = DP / 32, DB = DP / 16;
   typedef typename Vec<T>::x8 x8;
@@ -261,11 +285,11 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
   // This workgroup's units.  Every head cut into equal parts of at most `run` units, a workgroup each, where that gives
   // no more parts than workgroups; otherwise (heads shorter than a run) runs of units that go on from one head to the next.
   int const own_length = lane < P.sequences ? P.lengths[lane] : 0;
-  int const own_units = lane < P.sequences ? span_of<kUnit>(P, own_length).units : 0;
+  int const own_units = lane < P.sequences ? span_of<kUnit, MASK>(P, own_length).units : 0;
   auto over_sequences = [&](auto value) {  // the sum of value(units of a sequence)
     int x = lane < P.sequences ? value(own_units) : 0;
     for (int b = lane + 64; b < P.sequences; b += 64) {
-      x += value(span_of<kUnit>(P, P.lengths[b]).units);
+      x += value(span_of<kUnit, MASK>(P, P.lengths[b]).units);
     }
     return __builtin_amdgcn_readlane(wave_upto(x), 63) * P.heads;
   };
@@ -290,7 +314,7 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
       return;  // (fewer parts than workgroups)
     }
     int const b = base + lane, its = base == 0 ? own_length : (b < P.sequences ? P.lengths[b] : 0);
-    int units = base == 0 ? own_units : (b < P.sequences ? span_of<kUnit>(P, its).units : 0);
+    int units = base == 0 ? own_units : (b < P.sequences ? span_of<kUnit, MASK>(P, its).units : 0);
     units = apart ? parts_of(units) : units;
     int const upto = wave_upto(units) * P.heads;
     uint64_t const past = __ballot(before + upto > unit);
@@ -303,7 +327,7 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
     }
     before += __builtin_amdgcn_readlane(upto, 63);
   }
-  Span span = span_of<kUnit>(P, length);
+  Span span = span_of<kUnit, MASK>(P, length);
   int const cuts = apart ? parts_of(span.units) : span.units;
   int head = (unit - before) / cuts, first = (unit - before) - head * cuts, part_index = first;
   int kv = P.row_blocks == 1 ? head : head / P.row_blocks, row_block = head - kv * P.row_blocks;
@@ -339,6 +363,10 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
     auto as_scaled = [&](uintx4 x) { return uintx4{(x[0] & P.q_keep) ^ P.q_flip, (x[1] & P.q_keep) ^ P.q_flip, (x[2] & P.q_keep) ^ P.q_flip, (x[3] & P.q_keep) ^ P.q_flip}; };
     uintx4 q[KK];  // of one group of rows
     int limit[RG], least[RG];
+    int parent = -2;  // of a tree: node `lane`'s
+    if constexpr (MASK == kTree) {
+      parent = lane < P.new_tokens ? P.parents[(long long)sequence * P.new_tokens + lane] : -2;
+    }
     if constexpr (RG == 1) {
 #pragma unroll
       for (int kk = 0; kk < KK; kk++) {
@@ -358,8 +386,43 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
     // the keys that every row sees lie between these (rows of a block are in the order of their tokens)
     int const last_row = row0 + 16 * RG < R ? row0 + 16 * RG - 1 : R - 1;
     bool const one = P.new_tokens == 1;
-    int const all_limit = span.to - (one ? 0 : P.new_tokens - 1 - quotient(row0, P.group, P.group_magic));
+    int all_limit = span.to - (one ? 0 : P.new_tokens - 1 - quotient(row0, P.group, P.group_magic));
     int const all_least = P.window != 0 ? span.to - (one ? 0 : P.new_tokens - 1 - quotient(last_row, P.group, P.group_magic)) - P.window : 0;
+
+    // the nodes of a tree that a row sees, a bit each; none where an ancestor is not there
+    uint64_t above[RG];
+    int const context = span.to - P.new_tokens;
+    auto climb = [&]() {
+      bool all = true;
+      int at[RG];
+#pragma unroll
+      for (int r = 0; r < RG; r++) {
+        int const row = row0 + 16 * r + c, t = row < R ? (P.new_tokens == 1 ? 0 : quotient(row, P.group, P.group_magic)) : -2;
+        at[r] = t >= 0 && context + t >= 0 ? t : -2;
+        above[r] = 0;
+      }
+      for (bool some = true; some;) {
+        some = false;
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+          int const p = __shfl(parent, at[r] & 63, 64);
+          if (at[r] >= 0) {
+            above[r] |= 1ull << at[r];
+            at[r] = p >= -1 && p < at[r] && (p < 0 || context + p >= 0) ? p : -2;
+          }
+          some = some || at[r] >= 0;
+        }
+        some = __any(some);
+      }
+#pragma unroll
+      for (int r = 0; r < RG; r++) {
+        bool const is = at[r] == -1;
+        above[r] = is ? above[r] : 0;
+        limit[r] = is && context > 0 ? context : 0;
+        all = all && (is || row0 + 16 * r + c >= R);
+      }
+      all_limit = __all(all) ? context : 0;
+    };
 
     floatx4 acc[RG][DB];
     float m[RG], sum[RG];
@@ -378,15 +441,23 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
     uint64_t const k_base = reinterpret_cast<uint64_t>(P.k) + 16ull * kv * P.head_step, v_base = reinterpret_cast<uint64_t>(P.v) + 16ull * kv * P.head_step;
 
     // as many units at a time as the page numbers in LDS cover
-    int const fit = P.page_size < 1 << 16 ? (kIds - 1) * P.page_size / kUnit : 1 << 17;
+    int const fit = P.page_size < 1 << 16 ? (kIds - (MASK == kFirstKeys ? 3 : 1)) * P.page_size / kUnit : 1 << 17;
     for (int part = 0; part < units; part += fit) {
       int const part_units = units - part < fit ? units - part : fit;
       int const key0 = span.from + (first + part) * kUnit, key1 = key0 + part_units * kUnit < span.to ? key0 + part_units * kUnit : span.to;
-      int const page0 = quotient(key0, P.page_size, P.page_magic);
-      int const numbers = key1 > key0 ? quotient(key1 - 1, P.page_size, P.page_magic) + 1 - page0 : 0;
+      int page0 = quotient(key0, P.page_size, P.page_magic), kept_pages = 0, kept_page0 = 0;
+      int numbers = key1 > key0 ? quotient(key1 - 1, P.page_size, P.page_magic) + 1 - page0 : 0;
+      if constexpr (MASK == kFirstKeys) {  // the pages of the run's keys below `kept`, then those of the others
+        int const later = key0 > span.kept ? key0 : span.kept;
+        kept_page0 = page0;
+        kept_pages = key0 < span.kept && key1 > key0 ? quotient((key1 < span.kept ? key1 : span.kept) - 1, P.page_size, P.page_magic) + 1 - kept_page0 : 0;
+        page0 = later < key1 ? quotient(later + span.shift, P.page_size, P.page_magic) : 0;
+        numbers = kept_pages + (later < key1 ? quotient(key1 - 1 + span.shift, P.page_size, P.page_magic) + 1 - page0 : 0);
+        page0 -= kept_pages;
+      }
       __syncthreads();  // (the numbers of the part before, or the tiles as room for sums, are read)
       for (int i = tid; i < numbers; i += kThreads) {
-        ids[i] = table[page0 + i];
+        ids[i] = table[i < kept_pages ? kept_page0 + i : page0 + i];
       }
       if constexpr (RG == 1) {
 #pragma unroll
@@ -394,6 +465,9 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
           q[kk] = part == 0 ? as_scaled(q[kk]) : q[kk];
           asm volatile("" : "+v"(q[kk]));
         }
+      }
+      if constexpr (MASK == kTree) {
+        asm volatile("" : "+v"(parent));
       }
       __syncthreads();
 
@@ -403,9 +477,9 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
       uint32_t at[LOADS];     // where the rows begin that this lane loads chunks of, in 16 bytes; all ones: zeros
       uint32_t there = 0;     // keys that exist, a bit each
       auto locate = [&](int tile) {
-        int const key = mine + tile * kUnit + lane % kTile;
+        int const in_run = mine + tile * kUnit + lane % kTile, key = MASK != kFirstKeys || in_run < span.kept ? in_run : in_run + span.shift;
         int const page = quotient(key, P.page_size, P.page_magic);
-        int const number = key >= span.first && key < key1 ? ids[page - page0] : -1;
+        int const number = in_run >= span.first && in_run < key1 ? ids[page - (MASK == kFirstKeys && in_run < span.kept ? kept_page0 : page0)] : -1;
         bool const is = (unsigned)number < (unsigned)P.pages;
         there = (uint32_t)__ballot(is);
         uint32_t const step = is ? (uint32_t)number * P.page_step + (uint32_t)(key - page * P.page_size) * P.token_step : ~0u;
@@ -431,6 +505,9 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
         locate(0);
         load(k_base, k_lds, Keys{});
         load(v_base, v_lds, Values{});
+        if constexpr (MASK == kTree) {
+          climb();
+        }
       }
       for (int tile = 0; tile < tiles; tile++) {
         int const key = mine + tile * kUnit;
@@ -471,6 +548,7 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
         // that does
         bool const whole = is_there == ~0u && key >= all_least && key + kTile <= all_limit;
         uintx4 p[RG], rest[RG];
+        uint32_t seen_by[RG];
 #pragma unroll
         for (int r = 0; r < RG; r++) {
           float x[8];
@@ -483,6 +561,15 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
             uint32_t seen = is_there;
             seen = upto <= 0 ? 0 : (upto < kTile ? seen & ((1u << upto) - 1) : seen);
             seen = from <= 0 ? seen : (from < kTile ? seen & ~((1u << from) - 1) : 0);
+            if constexpr (MASK == kFirstKeys) {
+              int const first_keys = (P.sinks < limit[r] ? P.sinks : limit[r]) - key;
+              seen |= is_there & (first_keys <= 0 ? 0 : (first_keys < kTile ? (1u << first_keys) - 1 : ~0u));
+            }
+            if constexpr (MASK == kTree) {
+              int const past = key - context;
+              seen |= is_there & (uint32_t)(past >= 0 ? (past < 64 ? above[r] >> past : 0) : (past > -kTile ? above[r] << -past : 0));
+            }
+            seen_by[r] = seen;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
               x[e] = (seen >> (16 * (e / 4) + 4 * g + e % 4)) & 1 ? x[e] : -INFINITY;
@@ -560,7 +647,7 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
                 w[r] = e == at_e ? static_cast<float>(__builtin_bit_cast(x8, p[r])[e]) + static_cast<float>(__builtin_bit_cast(x8, rest[r])[e]) : w[r];
               }
               w[r] = __shfl(w[r], holder, 64);
-              sees[r] = key + j < limit[r] && key + j >= least[r];
+              sees[r] = MASK == kPlain ? key + j < limit[r] && key + j >= least[r] : (seen_by[r] >> j & 1) != 0;
             }
 #pragma unroll
             for (int d = 0; d < DB; d++) {
@@ -809,22 +896,22 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
       before = unit;
       sequence++;
       kv = 0;
-      span = span_of<kUnit>(P, __builtin_amdgcn_readfirstlane(next_length));
+      span = span_of<kUnit, MASK>(P, __builtin_amdgcn_readfirstlane(next_length));
     }
     __syncthreads();  // (`stat`, `is_last` and the tiles are free again)
   }
 }
 
-template <class T, int DP, int RG, int WAVES, bool PASSING>
-int launch_paged(PagedParams P, int kv_heads) {
-  auto *fn = paged_attention_kernel<T, DP, RG, WAVES, PASSING>;
+template <class T, int DP, int RG, int WAVES, bool PASSING, int MASK>
+int launch_paged(ParamsOf<MASK> P, int kv_heads) {
+  auto *fn = paged_attention_kernel<T, DP, RG, WAVES, PASSING, MASK>;
   constexpr int kUnit = kTile * WAVES, lds = lds_bytes<DP, RG, WAVES>(), per_unit = per_compute_unit<DP, RG, WAVES>();
   static_assert(lds <= 160 * 1024, "LDS of a compute unit");
   int const rows = P.new_tokens * P.group;
   P.row_blocks = (rows + 16 * RG - 1) / (16 * RG);
   P.heads = kv_heads * P.row_blocks;
   // workgroups that fit the chip together
-  long long const most = (long long)P.sequences * P.heads * (((long long)P.table_width * P.page_size + kUnit - 1) / kUnit + 1);
+  long long const most = (long long)P.sequences * P.heads * ((most_keys_of(P) + kUnit - 1) / kUnit + 1);
   long long const room = (long long)(state().scratch_bytes / (2 * part_floats<DP, RG>() * sizeof(float)));
   long long const fit = room < 256LL * per_unit ? room : 256LL * per_unit;
   unsigned const grid = (unsigned)(most < fit ? most : fit);
@@ -849,56 +936,56 @@ int launch_paged(PagedParams P, int kv_heads) {
 // Eight workgroups of one wavefront for thousands of heads that are short: no wavefront waits for another at a head's end (four
 // and one: 93 and 74 us of 1024 sequences x 8 heads x 100 keys, 355 and 244 of 4096 x 8 x 100, 181 and 177 of 1024 x 8 x 400;
 // against it 98 and 104 of 64 x 8 x 4096, 33.4 and 33.2 of 128 x 8 x 500, 7.7 and 11.4 of 64 x 8 x 100).
-template <class T, int DP, int RG>
-int launch_group(PagedParams const &P, int kv_heads, bool passing) {
+template <class T, int DP, int RG, int MASK>
+int launch_group(ParamsOf<MASK> const &P, int kv_heads, bool passing) {
   if constexpr ((DP <= 128 && RG <= 2) || (DP <= 64 && RG == 3)) {
     long long const heads = (long long)P.sequences * kv_heads * ((P.new_tokens * P.group + 16 * RG - 1) / (16 * RG));
-    long long const keys = (long long)P.table_width * P.page_size, units = heads * ((keys + 4 * kTile - 1) / (4 * kTile));
+    long long const keys = most_keys_of(P), units = heads * ((keys + 4 * kTile - 1) / (4 * kTile));
     if constexpr (RG == 1) {
       if (one_wavefront(heads, P.new_tokens * P.group, keys)) {
-        return passing ? launch_paged<T, DP, RG, 1, true>(P, kv_heads) : launch_paged<T, DP, RG, 1, false>(P, kv_heads);
+        return passing ? launch_paged<T, DP, RG, 1, true, MASK>(P, kv_heads) : launch_paged<T, DP, RG, 1, false, MASK>(P, kv_heads);
       }
     }
     if constexpr (RG <= 2) {
       if (passing && keys >= 1024) {
-        return launch_paged<T, DP, RG, (DP <= 64 ? 4 : 8), true>(P, kv_heads);
+        return launch_paged<T, DP, RG, (DP <= 64 ? 4 : 8), true, MASK>(P, kv_heads);
       }
     }
     bool const few = RG == 1 ? heads <= 96 : heads <= 48 || (heads <= 256 && heads * units <= 300 << 10);
     if (few && units >= 512) {
-      return launch_paged<T, DP, RG, 8, false>(P, kv_heads);
+      return launch_paged<T, DP, RG, 8, false, MASK>(P, kv_heads);
     }
   }
   if constexpr (DP > 128) {
     if (passing) {
-      return launch_paged<T, DP, RG, 4, true>(P, kv_heads);
+      return launch_paged<T, DP, RG, 4, true, MASK>(P, kv_heads);
     }
   }
-  return launch_paged<T, DP, RG, 4, false>(P, kv_heads);
+  return launch_paged<T, DP, RG, 4, false, MASK>(P, kv_heads);
 }
 
-template <class T, int DP>
-int launch_rows(PagedParams const &P, int kv_heads, bool passing) {
+template <class T, int DP, int MASK>
+int launch_rows(ParamsOf<MASK> const &P, int kv_heads, bool passing) {
   long long const rows = (long long)P.new_tokens * P.group;
   if (rows <= 16) {
-    return launch_group<T, DP, 1>(P, kv_heads, passing);
+    return launch_group<T, DP, 1, MASK>(P, kv_heads, passing);
   }
   if (rows <= 32 || DP > 128) {
-    return launch_group<T, DP, 2>(P, kv_heads, passing);
+    return launch_group<T, DP, 2, MASK>(P, kv_heads, passing);
   }
   if constexpr (DP <= 128) {
-    return rows <= 48 ? launch_group<T, DP, 3>(P, kv_heads, passing) : launch_group<T, DP, 4>(P, kv_heads, passing);
+    return rows <= 48 ? launch_group<T, DP, 3, MASK>(P, kv_heads, passing) : launch_group<T, DP, 4, MASK>(P, kv_heads, passing);
   }
   return MI355_OK;
 }
 
-template <class T>
-int launch_head(PagedParams const &P, int kv_heads, bool passing) {
-  return P.head_dim <= 64    ? launch_rows<T, 64>(P, kv_heads, passing)
-         : P.head_dim <= 96  ? launch_rows<T, 96>(P, kv_heads, passing)
-         : P.head_dim <= 128 ? launch_rows<T, 128>(P, kv_heads, passing)
-         : P.head_dim <= 192 ? launch_rows<T, 192>(P, kv_heads, passing)
-                             : launch_rows<T, 256>(P, kv_heads, passing);
+template <class T, int MASK = kPlain>
+int launch_head(ParamsOf<MASK> const &P, int kv_heads, bool passing) {
+  return P.head_dim <= 64    ? launch_rows<T, 64, MASK>(P, kv_heads, passing)
+         : P.head_dim <= 96  ? launch_rows<T, 96, MASK>(P, kv_heads, passing)
+         : P.head_dim <= 128 ? launch_rows<T, 128, MASK>(P, kv_heads, passing)
+         : P.head_dim <= 192 ? launch_rows<T, 192, MASK>(P, kv_heads, passing)
+                             : launch_rows<T, 256, MASK>(P, kv_heads, passing);
 }
 
 }  // namespace paged
