@@ -34,6 +34,10 @@ struct BlockParams {
   int const *parents;  // of trees
   int pages, page_size, head_dim, table_width, sequences, tokens, new_tokens, group, kv_heads, window, sinks;
   int row_blocks;  // of a sequence, where all have new_tokens
+  int blocks;      // of all sequences, at most
+  int slots;       // workgroups that the chip holds together
+  int splits;      // parts that the keys of a block are cut into, at most
+  float *parts;    // of every block and part: sums as the lanes hold them, then reference and sum of weights of its rows
   unsigned page_magic, group_magic;
   uint32_t q_keep, q_flip;
   float scale;
@@ -50,25 +54,24 @@ __device__ __forceinline__ floatx16 mfma(Vec<__bf16>::x8 a, Vec<__bf16>::x8 b, f
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// Where 16-byte chunk `chunk` of row `row` lies in a tile of C chunks a row (64 banks of 4 bytes: sixteen chunks).  Sixteen rows read
-// the same chunk of K; four rows read four chunks of V in a row.
-template <int C, bool VALUES>
+// Where 16-byte chunk `chunk` of row `row` lies in a tile of C chunks a row.  There are 64 banks of 4 bytes, sixteen chunks: sixteen rows in
+// a row that read the same chunk (keys) meet them all, and so do four rows that read four chunks in a row (values).
+template <int C>
 __device__ __forceinline__ int turn_of(int row) {
-  return VALUES ? (C == 8 || C == 24 ? 4 * ((row >> 1) & 1) : C == 12 ? 0 : 4 * (row & 3))
-                : (C == 8 || C == 24 ? (row >> 1) & 7 : C == 12 ? (row >> 2) & 3 : row & 15);
+  return C == 8 || C == 24 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : C == 12 ? row >> 2 & 3 : (row & 3) << 2 | (row >> 2 & 3);
 }
-template <int C, bool VALUES>
+template <int C>
 __device__ __forceinline__ int place_of(int row, int chunk) {
-  int const turn = turn_of<C, VALUES>(row);
+  int const turn = turn_of<C>(row);
   if constexpr ((C & (C - 1)) == 0) {
     return chunk ^ turn;
   }
   int const at = chunk + turn;
   return at >= C ? at - C : at;
 }
-template <int C, bool VALUES>
+template <int C>
 __device__ __forceinline__ int chunk_at(int row, int place) {
-  int const turn = turn_of<C, VALUES>(row);
+  int const turn = turn_of<C>(row);
   if constexpr ((C & (C - 1)) == 0) {
     return place ^ turn;
   }
@@ -84,91 +87,342 @@ __device__ __forceinline__ float over_halves(float x, Op op) {
   return op(a, b);
 }
 
+// sum + the eight elements: two to an instruction
+__device__ __forceinline__ float sum_of(Vec<_Float16>::x8 p, float sum) {
+  typedef _Float16 pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    sum = __builtin_amdgcn_fdot2(pair{p[i], p[i + 1]}, pair{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+  }
+  return sum;
+}
+__device__ __forceinline__ float sum_of(Vec<__bf16>::x8 p, float sum) {
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    sum = __builtin_amdgcn_fdot2_f32_bf16(pair{p[i], p[i + 1]}, pair{(__bf16)1.0f, (__bf16)1.0f}, sum, false);
+  }
+  return sum;
+}
+
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1); }
 
-constexpr int kThreads = 256, kWaves = 4, kIds = 1024;
+constexpr int kThreads = 256, kWaves = 4;
+// Of a part: one sequence, 8 heads of 128, 1000 keys, 48 rows takes 17.2, 13.8 and 15.1 us with four, two and one.
+constexpr int kLeastTiles = 2;
 template <int DP>
-constexpr int kKeys = DP <= 128 ? 64 : 32;  // of a tile
+constexpr int kKeys = DP == 192 ? 32 : 64;  // of a tile
+template <int DP>
+constexpr int kStepsOf = DP == 96 ? 1024 : 2048;  // keys of a run whose places a workgroup holds in LDS (96: three workgroups fit)
 template <int DP>
 constexpr int tile_bytes() { return kKeys<DP> * DP * 2; }
 template <int DP, bool TREE>
-constexpr int lds_bytes() { return 4 * tile_bytes<DP>() + 4 * kIds + (TREE ? 4 * MI355_MAX_TREE_NODES : 0); }
+constexpr int lds_bytes() { return 4 * tile_bytes<DP>() + 4 * kStepsOf<DP> + kStepsOf<DP> / 8 + (TREE ? 4 * MI355_MAX_TREE_NODES : 0); }
+// Workgroups that a compute unit's registers hold, at least.  Heads of 256: one, of tiles of 64 keys (one prompt of 8192 tokens, 32 heads, a window
+// of 1024: 440 us; two of tiles of 32, with registers spilled, 459).
+template <int DP>
+constexpr int kPerUnit = DP <= 192 ? 2 : 1;
 
-template <class T, int DP, bool TREE>
-__global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockParams const P) {
-  fetch_kernel_arguments<sizeof(BlockParams), 1>();
-  constexpr int KT = kKeys<DP>, G = KT / 32, C = DP / 8, LOADS = KT * C / kThreads, KK = DP / 16, DB = DP / 32;
-  typedef typename Vec<T>::x8 x8;
-  typedef typename Vec<T>::x4 x4;
-  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-  int *const ids = reinterpret_cast<int *>(lds + 4 * tile_bytes<DP>());
-  int *const tree = ids + kIds;
-  int const tid = threadIdx.x, lane = tid % 64, wave = tid / 64, h = lane / 32, c = lane % 32;
-  uint32_t const lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void const *)lds;
-
-  // the block: key-value heads side by side (eight of them lie on an XCD each, with the keys that its blocks share)
-  int const kv = (int)blockIdx.x % P.kv_heads;
-  int block = (int)blockIdx.x / P.kv_heads, sequence = 0, row_of_q = 0, new_tokens = P.new_tokens;
+// The rows of a block and the keys that any of them sees.
+struct Block {
+  int sequence, row_of_q, new_tokens, row0, rows, length;
+  int kept, shift, end;  // key j of the run is key j of the sequence below `kept`, j + shift from there on
+  bool is;
+};
+template <bool TREE>
+__device__ __forceinline__ Block block_of(BlockParams const &P, int block) {
+  int const lane = threadIdx.x % 64;
+  Block b{};
   if (P.starts == nullptr) {
-    sequence = block / P.row_blocks;
-    block -= sequence * P.row_blocks;
-    row_of_q = sequence * P.new_tokens;
+    b.sequence = block / P.row_blocks;
+    block -= b.sequence * P.row_blocks;
+    b.row_of_q = b.sequence * P.new_tokens;
+    b.new_tokens = P.new_tokens;
   } else {
     for (int base = 0;; base += 64) {
       if (base >= P.sequences) {
-        return;
+        return b;
       }
-      int const b = base + lane;
+      int const at = base + lane;
       auto start = [&](int i) {
         int const s = P.starts[i];
         return s < 0 ? 0 : (s < P.tokens ? s : P.tokens);
       };
-      int const from = b < P.sequences ? start(b) : 0, to = b < P.sequences ? start(b + 1) : 0;
+      int const from = at < P.sequences ? start(at) : 0, to = at < P.sequences ? start(at + 1) : 0;
       int const its = to > from ? (int)(((long long)(to - from) * P.group + kRows - 1) / kRows) : 0, upto = paged::wave_upto(its);
       uint64_t const past = __ballot(upto > block);
       if (past != 0) {
-        int const at = __builtin_ctzll(past);
-        sequence = base + at;
-        row_of_q = __builtin_amdgcn_readlane(from, at);
-        new_tokens = __builtin_amdgcn_readlane(to, at) - row_of_q;
-        block -= __builtin_amdgcn_readlane(upto - its, at);
+        int const which = __builtin_ctzll(past);
+        b.sequence = base + which;
+        b.row_of_q = __builtin_amdgcn_readlane(from, which);
+        b.new_tokens = __builtin_amdgcn_readlane(to, which) - b.row_of_q;
+        block -= __builtin_amdgcn_readlane(upto - its, which);
         break;
       }
       block -= __builtin_amdgcn_readlane(upto, 63);
     }
   }
-
-  // its rows and the keys that any of them sees, counted as kept + those from `first` on
-  int const R = new_tokens * P.group, row0 = block * kRows, rows = R - row0 < kRows ? R - row0 : kRows;
-  int const most = P.table_width * P.page_size, told = P.lengths[sequence];
-  int const length = told < 0 ? 0 : (told < most ? told : most);
-  auto token_of = [&](int row) { return quotient(row, P.group, P.group_magic); };
-  auto limit_of = [&](int t) { return length - (new_tokens - 1 - t); };
-  int const context = length - new_tokens;  // of a tree
-  int to = TREE ? length : limit_of(token_of(row0 + rows - 1));
+  b.is = true;
+  int const R = b.new_tokens * P.group, most = P.table_width * P.page_size, told = P.lengths[b.sequence];
+  b.row0 = block * kRows;
+  b.rows = R - b.row0 < kRows ? R - b.row0 : kRows;
+  b.length = told < 0 ? 0 : (told < most ? told : most);
+  int const before = b.length - b.new_tokens + 1;  // what the first new token sees, without a window
+  int to = TREE ? b.length : before + quotient(b.row0 + b.rows - 1, P.group, P.group_magic);
   to = to < 0 ? 0 : to;
-  int first = !TREE && P.window != 0 ? limit_of(token_of(row0)) - P.window : 0;
+  int first = !TREE && P.window != 0 ? before + quotient(b.row0, P.group, P.group_magic) - P.window : 0;
   first = first < 0 ? 0 : first;
-  int const kept = P.sinks < first ? P.sinks : first, shift = first - kept, end = to - shift;
+  b.kept = P.sinks < first ? P.sinks : first;
+  b.shift = first - b.kept;
+  b.end = to - b.shift;
+  return b;
+}
 
-  // this lane's row: the run's keys below `always`, and those from `least` up to `limit`
-  int const row = row0 + 32 * wave + c, my_token = token_of(row < R ? row : R - 1);
-  int limit = 0, least = 0, always = 0;
-  if (row < R) {
-    limit = TREE ? context : limit_of(my_token) - shift;
-    least = !TREE && P.window != 0 ? limit - P.window : 0;
-    always = P.sinks < limit ? P.sinks : limit;
+// A row of it: the keys of the run below `always`, and those from `least` up to `limit`; of a tree, those below `limit` (below zero:
+// none) and the token's and its ancestors'.
+struct Row {
+  int row, token, limit, least, always;
+};
+template <bool TREE>
+__device__ __forceinline__ Row row_of(BlockParams const &P, Block const &b, int in_block, int const *tree) {
+  Row r{b.row0 + in_block, 0, 0, 0, 0};
+  r.token = quotient(in_block < b.rows ? r.row : b.row0 + b.rows - 1, P.group, P.group_magic);
+  int const context = b.length - b.new_tokens;
+  if (in_block < b.rows) {
+    r.limit = TREE ? context : context + 1 + r.token - b.shift;
+    r.least = !TREE && P.window != 0 ? r.limit - P.window : 0;
+    r.always = P.sinks < r.limit ? P.sinks : r.limit;
+  }
+  if constexpr (TREE) {  // whether every ancestor is there
+    int at = in_block < b.rows && context + r.token >= 0 ? r.token : -2;
+    while (__any(at >= 0)) {
+      if (at >= 0) {
+        int const p = tree[at];
+        at = p >= -1 && p < at && (p < 0 || context + p >= 0) ? p : -2;
+      }
+    }
+    r.limit = at == -1 ? (r.limit < 0 ? 0 : r.limit) : -1;
+  }
+  return r;
+}
+// weights are at most 2^(bias + kSlack)
+constexpr float kSlack = 6.0f;
+template <class T>
+__device__ __forceinline__ float bias_of(int keys) {
+  return std::is_same<T, _Float16>::value ? 9.0f : (float)(__builtin_clz((unsigned)keys | 1u) - 33) - kSlack;
+}
+
+// A weight of zero does not keep an infinity or NaN among the values out of a sum: rows with one in their result are done again, a
+// wavefront a row, key by key, columns d0 up to d1.  (In the loop over tiles such values would have to be looked for in every tile that
+// not all rows see.)  `r` is the same in every lane.
+template <class T, int DP, bool TREE>
+__device__ void row_again(BlockParams const &P, Block const &b, int kv, Row r, int const *tree, int d0, int d1) {
+  typedef typename Vec<T>::x8 x8;
+  int const lane = threadIdx.x % 64;
+  T const *const q = static_cast<T const *>(P.q) + (long long)(b.row_of_q + r.token) * P.q_stride + (long long)(kv * P.group + r.row - r.token * P.group) * P.head_dim;
+  T *const out = static_cast<T *>(P.out) + (long long)(b.row_of_q + r.token) * P.out_stride + (long long)(kv * P.group + r.row - r.token * P.group) * P.head_dim;
+  int const *const table = P.table + (long long)b.sequence * P.table_width;
+  uint64_t const k_base = reinterpret_cast<uint64_t>(P.k) + 16ull * kv * P.head_step, v_base = reinterpret_cast<uint64_t>(P.v) + 16ull * kv * P.head_step;
+  int const context = b.length - b.new_tokens;
+  // the key of this lane of 64: where it lies, or all ones where the row does not see it
+  auto find = [&](int key) {
+    int const real = key < b.kept ? key : key + b.shift, page = quotient(real, P.page_size, P.page_magic);
+    bool sees = key < b.end && ((key < r.limit && key >= r.least) || (!TREE && key < r.always));
+    if constexpr (TREE) {
+      if (r.limit >= 0) {
+        for (int node = r.token; node >= 0; node = tree[node]) {
+          sees = sees || key == context + node;
+        }
+      }
+    }
+    int const number = sees ? table[page] : -1;
+    return (unsigned)number < (unsigned)P.pages ? (uint32_t)number * P.page_step + (uint32_t)(real - page * P.page_size) * P.token_step : ~0u;
+  };
+  auto score = [&](uint32_t at) {
+    float x = 0.0f;
+    if (at == ~0u) {
+      return -INFINITY;
+    }
+    for (int d = 0; d < P.head_dim; d += 8) {
+      x8 const k = *reinterpret_cast<x8 const *>(k_base + 16ull * (at + d / 8)), a = *reinterpret_cast<x8 const *>(q + d);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        x += static_cast<float>(a[e]) * static_cast<float>(k[e]);
+      }
+    }
+    x = P.q_keep == 0 ? x * 0.0f : x;
+    return (P.q_flip != 0 ? -x : x) * P.scale;
+  };
+  float high = -INFINITY;
+  bool wild = false;
+  for (int key = 0; key < b.end; key += 64) {
+    float const x = score(find(key + lane));
+    wild = wild || x != x;
+    high = fmaxf(high, x);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    high = fmaxf(high, __shfl_xor(high, off, 64));
+  }
+  wild = __any(wild) || high == INFINITY;
+  constexpr int N = (DP + 63) / 64;
+  float total = 0.0f, o[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    o[i] = 0.0f;
+  }
+  float const base = high == -INFINITY ? 0.0f : bias_of<T>(b.end) - high;
+  for (int key = 0; key < b.end && !wild; key += 64) {
+    uint32_t const at = find(key + lane);
+    float const w = at == ~0u ? 0.0f : exp2_fast(score(at) + base);
+    total += w;
+    for (uint64_t left = __ballot(at != ~0u); left != 0; left &= left - 1) {
+      int const j = __builtin_ctzll(left);
+      float const its = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), j));
+      T const *const v = reinterpret_cast<T const *>(v_base + 16ull * (uint32_t)__builtin_amdgcn_readlane((int)at, j));
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        int const d = d0 + 64 * i + lane;
+        if (d < d1) {
+          float const x = static_cast<float>(v[d]);
+          o[i] += __builtin_fabsf(x) == INFINITY && high != -INFINITY ? x : its * x;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    total += __shfl_xor(total, off, 64);
+  }
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    int const d = d0 + 64 * i + lane;
+    if (d < d1) {
+      out[d] = static_cast<T>(wild ? __builtin_nanf("") : (total == 0.0f ? 0.0f : o[i] * (1.0f / total)));
+    }
+  }
+}
+__device__ __forceinline__ Row of_lane(Row r, int lane) {
+  return {__builtin_amdgcn_readlane(r.row, lane), __builtin_amdgcn_readlane(r.token, lane), __builtin_amdgcn_readlane(r.limit, lane),
+          __builtin_amdgcn_readlane(r.least, lane), __builtin_amdgcn_readlane(r.always, lane)};
+}
+// How the blocks of a batch of trees are cut along their keys: a tree's all into as many parts as leave each at most `run` tiles, with the
+// least run for which the parts of all are no more than the workgroups that the chip holds together (P.slots, and the launch's).
+struct Cut {
+  int sequence, parts, before;  // a sequence, the parts of each of its blocks, the workgroups of the sequences before it
+};
+template <int DP>
+__device__ __forceinline__ Cut cut_of(BlockParams const &P, int work, int sequence) {  // of the sequence with that workgroup, or of that one (work -1)
+  int const lane = threadIdx.x % 64, each = P.row_blocks * P.kv_heads, most = P.table_width * P.page_size;
+  auto tiles_of = [&](int i) {
+    int const told = i < P.sequences ? P.lengths[i] : 0, length = told < 0 ? 0 : (told < most ? told : most);
+    int const tiles = (length + kKeys<DP> - 1) / kKeys<DP>;
+    return tiles < 1 ? 1 : (tiles < 1 << 20 ? tiles : 1 << 20);  // (their sum over fewer blocks than slots fits 32 bits)
+  };
+  int const own = tiles_of(lane);
+  auto total = [&](auto value) {
+    int x = lane < P.sequences ? value(own) : 0;
+    for (int i = lane + 64; i < P.sequences; i += 64) {
+      x += value(tiles_of(i));
+    }
+    return __builtin_amdgcn_readlane(paged::wave_upto(x), 63) * each;
+  };
+  int run = (total([](int tiles) { return tiles; }) + P.slots - 1) / P.slots;
+  run = run < kLeastTiles ? kLeastTiles : run;
+  auto parts_of = [&](int tiles) { return (int)(((unsigned)tiles + run - 1) / (unsigned)run); };
+  while (total(parts_of) > P.slots) {
+    run += 1 + run / 16;
+  }
+  Cut cut{-1, 0, 0};
+  for (int base = 0; base < P.sequences; base += 64) {
+    int const i = base + lane, parts = i < P.sequences ? parts_of(base == 0 ? own : tiles_of(i)) : 0, upto = paged::wave_upto(parts) * each;
+    uint64_t const past = work >= 0 ? __ballot(cut.before + upto > work) : (sequence < base + 64 ? 1ull << (sequence - base) : 0);
+    if (past != 0) {
+      int const at = __builtin_ctzll(past);
+      cut.sequence = base + at;
+      cut.parts = __builtin_amdgcn_readlane(parts, at);
+      cut.before += __builtin_amdgcn_readlane(upto - parts * each, at);
+      return cut;
+    }
+    cut.before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return cut;
+}
+// Any other block is cut into as many parts as all may have, of two tiles or more.
+template <int DP>
+__device__ __forceinline__ int parts_of(BlockParams const &P, Block const &b) {
+  int const most = b.end / (kKeys<DP> * kLeastTiles);
+  return most < 1 ? 1 : (most < P.splits ? most : P.splits);
+}
+// of a block's part
+template <int DP>
+constexpr int part_floats() { return kRows * (DP + 2); }
+
+template <class T, int DP, bool TREE>
+__global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kernel(BlockParams const P) {
+  fetch_kernel_arguments<sizeof(BlockParams), 1>();
+  constexpr int KT = kKeys<DP>, G = KT / 32, C = DP / 8, LOADS = KT * C / kThreads, KK = DP / 16, DB = DP / 32, kSteps = kStepsOf<DP>;
+  typedef typename Vec<T>::x8 x8;
+  typedef typename Vec<T>::x4 x4;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  uint64_t *const exist = reinterpret_cast<uint64_t *>(lds + 4 * tile_bytes<DP>());
+  uint32_t *const steps = reinterpret_cast<uint32_t *>(exist + kSteps / 64);
+  int *const tree = reinterpret_cast<int *>(steps + kSteps);
+  int const tid = threadIdx.x, lane = tid % 64, wave = tid / 64, h = lane / 32, c = lane % 32;
+  uint32_t const lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void const *)lds;
+
+  // the block and its part: key-value heads side by side (eight of them lie on an XCD each, with the keys that its blocks share)
+  int const kv = (int)blockIdx.x % P.kv_heads;
+  int item = (int)blockIdx.x / P.kv_heads, split = 0, parts = 1;
+  bool const dealt = TREE && P.sequences > 1;  // parts are, to blocks of different lengths
+  if (P.splits > 1) {
+    if (dealt) {
+      Cut const cut = cut_of<DP>(P, blockIdx.x, 0);
+      if (cut.sequence < 0) {
+        return;
+      }
+      int const rest = ((int)blockIdx.x - cut.before) / P.kv_heads;
+      parts = cut.parts;
+      split = rest / P.row_blocks;
+      item = cut.sequence * P.row_blocks + rest % P.row_blocks;
+    } else {
+      split = item / P.blocks;
+      item -= split * P.blocks;
+    }
+  }
+  Block const b = block_of<TREE>(P, item);
+  if (P.splits > 1 && !dealt) {
+    parts = parts_of<DP>(P, b);
+  }
+  if (!b.is || split >= parts) {
+    return;
+  }
+  if constexpr (TREE) {
+    for (int i = tid; i < b.new_tokens; i += kThreads) {
+      tree[i] = P.parents[(long long)b.sequence * b.new_tokens + i];
+    }
+    __syncthreads();
+  }
+  int const context = b.length - b.new_tokens, kept = b.kept, shift = b.shift;
+  int begin = 0, end = b.end;
+  if (parts > 1) {
+    int const tiles = (b.end + KT - 1) / KT;
+    begin = (int)((long long)tiles * split / parts) * KT;
+    end = (int)((long long)tiles * (split + 1) / parts) * KT;
+    end = end < b.end ? end : b.end;
   }
 
+  Row const r = row_of<TREE>(P, b, 32 * wave + c, tree);
+  bool const is_row = 32 * wave + c < b.rows;
   x8 q[KK];
   {
-    T const *const from = static_cast<T const *>(P.q) + (long long)(row_of_q + my_token) * P.q_stride +
-                          (long long)(kv * P.group + (row < R ? row : R - 1) - my_token * P.group) * P.head_dim;
+    T const *const from = static_cast<T const *>(P.q) + (long long)(b.row_of_q + r.token) * P.q_stride +
+                          (long long)(kv * P.group + (is_row ? r.row - r.token * P.group : 0)) * P.head_dim;
 #pragma unroll
     for (int kk = 0; kk < KK; kk++) {
       int const d = 16 * kk + 8 * h;
       uintx4 x = {0, 0, 0, 0};
-      if (row < R && d < P.head_dim) {
+      if (is_row && d < P.head_dim) {
         x = *reinterpret_cast<uintx4 const *>(from + d);
       }
 #pragma unroll
@@ -177,21 +431,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockPara
       }
       q[kk] = __builtin_bit_cast(x8, x);
     }
-  }
-  if constexpr (TREE) {
-    for (int i = tid; i < new_tokens; i += kThreads) {
-      tree[i] = P.parents[(long long)sequence * new_tokens + i];
-    }
-    __syncthreads();
-    // whether every ancestor is there: else the row sees nothing
-    int at = row < R && context + my_token >= 0 ? my_token : -2;
-    while (__any(at >= 0)) {
-      if (at >= 0) {
-        int const p = tree[at];
-        at = p >= -1 && p < at && (p < 0 || context + p >= 0) ? p : -2;
-      }
-    }
-    limit = at == -1 ? (limit < 0 ? 0 : limit) : -1;
   }
 
   floatx16 acc[DB];
@@ -203,55 +442,74 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockPara
       acc[d][e] = 0.0f;
     }
   }
-  // Weights are at most 2^(bias + kSlack): the reference follows the maximum only where that would be passed, so that sums are seldom
-  // scaled.  fp16: small ones stay above the type's end.  bf16: as values reach the end of 32 bits themselves, n weights add up to less than 1/2.
-  constexpr float kSlack = 6.0f;
-  float const bias = std::is_same<T, _Float16>::value ? 9.0f : (float)(__builtin_clz((unsigned)end | 1u) - 33) - kSlack;
+  // The reference follows the maximum only where weights would pass 2^(bias + kSlack), so that sums are seldom scaled.  fp16: small ones stay
+  // above the type's end.  bf16: as values reach the end of 32 bits themselves, n weights add up to less than 1/2.
+  float const bias = bias_of<T>(b.end);
   uint64_t const k_base = reinterpret_cast<uint64_t>(P.k) + 16ull * kv * P.head_step, v_base = reinterpret_cast<uint64_t>(P.v) + 16ull * kv * P.head_step;
-  int const *const table = P.table + (long long)sequence * P.table_width;
+  int const *const table = P.table + (long long)b.sequence * P.table_width;
 
-  // as many keys at a time as the page numbers in LDS cover
-  int const fit = P.page_size < 1 << 16 ? (kIds - 4) * P.page_size / KT * KT : 1 << 25;
-  for (int part = 0; part < end; part += fit) {
-    int const part_end = end - part < fit ? end : part + fit;
-    auto page_of = [&](int key) { return quotient(key, P.page_size, P.page_magic); };
-    int const kept_page = page_of(part), kept_end = part_end < kept ? part_end : kept;
-    int const kept_pages = part < kept ? page_of(kept_end - 1) + 1 - kept_page : 0;
-    int const later = part > kept ? part : kept, later_page = later < part_end ? page_of(later + shift) : 0;
-    int const later_pages = later < part_end ? page_of(part_end - 1 + shift) + 1 - later_page : 0;
+  // The chunk of its key that this thread loads to each of its places; past the head's end the last one, which queries of zero meet and
+  // no result is taken from.
+  uint32_t chunk_of[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; i++) {
+    int const n = kThreads * i + tid, chunk = chunk_at<C>(n / C, n % C), last = P.head_dim / 8 - 1;
+    chunk_of[i] = chunk < last ? chunk : last;
+  }
+
+  for (int part = begin; part < end; part += kSteps) {
+    int const part_end = end - part < kSteps ? end : part + kSteps;
+    // Where the part's keys lie, in 16 bytes, and which of them exist, a bit each.  In the place of a key that does not any of the 64 that do: it is
+    // masked, and what lies elsewhere may be no number.
     __syncthreads();
-    for (int i = tid; i < kept_pages + later_pages; i += kThreads) {
-      ids[i] = table[i < kept_pages ? kept_page + i : later_page + i - kept_pages];
+    for (int i = tid; i < (part_end - part + 63) / 64 * 64; i += kThreads) {
+      int const key = part + i, real = key < kept ? key : key + shift, page = quotient(real, P.page_size, P.page_magic);
+      int const number = key < part_end ? table[page] : -1;
+      bool const is = (unsigned)number < (unsigned)P.pages;
+      uint64_t const there = __ballot(is);
+      uint32_t const step = (uint32_t)number * P.page_step + (uint32_t)(real - page * P.page_size) * P.token_step;
+      uint32_t const some = there != 0 ? (uint32_t)__builtin_amdgcn_readlane((int)step, __builtin_ctzll(there)) : 0;
+      steps[i] = is ? step : some;
+      if (lane == 0) {
+        exist[i / 64] = there;
+      }
     }
     __syncthreads();
 
-    uint64_t there = 0;  // keys of the tile that exist, a bit each
-    auto load = [&](int at, int buffer) {
-      int const key = at + lane % KT, real = key < kept ? key : key + shift, page = page_of(real);
-      int const number = key < part_end ? ids[key < kept ? page - kept_page : kept_pages + page - later_page] : -1;
-      bool const is = (unsigned)number < (unsigned)P.pages;
-      there = __ballot(is);
-      uint32_t const step = is ? (uint32_t)number * P.page_step + (uint32_t)(real - page * P.page_size) * P.token_step : ~0u;
-      int chunks = P.head_dim / 8;
-      asm volatile("" : "+s"(chunks));
+    // the rows that this thread loads chunks of, looked up a tile before their loads
+    uint32_t from[LOADS];
+    uint64_t there;
+    auto locate = [&](int at) {
+      int const in_part = at < part_end ? at - part : 0;
+#pragma unroll
+      for (int i = 0; i < LOADS; i++) {
+        from[i] = steps[in_part + (kThreads * i + tid) / C] + chunk_of[i];
+      }
+      there = exist[in_part / 64];
+    };
+    auto load = [&](int buffer) {
       uint32_t const base = lds_at + buffer * 2 * tile_bytes<DP>() + 1024 * wave;
 #pragma unroll
       for (int i = 0; i < LOADS; i++) {
-        int const n = kThreads * i + tid, its = n / C, k_chunk = chunk_at<C, false>(its, n % C), v_chunk = chunk_at<C, true>(its, n % C);
-        uint32_t const from = (uint32_t)__shfl((int)step, its, 64);
-        uint64_t const zeros = reinterpret_cast<uint64_t>(&paged::kZeros);
-        paged::load_to_lds<false>(from != ~0u && k_chunk < chunks ? k_base + 16ull * (from + k_chunk) : zeros, base + 16 * kThreads * i);
-        paged::load_to_lds<false>(from != ~0u && v_chunk < chunks ? v_base + 16ull * (from + v_chunk) : zeros,
-                                  base + tile_bytes<DP>() + 16 * kThreads * i);
+        paged::load_to_lds<false>(k_base + 16ull * from[i], base + 16 * kThreads * i);
+      }
+#pragma unroll
+      for (int i = 0; i < LOADS; i++) {
+        paged::load_to_lds<false>(v_base + 16ull * from[i], base + tile_bytes<DP>() + 16 * kThreads * i);
       }
     };
-    load(part, 0);
+    locate(part);
+    load(0);
+    uint64_t next_there = there;
+    locate(part + KT);
     for (int at = part, buffer = 0; at < part_end; at += KT, buffer ^= 1) {
-      uint64_t const is_there = there;
+      uint64_t const is_there = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(next_there >> 32)) << 32 |
+                                (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)next_there);
+      next_there = there;
       paged::wait_loads<0>();
       __syncthreads();  // the tile is here, and everyone is done with the one before
       if (at + KT < part_end) {
-        load(at + KT, buffer ^ 1);
+        load(buffer ^ 1);
       }
       unsigned char const *const k_tile = lds + buffer * 2 * tile_bytes<DP>(), *const v_tile = k_tile + tile_bytes<DP>();
 
@@ -268,21 +526,30 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockPara
 #pragma unroll
         for (int j = 0; j < G; j++) {
           int const its = 32 * j + c;
-          s[j] = mfma(*reinterpret_cast<x8 const *>(k_tile + its * (2 * DP) + 16 * place_of<C, false>(its, 2 * kk + h)), q[kk], s[j]);
+          s[j] = mfma(*reinterpret_cast<x8 const *>(k_tile + its * (2 * DP) + 16 * place_of<C>(its, 2 * kk + h)), q[kk], s[j]);
         }
+      }
+      locate(at + 2 * KT);
+      // operands of the products some ahead of them
+      __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+      for (int i = 0; i < KK * G - 8; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
 
       // element e of s[j]: key 32 j + 8 (e / 4) + 4 h + e % 4 of row c
-      bool const all_there = is_there == (KT == 64 ? ~0ull : 0xffffffffull);
-      if (!all_there || __any(limit < at + KT || least > at)) {
+      int const half = KT == 32 ? (at - part) % 64 : 0;  // of a word of bits
+      bool const all_there = KT == 64 ? is_there == ~0ull : (uint32_t)(is_there >> half) == ~0u;
+      if (!all_there || __any(r.limit < at + KT || r.least > at)) {
         uint32_t seen[G];
 #pragma unroll
         for (int j = 0; j < G; j++) {
-          int const from = at + 32 * j;
-          seen[j] = (bits_below(limit - from) & ~bits_below(least - from)) | (TREE ? 0u : bits_below(always - from));
+          int const first = at + 32 * j;
+          seen[j] = (bits_below(r.limit - first) & ~bits_below(r.least - first)) | (TREE ? 0u : bits_below(r.always - first));
         }
         if constexpr (TREE) {
-          int node = limit >= 0 ? my_token : -1;
+          int node = r.limit >= 0 ? r.token : -1;
           while (__any(node >= 0)) {
             int const place = context + node - at;
             if (node >= 0) {
@@ -296,7 +563,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockPara
         }
 #pragma unroll
         for (int j = 0; j < G; j++) {
-          seen[j] = (seen[j] & (uint32_t)(is_there >> (32 * j))) >> (4 * h);
+          seen[j] = (seen[j] & (uint32_t)(is_there >> (32 * j + half))) >> (4 * h);
 #pragma unroll
           for (int e = 0; e < 16; e++) {
             s[j][e] = (seen[j] >> (8 * (e / 4) + e % 4)) & 1 ? s[j][e] : -INFINITY;
@@ -314,8 +581,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockPara
       }
       top = over_halves(top, [](float a, float b) { return fmaxf(a, b); }) * P.scale;
       if (__any(top > ref + kSlack || (ref == -INFINITY && top > ref))) {
-        float const higher = fmaxf(ref, top), less = exp2_fast(ref - (higher == -INFINITY ? 0.0f : higher));
-        ref = higher;
+        float const most = fmaxf(ref, top), less = exp2_fast(ref - (most == -INFINITY ? 0.0f : most));
+        ref = most;
         sum *= less;
 #pragma unroll
         for (int d = 0; d < DB; d++) {
@@ -323,20 +590,16 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockPara
         }
       }
       float const base = ref == -INFINITY ? 0.0f : bias - ref;
-      x8 p[2 * G];
-#pragma unroll
-      for (int j = 0; j < G; j++) {
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          float const w = exp2_fast(__builtin_fmaf(s[j][e], P.scale, base));
-          sum += w;
-          p[2 * j + e / 8][e % 8] = static_cast<T>(w);
-        }
-      }
 
-      // O^T: lane has columns 32 d + 8 (e / 4) + 4 h + e % 4 of row c
+      // Weights of sixteen keys at a time, and their products with the values.  O^T: lane has columns 32 d + 8 (e / 4) + 4 h + e % 4 of row c.
 #pragma unroll
       for (int k = 0; k < 2 * G; k++) {
+        x8 p;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          p[e] = static_cast<T>(exp2_fast(__builtin_fmaf(s[k / 2][8 * (k % 2) + e], P.scale, base)));
+        }
+        sum = sum_of(p, sum);
 #pragma unroll
         for (int d = 0; d < DB; d++) {
           uint64_t v[2];
@@ -344,21 +607,39 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockPara
           for (int half = 0; half < 2; half++) {
             int const its = 16 * k + 8 * half + 4 * h + lane % 16 / 4, chunk = 4 * d + 2 * (lane / 16 % 2) + lane % 4 / 2;
             typedef short shortx4 __attribute__((ext_vector_type(4)));
-            unsigned char const *const from = v_tile + its * (2 * DP) + 16 * place_of<C, true>(its, chunk) + 8 * (lane % 2);
+            unsigned char const *const at_v = v_tile + its * (2 * DP) + 16 * place_of<C>(its, chunk) + 8 * (lane % 2);
             v[half] = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                       (shortx4 __attribute__((address_space(3))) *)(__attribute__((address_space(3))) void const *)from));
+                                                       (shortx4 __attribute__((address_space(3))) *)(__attribute__((address_space(3))) void const *)at_v));
           }
           uintx4 const both = {(uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1], (uint32_t)(v[1] >> 32)};
-          acc[d] = mfma(__builtin_bit_cast(x8, both), p[k], acc[d]);
+          acc[d] = mfma(__builtin_bit_cast(x8, both), p, acc[d]);
         }
       }
     }
   }
 
   sum = over_halves(sum, [](float a, float b) { return a + b; });
+  if (parts > 1) {  // left as it is, for the kernel below
+    float *const part = P.parts + (long long)blockIdx.x * part_floats<DP>();
+    if (h == 0) {
+      part[kRows * DP + 2 * (32 * wave + c)] = ref;
+      part[kRows * DP + 2 * (32 * wave + c) + 1] = sum;
+    }
+    if (begin < end) {
+#pragma unroll
+      for (int d = 0; d < DB; d++) {
+#pragma unroll
+        for (int four = 0; four < 4; four++) {
+          *reinterpret_cast<paged::floatx4 *>(part + 4 * (((d * kWaves + wave) * 4 + four) * 64 + lane)) =
+              paged::floatx4{acc[d][4 * four], acc[d][4 * four + 1], acc[d][4 * four + 2], acc[d][4 * four + 3]};
+        }
+      }
+    }
+    return;
+  }
   float const by = sum == 0.0f ? 0.0f : 1.0f / sum;
   bool good = true;
-  T *const out = static_cast<T *>(P.out) + (long long)(row_of_q + my_token) * P.out_stride + (long long)(kv * P.group + row - my_token * P.group) * P.head_dim;
+  T *const out = static_cast<T *>(P.out) + (long long)(b.row_of_q + r.token) * P.out_stride + (long long)(kv * P.group + r.row - r.token * P.group) * P.head_dim;
 #pragma unroll
   for (int d = 0; d < DB; d++) {
 #pragma unroll
@@ -366,113 +647,156 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockPara
       x4 y;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        float const o = acc[d][4 * four + e] * by;
-        good = good && __builtin_fabsf(o) < INFINITY;  // (false for NaN)
-        y[e] = static_cast<T>(o);
+        y[e] = static_cast<T>(acc[d][4 * four + e] * by);
       }
       int const at = 32 * d + 8 * four + 4 * h;
-      if (row < R && at < P.head_dim) {
+      if (is_row && at < P.head_dim) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          good = good && __builtin_fabsf(acc[d][4 * four + e] * by) < INFINITY;  // (false for NaN)
+        }
         *reinterpret_cast<x4 *>(out + at) = y;
       }
     }
   }
-
-  // A weight of zero does not keep an infinity or NaN among the values out of a sum: rows with one in their result are done again,
-  // a wavefront a row, key by key.  (In the loop above such values would have to be looked for in every tile that not all rows see.)
-  uint64_t again = __ballot(!good && row < R);
+  uint64_t again = __ballot(!good && is_row);
   again = (again | again >> 32) & 0xffffffffull;
   for (; again != 0; again &= again - 1) {
-    int const which = __builtin_ctzll(again), its_row = row0 + 32 * wave + which, t = token_of(its_row);
-    int const its_limit = __builtin_amdgcn_readlane(limit, which), its_least = __builtin_amdgcn_readlane(least, which);
-    int const its_always = __builtin_amdgcn_readlane(always, which);
-    T const *const its_q = static_cast<T const *>(P.q) + (long long)(row_of_q + t) * P.q_stride + (long long)(kv * P.group + its_row - t * P.group) * P.head_dim;
-    T *const its_out = static_cast<T *>(P.out) + (long long)(row_of_q + t) * P.out_stride + (long long)(kv * P.group + its_row - t * P.group) * P.head_dim;
-    bool const negative = P.q_flip != 0, none = P.q_keep == 0;
-    // the key of this lane of 64: where it lies, or all ones where the row does not see it
-    auto find = [&](int key) {
-      int const real = key < kept ? key : key + shift, page = quotient(real, P.page_size, P.page_magic);
-      bool sees = key < end && ((key < its_limit && key >= its_least) || (!TREE && key < its_always));
-      if constexpr (TREE) {
-        if (its_limit >= 0) {
-          for (int node = t; node >= 0; node = tree[node]) {
-            sees = sees || key == context + node;
-          }
+    row_again<T, DP, TREE>(P, b, kv, of_lane(r, __builtin_ctzll(again)), tree, 0, P.head_dim);
+  }
+}
+
+// The parts of a block together: a workgroup has 32 columns of its 128 rows, a wavefront 32 rows of these, in the order in which the kernel
+// above left them.  Parts are asked for four at a time: one after the other each is a trip to memory.
+template <class T, int DP, bool TREE>
+__global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const P) {
+  fetch_kernel_arguments<sizeof(BlockParams), 0>();
+  constexpr int DB = DP / 32, kBatch = 4;
+  typedef typename Vec<T>::x4 x4;
+  __shared__ int tree[TREE ? MI355_MAX_TREE_NODES : 1];
+  int const tid = threadIdx.x, lane = tid % 64, wave = tid / 64, h = lane / 32, c = lane % 32;
+  int const d = (int)blockIdx.x % DB, kv = (int)blockIdx.x / DB % P.kv_heads, block = (int)blockIdx.x / DB / P.kv_heads;
+  Block const b = block_of<TREE>(P, block);
+  if (!b.is || 32 * wave >= b.rows) {
+    return;
+  }
+  int parts = parts_of<DP>(P, b), slot = block * P.kv_heads + kv, step = P.blocks * P.kv_heads;
+  if (TREE && P.sequences > 1) {
+    Cut const cut = cut_of<DP>(P, -1, b.sequence);
+    parts = cut.parts;
+    step = P.row_blocks * P.kv_heads;
+    slot = cut.before + (block - b.sequence * P.row_blocks) * P.kv_heads + kv;
+  }
+  if (parts == 1) {
+    return;  // (it has left the result)
+  }
+  int const in_block = 32 * wave + c;
+  bool const is_row = in_block < b.rows;
+  float top = -INFINITY, sum = 0.0f;
+  paged::floatx4 x[4];
+#pragma unroll
+  for (int four = 0; four < 4; four++) {
+    x[four] = paged::floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  for (int i0 = 0; i0 < parts; i0 += kBatch) {
+    float ref[kBatch], its[kBatch];
+    paged::floatx4 y[kBatch][4];
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) {
+      float const *const part = P.parts + (long long)(slot + (i0 + i < parts ? i0 + i : parts - 1) * step) * part_floats<DP>();
+      ref[i] = part[kRows * DP + 2 * in_block];
+      its[i] = part[kRows * DP + 2 * in_block + 1];
+#pragma unroll
+      for (int four = 0; four < 4; four++) {
+        y[i][four] = *reinterpret_cast<paged::floatx4 const *>(part + 4 * (((d * kWaves + wave) * 4 + four) * 64 + lane));
+      }
+    }
+    float const before = top;
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) {
+      ref[i] = i0 + i < parts ? ref[i] : -INFINITY;
+      top = fmaxf(top, ref[i]);
+    }
+    float const base = top == -INFINITY ? 0.0f : top, less = exp2_fast(before - base);
+    sum *= less;
+#pragma unroll
+    for (int four = 0; four < 4; four++) {
+      x[four] *= less;
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) {
+      float const by = exp2_fast(ref[i] - base);
+      sum += ref[i] > -INFINITY ? its[i] * by : 0.0f;
+#pragma unroll
+      for (int four = 0; four < 4; four++) {  // (a part without tiles left no sums)
+        paged::floatx4 const z = by * y[i][four];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          x[four][e] += ref[i] > -INFINITY ? z[e] : 0.0f;
         }
       }
-      int const number = sees ? table[page] : -1;
-      return (unsigned)number < (unsigned)P.pages ? (uint32_t)number * P.page_step + (uint32_t)(real - page * P.page_size) * P.token_step : ~0u;
-    };
-    auto score = [&](uint32_t at) {
-      float x = 0.0f;
-      if (at == ~0u) {
-        return -INFINITY;
+    }
+  }
+  float const by = sum == 0.0f ? 0.0f : 1.0f / sum;
+  int const row = b.row0 + (is_row ? in_block : 0), token = quotient(row, P.group, P.group_magic);
+  T *const out = static_cast<T *>(P.out) + (long long)(b.row_of_q + token) * P.out_stride + (long long)(kv * P.group + row - token * P.group) * P.head_dim;
+  bool good = true;
+#pragma unroll
+  for (int four = 0; four < 4; four++) {
+    x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      y[e] = static_cast<T>(x[four][e] * by);
+    }
+    int const at = 32 * d + 8 * four + 4 * h;
+    if (is_row && at < P.head_dim) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        good = good && __builtin_fabsf(x[four][e] * by) < INFINITY;
       }
-      for (int d = 0; d < P.head_dim; d += 8) {
-        x8 const k = *reinterpret_cast<x8 const *>(k_base + 16ull * (at + d / 8)), a = *reinterpret_cast<x8 const *>(its_q + d);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          x += static_cast<float>(a[e]) * static_cast<float>(k[e]);
-        }
+      *reinterpret_cast<x4 *>(out + at) = y;
+    }
+  }
+  uint64_t again = __ballot(!good && is_row);
+  if (again != 0) {
+    if constexpr (TREE) {  // (every wavefront for itself: they write the same)
+      for (int i = lane; i < b.new_tokens; i += 64) {
+        tree[i] = P.parents[(long long)b.sequence * b.new_tokens + i];
       }
-      x = none ? x * 0.0f : x;
-      return (negative ? -x : x) * P.scale;
-    };
-    float high = -INFINITY;
-    bool wild = false;
-    for (int key = 0; key < end; key += 64) {
-      float const x = score(find(key + lane));
-      wild = wild || x != x;
-      high = fmaxf(high, x);
+      paged::wait_lds_reads();
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      high = fmaxf(high, __shfl_xor(high, off, 64));
-    }
-    wild = __any(wild) || high == INFINITY;
-    float total = 0.0f, o[DP / 64 + 1];
-#pragma unroll
-    for (int i = 0; i <= DP / 64; i++) {
-      o[i] = 0.0f;
-    }
-    float const from_high = high == -INFINITY ? 0.0f : bias - high;
-    for (int key = 0; key < end && !wild; key += 64) {
-      uint32_t const at = find(key + lane);
-      float const w = at == ~0u ? 0.0f : exp2_fast(score(at) + from_high);
-      total += w;
-      for (uint64_t left = __ballot(at != ~0u); left != 0; left &= left - 1) {
-        int const j = __builtin_ctzll(left);
-        float const its = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), j));
-        T const *const v = reinterpret_cast<T const *>(v_base + 16ull * (uint32_t)__builtin_amdgcn_readlane((int)at, j));
-#pragma unroll
-        for (int i = 0; i <= DP / 64; i++) {
-          if (64 * i + lane < P.head_dim) {
-            float const x = static_cast<float>(v[64 * i + lane]);
-            o[i] += __builtin_fabsf(x) == INFINITY && high != -INFINITY ? x : its * x;
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      total += __shfl_xor(total, off, 64);
-    }
-#pragma unroll
-    for (int i = 0; i <= DP / 64; i++) {
-      if (64 * i + lane < P.head_dim) {
-        its_out[64 * i + lane] = static_cast<T>(wild ? __builtin_nanf("") : (total == 0.0f ? 0.0f : o[i] * (1.0f / total)));
-      }
+    Row const r = row_of<TREE>(P, b, in_block, tree);
+    int const d1 = 32 * d + 32 < P.head_dim ? 32 * d + 32 : P.head_dim;
+    again = (again | again >> 32) & 0xffffffffull;
+    for (; again != 0; again &= again - 1) {
+      row_again<T, DP, TREE>(P, b, kv, of_lane(r, __builtin_ctzll(again)), tree, 32 * d, d1);
     }
   }
 }
 
 template <class T, int DP, bool TREE>
-int launch_blocks(BlockParams const &P) {
+int launch_blocks(BlockParams P) {
   auto *fn = attention_blocks_kernel<T, DP, TREE>;
   constexpr int lds = lds_bytes<DP, TREE>();
-  static_assert(2 * lds <= 160 * 1024, "two workgroups to a compute unit");
-  long long const blocks = P.starts == nullptr ? (long long)P.sequences * P.row_blocks : blocks_of(P.tokens, P.group, P.sequences);
+  static_assert(kPerUnit<DP> * lds <= 160 * 1024, "LDS of a compute unit");
+  P.row_blocks = (int)(((long long)P.new_tokens * P.group + kRows - 1) / kRows);
+  P.blocks = (int)(P.starts == nullptr ? (long long)P.sequences * P.row_blocks : blocks_of(P.tokens, P.group, P.sequences));
+  // Blocks that do not fill the chip are cut along their keys, of which a part has kLeastTiles tiles at least.
+  long long const items = (long long)P.blocks * P.kv_heads, keys = (long long)P.table_width * P.page_size;
+  long long const seen = P.window != 0 ? (long long)P.window + P.sinks + kRows : keys, tiles = ((seen < keys ? seen : keys) + kKeys<DP> - 1) / kKeys<DP>;
+  long long const room = (long long)(state().scratch_bytes / sizeof(float)) / part_floats<DP>(), fill = 256 * kPerUnit<DP>;
+  P.slots = (int)(fill < room ? fill : room);
+  long long splits = P.slots / items;
+  splits = splits < tiles / kLeastTiles ? splits : tiles / kLeastTiles;
+  splits = splits < room / items ? splits : room / items;
+  P.splits = splits < 1 ? 1 : (int)splits;
+  P.parts = static_cast<float *>(state().scratch());
   MI355_GRANT_LDS(fn, lds);
-  MI355_HIP(launch_kernel(fn, dim3((unsigned)(blocks * P.kv_heads)), dim3(kThreads), lds, state().stream(), P));
+  long long const grid = TREE && P.sequences > 1 && P.splits > 1 ? P.slots : items * P.splits;
+  MI355_HIP(launch_kernel(fn, dim3((unsigned)grid), dim3(kThreads), lds, state().stream(), P));
+  if (P.splits > 1) {
+    MI355_HIP(launch_kernel(join_blocks_kernel<T, DP, TREE>, dim3((unsigned)(items * (DP / 32))), dim3(kThreads), 0, state().stream(), P));
+  }
   return MI355_OK;
 }
 

@@ -2,9 +2,6 @@
 // (attention_blocks.h).
 #include "attention_blocks.h"
 #include "slices.h"
-#ifndef ROWS_LIMIT
-#define ROWS_LIMIT 64
-#endif
 
 namespace mi355 {
 
@@ -73,10 +70,14 @@ int fill(BlockParams &P, char const *name, void const *q, long long q_stride, vo
 }
 
 // Few rows of a key-value head, as many in every sequence: a head's keys are dealt over workgroups, a wavefront has 32 of them at a time to
-// itself (paged_attention.h), and reading the cache is what counts.
+// itself (paged_attention.h), and reading the cache is what counts.  Measured (us, that and blocks; heads of 128 unless said): 12.2 and 14.0 of 1
+// sequence x 8 heads x 1000 keys, 16 rows, 66 and 76 of 32 x 8 x up to 4096, 16 rows, 95 and 112 of 64 x 8 x 2053, 8 rows, 20.6 and 25.2 of 4 x 8 x 4096,
+// 32 rows, 38 and 45 of 1 x 8 x 30000, 32 rows, 24.0 and 26.3 of 5 x 3 heads of 256 x 3000, 15 rows, 25.1 and 32.7 of 4 x 4 heads of 64 x 16384, 48
+// rows; against it 16.8 and 13.3 of 1 x 8 x 1000, 32 rows, 86 and 73 of 32 x 8 x 4096, 32 rows, 135 and 77 of the same, 48 rows, 35 and 27 of 5 x 3 heads of
+// 256, 30 rows.
 bool few_rows(BlockParams const &P) {
   long long const rows = (long long)P.new_tokens * P.group;
-  return P.starts == nullptr && rows <= ROWS_LIMIT && P.new_tokens <= 64 &&
+  return P.starts == nullptr && rows <= (P.head_dim <= 64 ? 64 : P.head_dim <= 128 ? 32 : 16) &&
          !paged::too_many_units(P.kv_heads, rows, (long long)P.table_width * P.page_size);
 }
 
@@ -126,7 +127,6 @@ int launch(BlockParams &P, int type, bool tree) {
   if (few_rows(P)) {
     return launch_few(P, type, tree);
   }
-  P.row_blocks = (int)(((long long)P.new_tokens * P.group + kRows - 1) / kRows);
   return type == MI355_TYPE_F16 ? launch_f16(P, tree) : launch_bf16(P, tree);
 }
 

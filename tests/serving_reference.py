@@ -70,14 +70,15 @@ def attended(q, k, v, seen, scale, kind):
         # A score is a sum of d products in 32 bits: within (d + 4) 2^-23 of the sum of their magnitudes (an addition may truncate).
         # The exponential's argument, as far from 0 as the scores lie apart, is rounded twice, its value to 2^-22; weights and
         # values add up over n keys in 32 bits, twice over where parts are joined: relative to the weight, and in their sum
-        # too.  Each weight is rounded to the values' type once, to half a step, but its sum is not (below 2^-23 of the greatest
+        # too.  Each weight is rounded to the values' type once, to half a step of it, and added up as that: the result is off by the sum of
+        # what each is off times the distance of its value from the result, half a step of w |v| and of |y| (below 2^-23 of the greatest
         # fp16 weights are cut at 2^-34 of it).  2^-150 and less counts as nothing.
         n = seen.sum(1)
         score = (d + 4) * 2.0 ** -23 * abs(scale) * np.where(seen, np.abs(q[:, h]) @ np.abs(kk).T, 0.0).max(1)
         spread = np.minimum(150.0, np.where(some, (top - np.where(seen, s, np.inf).min(1, keepdims=True))[:, 0], 0.0))
         weight = 2 * score + 2.0 ** -22 * (spread + 4) + 2 * (n + 16) * 2.0 ** -23
         near = np.where(seen, np.abs(vv).T[:, None, :], 0.0).max(-1).T if kind == "fp16" else 0.0
-        bound[:, h] += step * np.abs(y) + (2 * weight + step)[:, None] * (w @ np.abs(vv)) + (2.0 ** -34 * n[:, None] * near if kind == "fp16" else 0.0)
+        bound[:, h] += 2 * step * np.abs(y) + (2 * weight + step)[:, None] * (w @ np.abs(vv)) + (2.0 ** -34 * n[:, None] * near if kind == "fp16" else 0.0)
         out[:, h] = y
     return out, bound
 
