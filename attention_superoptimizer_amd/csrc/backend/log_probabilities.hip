@@ -8,6 +8,7 @@
 // it are looked at one by one.  The bound is the top-th of the lanes' own maxima, which the sums need anyway; after the first few
 // thousand logits hardly any passes it.
 #include "common.h"
+#include "mi355_kernels/kernarg.h"
 #include "slices.h"
 
 #include <climits>
@@ -31,6 +32,46 @@ struct LogParams {
 };
 constexpr int kPartWords = 4 + 2 * MI355_MAX_TOP;
 
+// x of the lane that the DPP control names
+template <int CONTROL>
+__device__ __forceinline__ uint32_t moved(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CONTROL, 0xf, 0xf, true); }
+// x[l ^ STRIDE]: by moves between registers, where a shuffle is a trip through LDS
+template <int STRIDE>
+__device__ __forceinline__ uint32_t across(uint32_t x, int lane) {
+  if constexpr (STRIDE == 1) {
+    return moved<0xb1>(x);  // within fours
+  } else if constexpr (STRIDE == 2) {
+    return moved<0x4e>(x);
+  } else if constexpr (STRIDE == 4) {
+    return moved<0x1b>(moved<0x141>(x));  // eights mirrored, then fours
+  } else if constexpr (STRIDE == 8) {
+    return moved<0x128>(x);  // sixteens turned by eight
+  } else {
+    uint32_t a = x, b = x;  // (exchanges the odd rows or the upper half of one with the even rows or the lower half of the other)
+    if constexpr (STRIDE == 16) {
+      asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+    } else {
+      asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+    }
+    return (lane & STRIDE) != 0 ? a : b;
+  }
+}
+// over all lanes, in every one; op commutes
+template <class Op>
+__device__ __forceinline__ float over_lanes(float x, Op op) {
+  auto of = [](uint32_t bits) { return __builtin_bit_cast(float, bits); };
+  auto bits = [](float v) { return __builtin_bit_cast(uint32_t, v); };
+  x = op(x, of(moved<0xb1>(bits(x))));
+  x = op(x, of(moved<0x4e>(bits(x))));
+  x = op(x, of(moved<0x141>(bits(x))));  // eights, and sixteens, mirrored
+  x = op(x, of(moved<0x140>(bits(x))));
+  float a = x, b = x;
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  a = b = op(a, b);
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  return op(a, b);
+}
+
 // A logit and its token; the better one of two is the greater, of equal ones the one with the lower token.
 struct Entry {
   float x;
@@ -38,65 +79,77 @@ struct Entry {
 };
 __device__ __forceinline__ Entry none() { return {-INFINITY, INT_MAX}; }
 __device__ __forceinline__ bool better(Entry a, Entry b) { return a.x > b.x || (a.x == b.x && a.token < b.token); }
-__device__ __forceinline__ Entry of_lane(Entry e, int lane) { return {__shfl(e.x, lane, 64), __shfl(e.token, lane, 64)}; }
-__device__ __forceinline__ Entry exchange(Entry e, int lane, int stride, bool first_better) {
-  Entry const other = of_lane(e, lane ^ stride);
-  return better(other, e) == (((lane & stride) == 0) == first_better) ? other : e;
+// towards best first, or last
+template <int STRIDE>
+__device__ __forceinline__ Entry exchanged(Entry e, int lane, bool first) {
+  Entry const other = {__builtin_bit_cast(float, across<STRIDE>(__builtin_bit_cast(uint32_t, e.x), lane)), (int)across<STRIDE>((uint32_t)e.token, lane)};
+  return better(other, e) == (((lane & STRIDE) == 0) == first) ? other : e;
 }
-// from any order to best first
-__device__ __forceinline__ Entry sorted(Entry e, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 64; size *= 2) {
-#pragma unroll
-    for (int stride = size / 2; stride > 0; stride /= 2) {
-      e = exchange(e, lane, stride, (lane & size) == 0);
-    }
+template <int STRIDE>
+__device__ __forceinline__ Entry cleaned(Entry e, int lane, bool first) {
+  e = exchanged<STRIDE>(e, lane, first);
+  if constexpr (STRIDE > 1) {
+    e = cleaned<STRIDE / 2>(e, lane, first);
   }
   return e;
 }
-// the best 64 of two lists, best first
-__device__ __forceinline__ Entry merged(Entry a, Entry b, int lane) {
-  Entry const back = of_lane(b, 63 - lane);
-  Entry e = better(back, a) ? back : a;
-#pragma unroll
-  for (int stride = 32; stride > 0; stride /= 2) {
-    e = exchange(e, lane, stride, true);
-  }
-  return e;
+// from any order to best last
+__device__ __forceinline__ Entry sorted_back(Entry e, int lane) {
+  e = cleaned<1>(e, lane, (lane & 2) == 0);
+  e = cleaned<2>(e, lane, (lane & 4) == 0);
+  e = cleaned<4>(e, lane, (lane & 8) == 0);
+  e = cleaned<8>(e, lane, (lane & 16) == 0);
+  e = cleaned<16>(e, lane, (lane & 32) == 0);
+  return cleaned<32>(e, lane, false);
 }
+// the best 64 of a list best first and one best last, best first
+__device__ __forceinline__ Entry merged(Entry a, Entry back, int lane) { return cleaned<32>(better(back, a) ? back : a, lane, true); }
 
-// the n-th greatest of the lanes' values (n <= 64; no NaN), bit by bit of an order-preserving whole number
+// The n-th greatest of the lanes' values (n <= 64; no NaN), bit by bit of an order-preserving whole number, of which a T has the upper BITS.
+template <int BITS>
 __device__ __forceinline__ float nth_of_lanes(float x, int n) {
   uint32_t const bits = __builtin_bit_cast(uint32_t, x), key = bits ^ ((int)bits < 0 ? ~0u : 0x80000000u);
   uint32_t found = 0;
 #pragma unroll
-  for (int bit = 31; bit >= 0; bit--) {
+  for (int bit = 31; bit >= 32 - BITS; bit--) {
     uint32_t const with = found | 1u << bit;
     found = __builtin_popcountll(__ballot(key >= with)) >= n ? with : found;
   }
+  found |= (int)found < 0 ? 0 : (BITS < 32 ? (1u << (32 - BITS)) - 1 : 0);  // (of a negative value the lower bits are ones)
   return __builtin_bit_cast(float, found ^ ((int)found < 0 ? 0x80000000u : ~0u));
 }
 
-// Maximum, sum of 2^z and sum of z 2^z relative to it, z = scale (x - m): two of them joined.
+// Maximum, sum of 2^z and sum of z 2^z relative to it, z = scale (x - m).
 struct Sums {
   float m, s, t;
 };
 // scale (m - base) for sums that base is to be the maximum of: 0 where there are none yet (nor is there a maximum), and no less than
 // -200, whose power is zero as that of minus infinity is, but not a product with it
 __device__ __forceinline__ float shift(float m, float s, float base, float scale) { return s == 0.0f ? 0.0f : fmaxf((m - base) * scale, -200.0f); }
+__device__ __forceinline__ Sums moved_to(Sums a, float m, float scale) {  // m: not below a's
+  float const z = shift(a.m, a.s, m == -INFINITY ? 0.0f : m, scale), less = __builtin_amdgcn_exp2f(z);
+  return {m, a.s * less, less * (a.t + z * a.s)};
+}
 __device__ __forceinline__ Sums joined(Sums a, Sums b, float scale) {
-  float const m = fmaxf(a.m, b.m), base = m == -INFINITY ? 0.0f : m;
-  float const za = shift(a.m, a.s, base, scale), zb = shift(b.m, b.s, base, scale);
-  float const fa = __builtin_amdgcn_exp2f(za), fb = __builtin_amdgcn_exp2f(zb);
-  return {m, a.s * fa + b.s * fb, fa * (a.t + za * a.s) + fb * (b.t + zb * b.s)};
+  float const m = fmaxf(a.m, b.m);
+  a = moved_to(a, m, scale);
+  b = moved_to(b, m, scale);
+  return {m, a.s + b.s, a.t + b.t};
+}
+__device__ __forceinline__ Sums over_lanes(Sums a, float scale) {
+  auto add = [](float x, float y) { return x + y; };
+  a = moved_to(a, over_lanes(a.m, [](float x, float y) { return fmaxf(x, y); }), scale);
+  return {a.m, over_lanes(a.s, add), over_lanes(a.t, add)};
 }
 
-__device__ __forceinline__ float load_shared(float const *p) {
-  return __hip_atomic_load((__attribute__((address_space(1))) float const *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ uint64_t load_shared(float const *p) {
+  return __hip_atomic_load((__attribute__((address_space(1))) uint64_t const *)(uint64_t const *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ void store_shared(float *p, float x) {
-  __hip_atomic_store((__attribute__((address_space(1))) float *)p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ void store_shared(float *p, float x, uint32_t y) {
+  __hip_atomic_store((__attribute__((address_space(1))) uint64_t *)(uint64_t *)p, (uint64_t)__builtin_bit_cast(uint32_t, x) | (uint64_t)y << 32, __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
 }
+__device__ __forceinline__ float low_of(uint64_t x) { return __builtin_bit_cast(float, (uint32_t)x); }
 
 template <class T, bool TOP>
 __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams const P) {
@@ -106,6 +159,7 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
   __shared__ Entry lists[kWaves][64];
   __shared__ Sums sums[kWaves];
   __shared__ int is_last;
+  fetch_kernel_arguments<sizeof(LogParams), 0>();
   int const tid = threadIdx.x, lane = tid % 64, wave = tid / 64, N = P.vocabulary;
   int const part = (int)(blockIdx.x % (unsigned)P.row_parts);
   long long const row = blockIdx.x / (unsigned)P.row_parts;
@@ -127,25 +181,46 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
         h.x[r] = *reinterpret_cast<piece const *>(logits + j0 + (64 * r + lane) * V);
       }
     } else {
+      // A row's first and last chunk: pieces that lie in the row whole are asked for as ever (in the place of others the first such one), of
+      // those that do in part, one at either end, each element.
+      bool const some = N >= 2 * V;
 #pragma unroll
       for (int r = 0; r < kRounds; r++) {
+        int const j = j0 + (64 * r + lane) * V, first = ahead == 0 ? 0 : V - ahead;
+        h.x[r] = some ? *reinterpret_cast<piece const *>(logits + (j >= 0 && j <= N - V ? j : first)) : piece{};
+      }
 #pragma unroll
-        for (int e = 0; e < V; e++) {
-          int const j = j0 + (64 * r + lane) * V + e;
-          h.x[r][e] = j >= 0 && j < N ? logits[j] : static_cast<T>(-INFINITY);
+      for (int r = 0; r < kRounds; r++) {
+        int const j = j0 + (64 * r + lane) * V;
+        if (!some || j < 0 || j > N - V) {
+#pragma unroll
+          for (int e = 0; e < V; e++) {
+            h.x[r][e] = static_cast<T>(-INFINITY);
+          }
+          if (j > -V && j < N) {
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+              h.x[r][e] = j + e >= 0 && j + e < N ? logits[j + e] : static_cast<T>(-INFINITY);
+            }
+          }
         }
       }
     }
     return h;
   };
+  // the tokens asked for, on their way while the row is read (whoever comes last has them)
+  float asked_x = -INFINITY;
+  if (wave == 0 && lane < P.asked) {
+    int const token = P.tokens[row * P.asked + lane];
+    asked_x = token >= 0 && token < N ? static_cast<float>(logits[token]) : -INFINITY;
+  }
 
   Sums own = {-INFINITY, 0.0f, 0.0f};
   Entry best = none();
   float bound = -INFINITY;
   int waiting = 0;  // entries of this wavefront's that are not in `best` yet
   auto take = [&](int n) {
-    Entry e = lane < n ? pending[wave][lane] : none();
-    best = merged(best, sorted(e, lane), lane);
+    best = merged(best, sorted_back(lane < n ? pending[wave][lane] : none(), lane), lane);
   };
   int chunk = part * kWaves + wave;
   if (chunk < chunks) {
@@ -161,11 +236,8 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
         x[i] = static_cast<float>(h.x[i / V][i % V]);
         top = fmaxf(top, x[i]);
       }
-      float const m = fmaxf(own.m, top), base = m == -INFINITY ? 0.0f : m;
-      float const down = shift(own.m, own.s, base, P.scale), less = __builtin_amdgcn_exp2f(down);
-      own.t = less * (own.t + down * own.s);
-      own.s *= less;
-      own.m = m;
+      own = moved_to(own, fmaxf(own.m, top), P.scale);
+      float const base = own.m == -INFINITY ? 0.0f : own.m;
       float s = 0.0f, t = 0.0f;
 #pragma unroll
       for (int i = 0; i < kRounds * V; i++) {
@@ -178,7 +250,7 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
       own.t += t;
       if constexpr (TOP) {
         if (__any(top > bound)) {
-          float const before = bound, reached = nth_of_lanes(own.m, P.top);
+          float const before = bound, reached = nth_of_lanes<(sizeof(T) == 4 ? 32 : __is_same(T, _Float16) ? 19 : 16)>(own.m, P.top);
           bound = fmaxf(bound, reached);
           int const j0 = first_of(chunk) + lane * V;
 #pragma unroll
@@ -205,19 +277,12 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
   }
 
   // the wavefront's, then the workgroup's
-  auto over_lanes = [&](Sums a) {
-#pragma unroll
-    for (int off = 32; off > 0; off /= 2) {
-      a = joined(a, {__shfl_xor(a.m, off, 64), __shfl_xor(a.s, off, 64), __shfl_xor(a.t, off, 64)}, P.scale);
-    }
-    return a;
-  };
-  own = over_lanes(own);
+  own = over_lanes(own, P.scale);
   if constexpr (TOP) {
     if (waiting > 0) {
       take(waiting);
     }
-    lists[wave][lane] = best;
+    lists[wave][63 - lane] = best;
   }
   if (lane == 0) {
     sums[wave] = own;
@@ -239,12 +304,12 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
   if (P.row_parts > 1) {
     float *const mine = P.parts + (long long)blockIdx.x * kPartWords;
     if (wave == 0) {
-      if (lane < 3) {
-        store_shared(mine + lane, lane == 0 ? own.m : (lane == 1 ? own.s : own.t));
+      if (lane == 0) {
+        store_shared(mine, own.m, __builtin_bit_cast(uint32_t, own.s));
+        store_shared(mine + 2, own.t, 0);
       }
       if (TOP && lane < P.top) {
-        store_shared(mine + 4 + 2 * lane, best.x);
-        store_shared(mine + 5 + 2 * lane, __builtin_bit_cast(float, best.token));
+        store_shared(mine + 4 + 2 * lane, best.x, (uint32_t)best.token);
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
@@ -263,21 +328,29 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
     float const *const parts = P.parts + row * P.row_parts * kPartWords;
     own = {-INFINITY, 0.0f, 0.0f};
     if (tid < P.row_parts) {
-      own = {load_shared(parts + tid * kPartWords), load_shared(parts + tid * kPartWords + 1), load_shared(parts + tid * kPartWords + 2)};
+      uint64_t const m_s = load_shared(parts + tid * kPartWords), t = load_shared(parts + tid * kPartWords + 2);
+      own = {low_of(m_s), __builtin_bit_cast(float, (uint32_t)(m_s >> 32)), low_of(t)};
     }
-    own = over_lanes(own);
     if constexpr (TOP) {
-      best = none();
-      for (int i = wave; i < P.row_parts; i += kWaves) {
-        Entry e = none();
-        if (lane < P.top) {
-          e.x = load_shared(parts + i * kPartWords + 4 + 2 * lane);
-          e.token = __builtin_bit_cast(int, load_shared(parts + i * kPartWords + 5 + 2 * lane));
+      constexpr int kEach = kLargestParts / kWaves;
+      uint64_t its[kEach];  // all lists of this wavefront's parts, best last, asked for together
+#pragma unroll
+      for (int i = 0; i < kEach; i++) {
+        int const part_i = wave + i * kWaves;
+        if (i * kWaves < P.row_parts) {
+          its[i] = load_shared(parts + (part_i < P.row_parts ? part_i : 0) * kPartWords + 4 + 2 * (63 - lane < P.top ? 63 - lane : 0));
         }
-        best = merged(best, e, lane);
       }
-      lists[wave][lane] = best;
+      best = none();
+#pragma unroll
+      for (int i = 0; i < kEach; i++) {
+        if (wave + i * kWaves < P.row_parts) {
+          best = merged(best, 63 - lane < P.top ? Entry{low_of(its[i]), (int)(its[i] >> 32)} : none(), lane);
+        }
+      }
+      lists[wave][63 - lane] = best;
     }
+    own = over_lanes(own, P.scale);
     if (lane == 0) {
       sums[wave] = own;
     }
@@ -297,8 +370,11 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
     return wild ? nan : (empty || x == -INFINITY ? -INFINITY : kLn2 * ((x - own.m) * P.scale - log_z));
   };
   for (int i = lane; i < P.asked; i += 64) {
-    int const token = P.tokens[row * P.asked + i];
-    P.log_probs[row * P.asked + i] = log_of(token >= 0 && token < N ? static_cast<float>(logits[token]) : -INFINITY);
+    if (i >= 64) {
+      int const token = P.tokens[row * P.asked + i];
+      asked_x = token >= 0 && token < N ? static_cast<float>(logits[token]) : -INFINITY;
+    }
+    P.log_probs[row * P.asked + i] = log_of(asked_x);
   }
   if (lane == 0) {
     P.entropy[row] = wild ? nan : (empty ? 0.0f : kLn2 * (log_z - own.t / own.s));
