@@ -13,10 +13,13 @@
 
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 namespace mi355 {
 namespace {
 
+constexpr int kPending = 192;   // tokens that a wavefront has yet to look at; more than 128 are thinned out
+constexpr int kGathered = 512;  // entries of a workgroup that are told apart all at once
 constexpr int kThreads = 256, kWaves = kThreads / 64, kRounds = 4, kLargestParts = 64;
 
 struct LogParams {
@@ -72,51 +75,59 @@ __device__ __forceinline__ float over_lanes(float x, Op op) {
   return op(a, b);
 }
 
-// A logit and its token; the better one of two is the greater, of equal ones the one with the lower token.
-struct Entry {
-  float x;
-  int token;
-};
-__device__ __forceinline__ Entry none() { return {-INFINITY, INT_MAX}; }
-__device__ __forceinline__ bool better(Entry a, Entry b) { return a.x > b.x || (a.x == b.x && a.token < b.token); }
-// towards best first, or last
-template <int STRIDE>
-__device__ __forceinline__ Entry exchanged(Entry e, int lane, bool first) {
-  Entry const other = {__builtin_bit_cast(float, across<STRIDE>(__builtin_bit_cast(uint32_t, e.x), lane)), (int)across<STRIDE>((uint32_t)e.token, lane)};
-  return better(other, e) == (((lane & STRIDE) == 0) == first) ? other : e;
+// A logit and its token as one whole number: the better one of two, that with the greater logit or, of equal ones, the lower token, is the greater
+// number.  Zero: none.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  uint32_t const bits = __builtin_bit_cast(uint32_t, x);
+  return bits ^ ((int)bits < 0 ? ~0u : 0x80000000u);
 }
-template <int STRIDE>
-__device__ __forceinline__ Entry cleaned(Entry e, int lane, bool first) {
-  e = exchanged<STRIDE>(e, lane, first);
-  if constexpr (STRIDE > 1) {
-    e = cleaned<STRIDE / 2>(e, lane, first);
-  }
-  return e;
-}
-// from any order to best last
-__device__ __forceinline__ Entry sorted_back(Entry e, int lane) {
-  e = cleaned<1>(e, lane, (lane & 2) == 0);
-  e = cleaned<2>(e, lane, (lane & 4) == 0);
-  e = cleaned<4>(e, lane, (lane & 8) == 0);
-  e = cleaned<8>(e, lane, (lane & 16) == 0);
-  e = cleaned<16>(e, lane, (lane & 32) == 0);
-  return cleaned<32>(e, lane, false);
-}
-// the best 64 of a list best first and one best last, best first
-__device__ __forceinline__ Entry merged(Entry a, Entry back, int lane) { return cleaned<32>(better(back, a) ? back : a, lane, true); }
+__device__ __forceinline__ float unordered(uint32_t key) { return __builtin_bit_cast(float, key ^ ((int)key < 0 ? 0x80000000u : ~0u)); }
+__device__ __forceinline__ uint64_t entry_of(float x, int token) { return (uint64_t)ordered(x + 0.0f) << 32 | (uint32_t)~token; }  // (no negative zero)
+__device__ __forceinline__ float logit_of(uint64_t entry) { return unordered((uint32_t)(entry >> 32)); }
+__device__ __forceinline__ int token_of(uint64_t entry) { return (int)~(uint32_t)entry; }
 
-// The n-th greatest of the lanes' values (n <= 64; no NaN), bit by bit of an order-preserving whole number, of which a T has the upper BITS.
-template <int BITS>
-__device__ __forceinline__ float nth_of_lanes(float x, int n) {
-  uint32_t const bits = __builtin_bit_cast(uint32_t, x), key = bits ^ ((int)bits < 0 ? ~0u : 0x80000000u);
-  uint32_t found = 0;
-#pragma unroll
-  for (int bit = 31; bit >= 32 - BITS; bit--) {
-    uint32_t const with = found | 1u << bit;
-    found = __builtin_popcountll(__ballot(key >= with)) >= n ? with : found;
+template <int STRIDE>
+__device__ __forceinline__ uint64_t across(uint64_t x, int lane) {
+  return (uint64_t)across<STRIDE>((uint32_t)(x >> 32), lane) << 32 | across<STRIDE>((uint32_t)x, lane);
+}
+// Sorts runs of 2 STRIDE lanes that rise and then fall, or the other way round: greatest first, or last.
+template <int STRIDE, class T>
+__device__ __forceinline__ T cleaned(T x, int lane, bool first) {
+  T const other = across<STRIDE>(x, lane);
+  x = (other > x) == (((lane & STRIDE) == 0) == first) ? other : x;
+  if constexpr (STRIDE > 1) {
+    x = cleaned<STRIDE / 2>(x, lane, first);
   }
-  found |= (int)found < 0 ? 0 : (BITS < 32 ? (1u << (32 - BITS)) - 1 : 0);  // (of a negative value the lower bits are ones)
-  return __builtin_bit_cast(float, found ^ ((int)found < 0 ? 0x80000000u : ~0u));
+  return x;
+}
+template <class T>
+__device__ __forceinline__ T sorted(T x, int lane, bool first) {
+  x = cleaned<1>(x, lane, (lane & 2) == 0);
+  x = cleaned<2>(x, lane, (lane & 4) == 0);
+  x = cleaned<4>(x, lane, (lane & 8) == 0);
+  x = cleaned<8>(x, lane, (lane & 16) == 0);
+  x = cleaned<16>(x, lane, (lane & 32) == 0);
+  return cleaned<32>(x, lane, first);
+}
+// the greatest 64 of a list greatest first and one greatest last, greatest first
+__device__ __forceinline__ uint64_t merged(uint64_t a, uint64_t back, int lane) { return cleaned<32>(back > a ? back : a, lane, true); }
+
+// The n-th greatest of the lanes' values (n <= 64; no NaN), and the one in place (n + 3) / 4.
+struct Two {
+  float nth, earlier;
+};
+__device__ __forceinline__ Two nth_of_lanes(float value, int n, int lane) {
+  if (n == 1) {
+    float const most = over_lanes(value, [](float x, float y) { return fmaxf(x, y); });
+    return {most, most};
+  }
+  uint32_t const x = sorted(ordered(value), lane, true);
+  return {unordered((uint32_t)__builtin_amdgcn_readlane((int)x, n - 1)), unordered((uint32_t)__builtin_amdgcn_readlane((int)x, (n + 3) / 4 - 1))};
+}
+// the least value above x
+__device__ __forceinline__ float above(float x) {
+  int const bits = __builtin_bit_cast(int, x + 0.0f);  // (no negative zero)
+  return __builtin_bit_cast(float, bits + (bits < 0 ? -1 : 1));
 }
 
 // Maximum, sum of 2^z and sum of z 2^z relative to it, z = scale (x - m).
@@ -139,26 +150,28 @@ __device__ __forceinline__ Sums joined(Sums a, Sums b, float scale) {
 __device__ __forceinline__ Sums over_lanes(Sums a, float scale) {
   auto add = [](float x, float y) { return x + y; };
   a = moved_to(a, over_lanes(a.m, [](float x, float y) { return fmaxf(x, y); }), scale);
+  asm("" : "+v"(a.s), "+v"(a.t));  // (a product fused with the first addition would be rounded in one lane of each two only, and the lanes disagree)
   return {a.m, over_lanes(a.s, add), over_lanes(a.t, add)};
 }
 
 __device__ __forceinline__ uint64_t load_shared(float const *p) {
   return __hip_atomic_load((__attribute__((address_space(1))) uint64_t const *)(uint64_t const *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ void store_shared(float *p, float x, uint32_t y) {
-  __hip_atomic_store((__attribute__((address_space(1))) uint64_t *)(uint64_t *)p, (uint64_t)__builtin_bit_cast(uint32_t, x) | (uint64_t)y << 32, __ATOMIC_RELAXED,
-                     __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ void store_shared(float *p, uint64_t x) {
+  __hip_atomic_store((__attribute__((address_space(1))) uint64_t *)(uint64_t *)p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+__device__ __forceinline__ uint64_t both(float x, float y) { return (uint64_t)__builtin_bit_cast(uint32_t, x) | (uint64_t)__builtin_bit_cast(uint32_t, y) << 32; }
 __device__ __forceinline__ float low_of(uint64_t x) { return __builtin_bit_cast(float, (uint32_t)x); }
 
 template <class T, bool TOP>
 __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams const P) {
   constexpr int V = 16 / sizeof(T), kChunk = 64 * kRounds * V;
   typedef T piece __attribute__((ext_vector_type(V)));
-  __shared__ Entry pending[kWaves][128];
-  __shared__ Entry lists[kWaves][64];
+  __shared__ int pending[kWaves][kPending];  // tokens
+  __shared__ uint64_t gathered[kGathered], lists[kWaves][64];
   __shared__ Sums sums[kWaves];
-  __shared__ int is_last;
+  __shared__ float bounds[kWaves], quarters[kWaves];
+  __shared__ int counts[kWaves], count, is_last;
   fetch_kernel_arguments<sizeof(LogParams), 0>();
   int const tid = threadIdx.x, lane = tid % 64, wave = tid / 64, N = P.vocabulary;
   int const part = (int)(blockIdx.x % (unsigned)P.row_parts);
@@ -216,11 +229,19 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
   }
 
   Sums own = {-INFINITY, 0.0f, 0.0f};
-  Entry best = none();
-  float bound = -INFINITY;
-  int waiting = 0;  // entries of this wavefront's that are not in `best` yet
-  auto take = [&](int n) {
-    best = merged(best, sorted_back(lane < n ? pending[wave][lane] : none(), lane), lane);
+  float bound = -INFINITY, quarter = -INFINITY;  // that as many as asked for, and a quarter of these, reach
+  int waiting = 0;    // tokens of this wavefront's that may be among the top ones
+  uint64_t best = 0;  // the best of those that were thinned out, a lane each, best first
+  auto waiting_entry = [&](int i) {  // (their logits are read again: finding them again in registers takes longer)
+    int const token = i < waiting ? pending[wave][i] : 0;
+    return i < waiting ? entry_of(static_cast<float>(logits[token]), token) : 0;
+  };
+  auto thin = [&]() {  // the first 64
+    best = merged(best, sorted(waiting_entry(lane), lane, false), lane);
+    int const second = pending[wave][64 + lane], third = pending[wave][128 + lane];
+    pending[wave][lane] = second;
+    pending[wave][64 + lane] = third;
+    waiting = waiting > 64 ? waiting - 64 : 0;
   };
   int chunk = part * kWaves + wave;
   if (chunk < chunks) {
@@ -250,25 +271,27 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
       own.t += t;
       if constexpr (TOP) {
         if (__any(top > bound)) {
-          float const before = bound, reached = nth_of_lanes<(sizeof(T) == 4 ? 32 : __is_same(T, _Float16) ? 19 : 16)>(own.m, P.top);
-          bound = fmaxf(bound, reached);
+          // (an element that equals an earlier bound comes behind as many that are no less)
+          Two const reached = nth_of_lanes(own.m, P.top, lane);
+          float const least = reached.nth > bound ? reached.nth : above(bound);
+          bound = fmaxf(bound, reached.nth);
+          quarter = reached.earlier;
           int const j0 = first_of(chunk) + lane * V;
+          uint32_t passing = 0;
 #pragma unroll
           for (int i = 0; i < kRounds * V; i++) {
-            bool const passes = x[i] > before && x[i] >= bound;
-            uint64_t const which = __ballot(passes);
-            if (which != 0) {
-              if (passes) {
-                int const place = waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(which >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)which, 0));
-                pending[wave][place] = {x[i], j0 + 64 * V * (i / V) + i % V};
-              }
-              waiting += __builtin_popcountll(which);
-              if (waiting > 64) {
-                take(64);
-                waiting -= 64;
-                Entry const e = pending[wave][64 + lane];
-                pending[wave][lane] = e;
-              }
+            passing |= x[i] >= least ? 1u << i : 0u;
+          }
+          for (uint64_t which = __ballot(passing != 0); which != 0; which = __ballot(passing != 0)) {
+            if (passing != 0) {
+              int const i = __builtin_ctz(passing);
+              int const place = waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(which >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)which, 0));
+              pending[wave][place] = j0 + 64 * V * (i / V) + i % V;
+              passing &= passing - 1;
+            }
+            waiting += __builtin_popcountll(which);
+            if (waiting > 128) {
+              thin();
             }
           }
         }
@@ -276,121 +299,223 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
     }
   }
 
-  // the wavefront's, then the workgroup's
+  // The wavefronts' sums together, and their entries that no bound rules out.
   own = over_lanes(own, P.scale);
-  if constexpr (TOP) {
-    if (waiting > 0) {
-      take(waiting);
-    }
-    lists[wave][63 - lane] = best;
-  }
   if (lane == 0) {
     sums[wave] = own;
+    bounds[wave] = bound;
+    quarters[wave] = quarter;
   }
-  auto join_waves = [&]() {  // by the first wavefront
-    own = sums[0];
+  if (tid == 0) {
+    count = 0;
+  }
+  // Puts those of N entries a lane that reach the bound into `gathered`; more than fit are counted only.
+  auto gather = [&](auto n, auto const &its) {
+    constexpr int kN = decltype(n)::value;
+    int total = 0, before[kN];
+    uint64_t which[kN];
+    uint64_t const least = (uint64_t)ordered(bound > -INFINITY ? bound + 0.0f : above(bound)) << 32;
 #pragma unroll
-    for (int w = 1; w < kWaves; w++) {
-      own = joined(own, sums[w], P.scale);
-      if constexpr (TOP) {
+    for (int i = 0; i < kN; i++) {
+      which[i] = __ballot(its[i] >= least);
+      before[i] = total;
+      total += __builtin_popcountll(which[i]);
+    }
+    if (total != 0) {
+      int base = 0;
+      if (lane == 0) {
+        base = __hip_atomic_fetch_add(&count, total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      }
+      base = __builtin_amdgcn_readfirstlane(base);
+#pragma unroll
+      for (int i = 0; i < kN; i++) {
+        int const place = base + before[i] + __builtin_amdgcn_mbcnt_hi((uint32_t)(which[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)which[i], 0));
+        if ((which[i] >> lane & 1) != 0 && place < kGathered) {
+          gathered[place] = its[i];
+        }
+      }
+    }
+  };
+  // put(place, entry) for the `top` best of those gathered, by the thread that has it, best first, and none behind them.  How many are better
+  // is an entry's place: a few instructions for each two of them, where sorting takes 140 cycles for each of 21 steps.
+  auto place_gathered = [&](auto put) {
+    int const n = count;
+    for (int mine = tid; mine < n; mine += kThreads) {
+      uint64_t const entry = gathered[mine];
+      int place = 0;
+      int j = 0;
+      for (; j + 8 <= n; j += 8) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          place += gathered[j + i] > entry ? 1 : 0;
+        }
+      }
+      for (; j < n; j++) {
+        place += gathered[j] > entry ? 1 : 0;
+      }
+      if (place < P.top) {
+        put(place, entry);
+      }
+    }
+    if (tid >= n && tid < P.top) {
+      put(tid, 0);
+    }
+  };
+  auto place_lists = [&](auto put) {  // the same of the wavefronts' `best`
+    lists[wave][63 - lane] = best;
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int w = 1; w < kWaves; w++) {
         best = merged(best, lists[w][lane], lane);
+      }
+      if (lane < P.top) {
+        put(lane, best);
       }
     }
   };
   __syncthreads();
-  if (wave == 0) {
-    join_waves();
+  own = joined(joined(sums[0], sums[1], P.scale), joined(sums[2], sums[3], P.scale), P.scale);
+  if constexpr (TOP) {
+    static_assert(kWaves == 4, "sums and bounds");
+    bound = fmaxf(fmaxf(bounds[0], bounds[1]), fmaxf(bounds[2], bounds[3]));
+    bound = fmaxf(bound, fminf(fminf(quarters[0], quarters[1]), fminf(quarters[2], quarters[3])));
+    uint64_t const its[3] = {lane < P.top ? best : 0, waiting_entry(lane), waiting_entry(64 + lane)};
+    gather(std::integral_constant<int, 3>(), its);
+    __syncthreads();
   }
-  if (P.row_parts > 1) {
-    float *const mine = P.parts + (long long)blockIdx.x * kPartWords;
+  auto place_own = [&](auto put) {
+    if (count <= kGathered) {
+      place_gathered(put);
+    } else {
+      while (waiting > 0) {
+        thin();
+      }
+      place_lists(put);
+    }
+  };
+
+  auto answer = [&](auto place) {
+    constexpr float kLn2 = 0.693147180559945309f;
+    bool const empty = own.m == -INFINITY && own.s == 0.0f, wild = !(own.s < INFINITY) || own.m == INFINITY;
+    float const log_z = log2f(own.s), nan = __builtin_nanf("");
+    auto log_of = [&](float x) {
+      return wild ? nan : (empty || x == -INFINITY ? -INFINITY : kLn2 * ((x - own.m) * P.scale - log_z));
+    };
     if (wave == 0) {
+      for (int i = lane; i < P.asked; i += 64) {
+        if (i >= 64) {
+          int const token = P.tokens[row * P.asked + i];
+          asked_x = token >= 0 && token < N ? static_cast<float>(logits[token]) : -INFINITY;
+        }
+        P.log_probs[row * P.asked + i] = log_of(asked_x);
+      }
       if (lane == 0) {
-        store_shared(mine, own.m, __builtin_bit_cast(uint32_t, own.s));
-        store_shared(mine + 2, own.t, 0);
+        P.entropy[row] = wild ? nan : (empty ? 0.0f : kLn2 * (log_z - own.t / own.s));
       }
-      if (TOP && lane < P.top) {
-        store_shared(mine + 4 + 2 * lane, best.x, (uint32_t)best.token);
-      }
-    }
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-    __syncthreads();
-    if (tid == 0) {
-      int *const ticket = P.tickets + row * State::kJoinStep;
-      is_last = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == P.row_parts - 1;
-      if (is_last) {
-        __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
-      }
-    }
-    __syncthreads();
-    if (!is_last) {
-      return;
-    }
-    float const *const parts = P.parts + row * P.row_parts * kPartWords;
-    own = {-INFINITY, 0.0f, 0.0f};
-    if (tid < P.row_parts) {
-      uint64_t const m_s = load_shared(parts + tid * kPartWords), t = load_shared(parts + tid * kPartWords + 2);
-      own = {low_of(m_s), __builtin_bit_cast(float, (uint32_t)(m_s >> 32)), low_of(t)};
     }
     if constexpr (TOP) {
-      constexpr int kEach = kLargestParts / kWaves;
-      uint64_t its[kEach];  // all lists of this wavefront's parts, best last, asked for together
-#pragma unroll
-      for (int i = 0; i < kEach; i++) {
-        int const part_i = wave + i * kWaves;
-        if (i * kWaves < P.row_parts) {
-          its[i] = load_shared(parts + (part_i < P.row_parts ? part_i : 0) * kPartWords + 4 + 2 * (63 - lane < P.top ? 63 - lane : 0));
-        }
-      }
-      best = none();
-#pragma unroll
-      for (int i = 0; i < kEach; i++) {
-        if (wave + i * kWaves < P.row_parts) {
-          best = merged(best, 63 - lane < P.top ? Entry{low_of(its[i]), (int)(its[i] >> 32)} : none(), lane);
-        }
-      }
-      lists[wave][63 - lane] = best;
+      place([&](int i, uint64_t entry) {
+        bool const is = entry != 0 && !wild;
+        P.top_log_probs[row * P.top + i] = wild ? nan : (is ? log_of(logit_of(entry)) : -INFINITY);
+        P.top_tokens[row * P.top + i] = is ? token_of(entry) : -1;
+      });
     }
-    own = over_lanes(own, P.scale);
-    if (lane == 0) {
-      sums[wave] = own;
-    }
-    __syncthreads();
-    if (wave == 0) {
-      join_waves();
-    }
-  }
-  if (wave != 0) {
+  };
+  if (P.row_parts == 1) {
+    answer(place_own);
     return;
   }
 
-  constexpr float kLn2 = 0.693147180559945309f;
-  bool const empty = own.m == -INFINITY && own.s == 0.0f, wild = !(own.s < INFINITY) || own.m == INFINITY;
-  float const log_z = log2f(own.s), nan = __builtin_nanf("");
-  auto log_of = [&](float x) {
-    return wild ? nan : (empty || x == -INFINITY ? -INFINITY : kLn2 * ((x - own.m) * P.scale - log_z));
-  };
-  for (int i = lane; i < P.asked; i += 64) {
-    if (i >= 64) {
-      int const token = P.tokens[row * P.asked + i];
-      asked_x = token >= 0 && token < N ? static_cast<float>(logits[token]) : -INFINITY;
+  float *const mine = P.parts + (long long)blockIdx.x * kPartWords;
+  if (tid == 0) {
+    store_shared(mine, both(own.m, own.s));
+    store_shared(mine + 2, both(own.t, 0.0f));
+  }
+  if constexpr (TOP) {
+    place_own([&](int i, uint64_t entry) { store_shared(mine + 4 + 2 * i, entry); });
+  }
+  asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+  __syncthreads();
+  if (tid == 0) {
+    int *const ticket = P.tickets + row * State::kJoinStep;
+    is_last = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == P.row_parts - 1;
+    if (is_last) {
+      __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
     }
-    P.log_probs[row * P.asked + i] = log_of(asked_x);
+    count = 0;
   }
-  if (lane == 0) {
-    P.entropy[row] = wild ? nan : (empty ? 0.0f : kLn2 * (log_z - own.t / own.s));
+  __syncthreads();
+  if (!is_last) {
+    return;
   }
-  if (TOP && lane < P.top) {
-    bool const is = best.x > -INFINITY && !wild;
-    P.top_log_probs[row * P.top + lane] = is || wild ? log_of(best.x) : -INFINITY;
-    P.top_tokens[row * P.top + lane] = is ? best.token : -1;
+  // Every wavefront has the sums of all parts, and the lists of some, four at a time; what their last ones reach rules out most of the others.
+  float const *const parts = P.parts + row * P.row_parts * kPartWords;
+  static_assert(kLargestParts <= 64, "a lane has a part");
+  constexpr int kEach = 4;
+  auto ask = [&](int first, uint64_t (&its)[kEach]) {  // best last
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+      int const which = first + wave + i * kWaves;
+      its[i] = load_shared(parts + (which < P.row_parts ? which : 0) * kPartWords + 4 + 2 * (63 - lane < P.top ? 63 - lane : 0));
+    }
+  };
+  auto only_theirs = [&](int first, uint64_t (&its)[kEach]) {
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+      its[i] = first + wave + i * kWaves < P.row_parts && 63 - lane < P.top ? its[i] : 0;
+    }
+  };
+  uint64_t its[kEach], ends = 0, earlier = 0;
+  float const *const its_part = parts + (lane < P.row_parts ? lane : 0) * kPartWords;
+  uint64_t const m_s = load_shared(its_part), t = load_shared(its_part + 2);
+  if constexpr (TOP) {
+    ends = load_shared(its_part + 4 + 2 * (P.top - 1));
+    earlier = load_shared(its_part + 4 + 2 * ((P.top - 1) / P.row_parts));
+    ask(0, its);
   }
+  own = lane < P.row_parts ? Sums{low_of(m_s), low_of(m_s >> 32), low_of(t)} : Sums{-INFINITY, 0.0f, 0.0f};
+  own = over_lanes(own, P.scale);
+  if constexpr (TOP) {
+    // what every list's last one reaches, and what its share of them does
+    auto reached = [](uint64_t entry) { return entry != 0 ? logit_of(entry) : -INFINITY; };
+    bound = over_lanes(lane < P.row_parts ? reached(ends) : -INFINITY, [](float x, float y) { return fmaxf(x, y); });
+    bound = fmaxf(bound, over_lanes(lane < P.row_parts ? reached(earlier) : INFINITY, [](float x, float y) { return fminf(x, y); }));
+    for (int first = 0; first < P.row_parts; first += kEach * kWaves) {
+      if (first > 0) {
+        ask(first, its);
+      }
+      only_theirs(first, its);
+      gather(std::integral_constant<int, kEach>(), its);
+    }
+    __syncthreads();
+  }
+  answer([&](auto put) {
+    if (count <= kGathered) {
+      place_gathered(put);
+    } else {
+      best = 0;
+      for (int first = 0; first < P.row_parts; first += kEach * kWaves) {
+        ask(first, its);
+        only_theirs(first, its);
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+          best = merged(best, its[i], lane);
+        }
+      }
+      place_lists(put);
+    }
+  });
 }
 
 template <class T>
 int launch_log(LogParams P, int rows) {
   constexpr int kChunk = 64 * kRounds * (16 / (int)sizeof(T));
-  // As many workgroups to a row as fill the chip four times over, each with a chunk for every wavefront at least.
-  int const most = (P.vocabulary - 1) / (kWaves * kChunk) + 1, wanted = rows < 1024 ? (1023 / rows) + 1 : 1;
+  // As many workgroups to a row as leave two to a compute unit, each with a chunk for every wavefront at least.  Measured (us, one, two and four to a
+  // compute unit): 13.6, 12.6 and 13.6 of 64 rows of 131072 bf16 with 20 top tokens, 24.4 us being the two of 200 rows, against 26.1 and 24.7; alike for few
+  // rows.
+  constexpr int kFill = 512;
+  int const most = (P.vocabulary - 1) / (kWaves * kChunk) + 1, wanted = rows < kFill ? (kFill - 1) / rows + 1 : 1;
   P.row_parts = wanted < most ? wanted : most;
   P.row_parts = P.row_parts < kLargestParts ? P.row_parts : kLargestParts;
   auto *fn = P.top > 0 ? log_probabilities_kernel<T, true> : log_probabilities_kernel<T, false>;
