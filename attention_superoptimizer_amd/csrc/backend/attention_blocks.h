@@ -779,7 +779,7 @@ int launch_blocks(BlockParams P) {
   auto *fn = attention_blocks_kernel<T, DP, TREE>;
   constexpr int lds = lds_bytes<DP, TREE>();
   static_assert(kPerUnit<DP> * lds <= 160 * 1024, "LDS of a compute unit");
-  P.row_blocks = (int)(((long long)P.new_tokens * P.group + kRows - 1) / kRows);
+  P.row_blocks = (int)row_blocks((long long)P.new_tokens * P.group);
   P.blocks = (int)(P.starts == nullptr ? (long long)P.sequences * P.row_blocks : blocks_of(P.tokens, P.group, P.sequences));
   // Blocks that do not fill the chip are cut along their keys, of which a part has kLeastTiles tiles at least.
   long long const items = (long long)P.blocks * P.kv_heads, keys = (long long)P.table_width * P.page_size;

@@ -13,13 +13,13 @@ using namespace blocks;
 
 // What both entry points take; `name` is the caller's.  P is filled but for what masks are made of.
 int fill(BlockParams &P, char const *name, void const *q, long long q_stride, void *out, long long out_stride, mi355_paged_cache const &c,
-         int const *table, int table_width, int const *lengths, int sequences, long long tokens, int q_heads, float scale) {
+         int const *table, int table_width, int const *lengths, int sequences, long long tokens, bool ragged, int q_heads, float scale) {
   if (sequences < 0 || q_heads < 1 || q_heads % c.kv_heads != 0 || table_width < 1 || !std::isfinite(scale) || q_stride < 0 || out_stride < 0) {
     return fail(MI355_ERR_INVALID, "%s: %d sequences, %d heads over %d, table of %d", name, sequences, q_heads, c.kv_heads, table_width);
   }
   long long const keys = (long long)table_width * c.page_size;
   if (c.head_dim % 8 != 0 || c.head_dim > MI355_MAX_PAGED_HEAD_DIM || keys > 1 << 30 || tokens > INT_MAX ||
-      (long long)q_heads * c.head_dim > INT_MAX || !fit(tokens, q_heads / c.kv_heads, c.kv_heads, sequences)) {
+      (long long)q_heads * c.head_dim > INT_MAX || !fit(tokens, q_heads / c.kv_heads, c.kv_heads, sequences, ragged)) {
     return fail(MI355_ERR_UNSUPPORTED, "%s: heads of %d, a table of %d pages of %d, %lld tokens, %d heads", name, c.head_dim, table_width,
                 c.page_size, tokens, q_heads);
   }
@@ -127,7 +127,22 @@ int launch(BlockParams &P, int type, bool tree) {
   if (few_rows(P)) {
     return launch_few(P, type, tree);
   }
-  return type == MI355_TYPE_F16 ? launch_f16(P, tree) : launch_bf16(P, tree);
+  auto run = [&](BlockParams const &Q) { return type == MI355_TYPE_F16 ? launch_f16(Q, tree) : launch_bf16(Q, tree); };
+  if (P.starts != nullptr) {
+    return run(P);
+  }
+  long long const slice = sequences_at_once((long long)P.new_tokens * P.group, P.kv_heads);
+  return in_slices(P.sequences, slice, [&](long long at, long long count) -> int {
+    BlockParams Q = P;
+    Q.sequences = (int)count;
+    Q.tokens = (int)(count * P.new_tokens);
+    Q.q = static_cast<char const *>(P.q) + 2 * at * P.new_tokens * P.q_stride;
+    Q.out = static_cast<char *>(P.out) + 2 * at * P.new_tokens * P.out_stride;
+    Q.table = P.table + at * P.table_width;
+    Q.lengths = P.lengths + at;
+    Q.parents = tree ? P.parents + at * P.new_tokens : nullptr;
+    return run(Q);
+  });
 }
 
 }  // namespace
@@ -150,7 +165,7 @@ extern "C" int mi355_tree_attention(void const *q, long long q_stride, void *out
   }
   blocks::BlockParams P{};
   if (int rc = fill(P, "mi355_tree_attention", q, q_stride, out, out_stride, *cache, table, table_width, lengths, sequences,
-                    (long long)sequences * nodes, q_heads, scale)) {
+                    (long long)sequences * nodes, false, q_heads, scale)) {
     return rc;
   }
   if (sequences == 0) {
@@ -178,8 +193,8 @@ extern "C" int mi355_window_attention(void const *q, long long q_stride, void *o
     return fail(MI355_ERR_INVALID, "mi355_window_attention: %d tokens of %d sequences, window %d, %d kept", tokens, sequences, window, sinks);
   }
   blocks::BlockParams P{};
-  if (int rc = fill(P, "mi355_window_attention", q, q_stride, out, out_stride, *cache, table, table_width, lengths, sequences, tokens, q_heads,
-                    scale)) {
+  if (int rc = fill(P, "mi355_window_attention", q, q_stride, out, out_stride, *cache, table, table_width, lengths, sequences, tokens,
+                    starts != nullptr, q_heads, scale)) {
     return rc;
   }
   if (sequences == 0 || tokens == 0) {

@@ -519,7 +519,7 @@ int launch_log(LogParams P, int rows) {
   P.row_parts = wanted < most ? wanted : most;
   P.row_parts = P.row_parts < kLargestParts ? P.row_parts : kLargestParts;
   auto *fn = P.top > 0 ? log_probabilities_kernel<T, true> : log_probabilities_kernel<T, false>;
-  return in_slices(rows, (1 << 30) / kLargestParts, [&](long long at, long long count) -> int {
+  return in_slices(rows, 1 << 22, [&](long long at, long long count) -> int {
     LogParams Q = P;
     Q.logits = static_cast<T const *>(P.logits) + at * P.stride;
     Q.tokens = P.tokens != nullptr ? P.tokens + at * P.asked : nullptr;

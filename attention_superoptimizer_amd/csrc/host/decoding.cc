@@ -207,7 +207,7 @@ bool tree_ok(DTensor const &q, DTensor const &k, DTensor const &v, DTensor const
   int const heads = cached_heads(q, k, v, table, lengths, scale, heads_first);
   return heads > 0 && parents.num_dims == 2 && positive(parents) && parents.dim[0] == table.dim[0] && parents.dim[1] <= MI355_MAX_TREE_NODES &&
          parents.data_type == DT_INT32 && row_major(parents) && (long long)parents.dim[0] * parents.dim[1] == q.dim[0] &&
-         mi355::blocks::fit(q.dim[0], heads / CacheShape(k, heads_first).kv_heads, CacheShape(k, heads_first).kv_heads, table.dim[0]);
+         mi355::blocks::fit(q.dim[0], heads / CacheShape(k, heads_first).kv_heads, CacheShape(k, heads_first).kv_heads, table.dim[0], false);
 }
 
 bool window_ok(DTensor const &q, DTensor const &k, DTensor const &v, DTensor const &table, DTensor const &lengths, DTensor const *starts,
@@ -217,7 +217,8 @@ bool window_ok(DTensor const &q, DTensor const &k, DTensor const &v, DTensor con
                                       : heads > 0 && table.dim[0] < INT_MAX && has_dims(*starts, {table.dim[0] + 1}) &&
                                             starts->data_type == DT_INT32 && row_major(*starts);
   return rows && window >= 0 && sinks >= 0 &&
-         mi355::blocks::fit(q.dim[0], heads / CacheShape(k, heads_first).kv_heads, CacheShape(k, heads_first).kv_heads, table.dim[0]);
+         mi355::blocks::fit(q.dim[0], heads / CacheShape(k, heads_first).kv_heads, CacheShape(k, heads_first).kv_heads, table.dim[0],
+                            starts != nullptr);
 }
 
 std::vector<DTensor> window_inputs(DTensor const &q, DTensor const &k, DTensor const &v, DTensor const &table, DTensor const &lengths,

@@ -121,6 +121,7 @@ def test_scales(rt, scale):
 
 def test_many_sequences(rt):
     _check(4, 6, [6 + (37 * i) % 90 for i in range(150)], kv_heads=1, group=2)
+    _check(4, 20, [20 + (137 * i) % 900 for i in range(150)], kv_heads=1, group=2)  # parts dealt to them by their lengths
 
 
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
@@ -143,6 +144,22 @@ def test_places_that_are_not_seen_hold_anything(rt, value, nodes, kind):
     got = _run(*x, kind, 0.1)
     check(got[clean], want[clean], bound[clean])
     assert (np.isnan(got[~clean]) if np.isnan(value) else got[~clean] == value).all()
+
+
+@pytest.mark.parametrize("value", [np.nan, -np.inf])
+@pytest.mark.parametrize("sequences", [1, 2])
+def test_such_places_among_keys_that_several_workgroups_read(rt, value, sequences):
+    nodes, length = 20, 3000
+    *x, values = _case(15, nodes, [length, 700][:sequences], 1, 4, 80, 16, "bf16")
+    q, k, v, table, lengths, parents = x
+    want, bound = _expected(q, values, lengths, parents, 0.1, "bf16")
+    j = length - 8
+    v[table[0, j // 16], j % 16] = value
+    got = _run(*x, "bf16", 0.1)
+    sees = np.concatenate([tree_seen(length, parents[0])[:, j], np.zeros((sequences - 1) * nodes, bool)])
+    assert sees.any() and not sees[:nodes].all()
+    check(got[~sees], want[~sees], bound[~sees])
+    assert (np.isnan(got[sees]) if np.isnan(value) else got[sees] == value).all()
 
 
 @pytest.mark.parametrize("nodes", [6, 40])

@@ -105,6 +105,14 @@ def test_ragged_batches(rt, kind, new, past, window):
 
 
 @pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("head", [64, 80, 128, 192, 256])
+@pytest.mark.parametrize("window", [0, 2500])
+def test_ragged_batches_behind_long_caches(rt, kind, head, window):
+    """Few blocks of rows, cut along their keys."""
+    _check(head, [3, 0, 50, 1], [4100, 10, 2950, 700], window, 4, head=head, kind=kind, ragged=True, kv_heads=1, group=3, spare_rows=2)
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
 @pytest.mark.parametrize("head,group", [(128, 4), (64, 1), (256, 2)])
 def test_prompts(rt, kind, head, group):
     _check(head, [700], [700], 0, 0, head=head, group=group, kind=kind, kv_heads=1)
@@ -214,6 +222,18 @@ def test_places_that_are_not_seen_hold_anything(rt, value, new):
         check(got[clean], want[clean], bound[clean])
         wild = got[seen[:, 299] | seen[:, 298]]
         assert (np.isnan(wild) if np.isnan(value) else wild == value).all()
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_such_places_among_keys_that_several_workgroups_read(rt, ragged):
+    q, k, v, table, n, values = _case(16, [40], [3000], 1, 3, 128, 16, "fp16")
+    want, bound = _expected(q, values, [40], [3000], 2000, 6, 0.1, "fp16")
+    seen = window_seen(3000, 40, 2000, 6)
+    j = 2980
+    v[table[0, j // 16], j % 16] = np.inf
+    got = _run(q, k, v, table, n, "fp16", 2000, 6, 0.1, [40] if ragged else None)
+    check(got[~seen[:, j]], want[~seen[:, j]], bound[~seen[:, j]])
+    assert (~seen[:, j]).any() and (got[seen[:, j]] == np.inf).all()
 
 
 @pytest.mark.parametrize("new", [1, 40])
@@ -357,5 +377,6 @@ def test_refusals(rt, abi):
             assert call(cache(**change)) == code, change
         assert call(width=1 << 29) == -4
         assert call(heads=1 << 20, tokens=1 << 14, sequences=1, q_stride=1 << 26, out_stride=1 << 26) == -4
+        assert call(starts=i, sequences=1 << 24, tokens=4) == -4
     finally:
         g.close()
