@@ -11,6 +11,7 @@
 #include "mi355_kernels/kernarg.h"
 #include "slices.h"
 
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -563,6 +564,6 @@ extern "C" int mi355_log_probabilities(void const *logits, long long stride, int
   }
   State &s = state();
   LogParams const P{logits, stride, tokens, log_probs, entropy, top_log_probs, top_tokens, static_cast<float *>(s.scratch()), s.queue_join_tickets(),
-                    asked, top, vocabulary, 1, scale * 1.44269504088896341f};
+                    asked, top, vocabulary, 1, fminf(scale * 1.44269504088896341f, FLT_MAX)};
   return type == MI355_TYPE_F16 ? launch_log<_Float16>(P, rows) : type == MI355_TYPE_BF16 ? launch_log<__bf16>(P, rows) : launch_log<float>(P, rows);
 }

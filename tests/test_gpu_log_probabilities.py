@@ -96,6 +96,24 @@ def test_scales(rt, scale, kind):
     _check(*_logits(4, 5, 5003, kind), 9, kind, scale)
 
 
+@pytest.mark.parametrize("rows", [1, 600])
+def test_the_largest_and_smallest_scale(rt, rows):
+    """All but the most probable six are too improbable for 32 bits; all are alike."""
+    logits = np.tile(np.arange(1000) % 7 * -2.0, (rows, 1))
+    logits[:, 3::7] = 2.0
+    logits[:, 40:] = -20.0  # the greatest: 3, 10, 17, 24, 31, 38
+    tokens = np.tile(np.array([10, 11, 999], np.int32), (rows, 1))
+    logp, entropy, top_logp, top = _run(logits, tokens, 8, float(np.finfo(np.float32).max), "fp16")
+    check(logp[:, 0], np.full(rows, -np.log(6)), 2.0 ** -20)
+    check(entropy, np.full(rows, np.log(6)), 2.0 ** -20)
+    assert (logp[:, 1:] == -np.inf).all() and (top_logp[:, 6:] == -np.inf).all()
+    np.testing.assert_array_equal(top, np.tile([3, 10, 17, 24, 31, 38, 0, 7], (rows, 1)))
+    logp, entropy, top_logp, top = _run(logits, tokens, 8, 1e-38, "fp16")
+    for x, want in ((logp, -np.log(1000)), (top_logp, -np.log(1000)), (entropy, np.log(1000))):
+        check(x, np.full(x.shape, want), 2.0 ** -18)  # of a sum of 1000 ones, exact, the logarithm: within 2^-22 of itself, taken times ln 2
+    np.testing.assert_array_equal(top, np.tile([3, 10, 17, 24, 31, 38, 0, 7], (rows, 1)))
+
+
 @pytest.mark.parametrize("kind", ["fp16", "bf16", "fp32"])
 @pytest.mark.parametrize("top", [1, 20, 64])
 def test_equal_logits_in_the_order_of_their_tokens(rt, kind, top):
