@@ -108,20 +108,23 @@ __device__ __forceinline__ float sum_of(Vec<__bf16>::x8 p, float sum) {
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1); }
 
 constexpr int kThreads = 256, kWaves = 4;
-// Of a part: one sequence, 8 heads of 128, 1000 keys, 48 rows takes 17.2, 13.8 and 15.1 us with four, two and one.
-constexpr int kLeastTiles = 2;
+// Of a part: one sequence, 8 heads of 128, 1000 keys, 48 rows takes 17.2, 13.8 and 15.1 us with 256, 128 and 64.
+constexpr int kLeastKeys = 128;
 template <int DP>
 constexpr int kKeys = DP == 192 ? 32 : 64;  // of a tile
 template <int DP>
-constexpr int kStepsOf = DP == 96 ? 1024 : 2048;  // keys of a run whose places a workgroup holds in LDS (96: three workgroups fit)
+constexpr int kLeastTiles = kLeastKeys / kKeys<DP>;
+template <int DP, bool TREE>
+constexpr int kStepsOf = DP != 96 ? 2048 : (TREE ? 512 : 1024);  // keys of a run whose places a workgroup holds in LDS (96: three workgroups fit)
 template <int DP>
 constexpr int tile_bytes() { return kKeys<DP> * DP * 2; }
 template <int DP, bool TREE>
-constexpr int lds_bytes() { return 4 * tile_bytes<DP>() + 4 * kStepsOf<DP> + kStepsOf<DP> / 8 + (TREE ? 4 * MI355_MAX_TREE_NODES : 0); }
-// Workgroups that a compute unit's registers hold, at least.  Heads of 256: one, of tiles of 64 keys (one prompt of 8192 tokens, 32 heads, a window
+constexpr int lds_bytes() { return 4 * tile_bytes<DP>() + 4 * kStepsOf<DP, TREE> + kStepsOf<DP, TREE> / 8 + (TREE ? 2 * MI355_MAX_TREE_NODES : 0); }
+// Workgroups that a compute unit holds, its registers and LDS (of trees with heads up to 64: three, 45 us, where two are asked for, 50; 4 x 4 heads x up to
+// 16384 keys, 512 rows).  Heads of 256: one, of tiles of 64 keys (one prompt of 8192 tokens, 32 heads, a window
 // of 1024: 440 us; two of tiles of 32, with registers spilled, 459).
 template <int DP>
-constexpr int kPerUnit = DP <= 192 ? 2 : 1;
+constexpr int kPerUnit = DP <= 96 ? 3 : DP <= 192 ? 2 : 1;
 
 // The rows of a block and the keys that any of them sees.
 struct Block {
@@ -178,13 +181,21 @@ __device__ __forceinline__ Block block_of(BlockParams const &P, int block) {
   return b;
 }
 
+// the parents of its nodes, -2 in the place of any that is none
+__device__ __forceinline__ void fetch_tree(BlockParams const &P, Block const &b, short *tree, int first, int step) {
+  for (int i = first; i < b.new_tokens; i += step) {
+    int const p = P.parents[(long long)b.sequence * b.new_tokens + i];
+    tree[i] = (short)(p >= -1 && p < i ? p : -2);
+  }
+}
+
 // A row of it: the keys of the run below `always`, and those from `least` up to `limit`; of a tree, those below `limit` (below zero:
 // none) and the token's and its ancestors'.
 struct Row {
   int row, token, limit, least, always;
 };
 template <bool TREE>
-__device__ __forceinline__ Row row_of(BlockParams const &P, Block const &b, int in_block, int const *tree) {
+__device__ __forceinline__ Row row_of(BlockParams const &P, Block const &b, int in_block, short const *tree) {
   Row r{b.row0 + in_block, 0, 0, 0, 0};
   r.token = quotient(in_block < b.rows ? r.row : b.row0 + b.rows - 1, P.group, P.group_magic);
   int const context = b.length - b.new_tokens;
@@ -198,7 +209,7 @@ __device__ __forceinline__ Row row_of(BlockParams const &P, Block const &b, int 
     while (__any(at >= 0)) {
       if (at >= 0) {
         int const p = tree[at];
-        at = p >= -1 && p < at && (p < 0 || context + p >= 0) ? p : -2;
+        at = p < 0 || context + p >= 0 ? p : -2;
       }
     }
     r.limit = at == -1 ? (r.limit < 0 ? 0 : r.limit) : -1;
@@ -216,7 +227,7 @@ __device__ __forceinline__ float bias_of(int keys) {
 // wavefront a row, key by key, columns d0 up to d1.  (In the loop over tiles such values would have to be looked for in every tile that
 // not all rows see.)  `r` is the same in every lane.
 template <class T, int DP, bool TREE>
-__device__ void row_again(BlockParams const &P, Block const &b, int kv, Row r, int const *tree, int d0, int d1) {
+__device__ void row_again(BlockParams const &P, Block const &b, int kv, Row r, short const *tree, int d0, int d1) {
   typedef typename Vec<T>::x8 x8;
   int const lane = threadIdx.x % 64;
   T const *const q = static_cast<T const *>(P.q) + (long long)(b.row_of_q + r.token) * P.q_stride + (long long)(kv * P.group + r.row - r.token * P.group) * P.head_dim;
@@ -328,7 +339,7 @@ __device__ __forceinline__ Cut cut_of(BlockParams const &P, int work, int sequen
     return __builtin_amdgcn_readlane(paged::wave_upto(x), 63) * each;
   };
   int run = (total([](int tiles) { return tiles; }) + P.slots - 1) / P.slots;
-  run = run < kLeastTiles ? kLeastTiles : run;
+  run = run < kLeastTiles<DP> ? kLeastTiles<DP> : run;
   auto parts_of = [&](int tiles) { return (int)(((unsigned)tiles + run - 1) / (unsigned)run); };
   while (total(parts_of) > P.slots) {
     run += 1 + run / 16;
@@ -348,10 +359,9 @@ __device__ __forceinline__ Cut cut_of(BlockParams const &P, int work, int sequen
   }
   return cut;
 }
-// Any other block is cut into as many parts as all may have, of two tiles or more.
-template <int DP>
+// Any other block is cut into as many parts as all may have, of kLeastKeys or more.
 __device__ __forceinline__ int parts_of(BlockParams const &P, Block const &b) {
-  int const most = b.end / (kKeys<DP> * kLeastTiles);
+  int const most = b.end / kLeastKeys;
   return most < 1 ? 1 : (most < P.splits ? most : P.splits);
 }
 // of a block's part
@@ -361,13 +371,13 @@ constexpr int part_floats() { return kRows * (DP + 2); }
 template <class T, int DP, bool TREE>
 __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kernel(BlockParams const P) {
   fetch_kernel_arguments<sizeof(BlockParams), 1>();
-  constexpr int KT = kKeys<DP>, G = KT / 32, C = DP / 8, LOADS = KT * C / kThreads, KK = DP / 16, DB = DP / 32, kSteps = kStepsOf<DP>;
+  constexpr int KT = kKeys<DP>, G = KT / 32, C = DP / 8, LOADS = KT * C / kThreads, KK = DP / 16, DB = DP / 32, kSteps = kStepsOf<DP, TREE>;
   typedef typename Vec<T>::x8 x8;
   typedef typename Vec<T>::x4 x4;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   uint64_t *const exist = reinterpret_cast<uint64_t *>(lds + 4 * tile_bytes<DP>());
   uint32_t *const steps = reinterpret_cast<uint32_t *>(exist + kSteps / 64);
-  int *const tree = reinterpret_cast<int *>(steps + kSteps);
+  short *const tree = reinterpret_cast<short *>(steps + kSteps);
   int const tid = threadIdx.x, lane = tid % 64, wave = tid / 64, h = lane / 32, c = lane % 32;
   uint32_t const lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void const *)lds;
 
@@ -392,15 +402,13 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
   }
   Block const b = block_of<TREE>(P, item);
   if (P.splits > 1 && !dealt) {
-    parts = parts_of<DP>(P, b);
+    parts = parts_of(P, b);
   }
   if (!b.is || split >= parts) {
     return;
   }
   if constexpr (TREE) {
-    for (int i = tid; i < b.new_tokens; i += kThreads) {
-      tree[i] = P.parents[(long long)b.sequence * b.new_tokens + i];
-    }
+    fetch_tree(P, b, tree, tid, kThreads);
     __syncthreads();
   }
   int const context = b.length - b.new_tokens, kept = b.kept, shift = b.shift;
@@ -511,6 +519,10 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
       if (at + KT < part_end) {
         load(buffer ^ 1);
       }
+      if (TREE && 32 * wave >= b.rows) {  // (a wavefront without rows loads its share of the tiles, no more)
+        locate(at + 2 * KT);
+        continue;
+      }
       unsigned char const *const k_tile = lds + buffer * 2 * tile_bytes<DP>(), *const v_tile = k_tile + tile_bytes<DP>();
 
       floatx16 s[G];
@@ -618,6 +630,9 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
     }
   }
 
+  if (32 * wave >= b.rows) {
+    return;
+  }
   sum = over_halves(sum, [](float a, float b) { return a + b; });
   if (parts > 1) {  // left as it is, for the kernel below
     float *const part = P.parts + (long long)blockIdx.x * part_floats<DP>();
@@ -666,21 +681,24 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
   }
 }
 
-// The parts of a block together: a workgroup has 32 columns of its 128 rows, a wavefront 32 rows of these, in the order in which the kernel
-// above left them.  Parts are asked for four at a time: one after the other each is a trip to memory.
-template <class T, int DP, bool TREE>
+// The parts of a block together, in the order in which the kernel above left them: WAYS wavefronts have 32 columns of 32 rows, each every
+// WAYS-th part, asked for four at a time (one after the other each is a trip to memory), and then a share of the columns.
+template <class T, int DP, bool TREE, int WAYS>
 __global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const P) {
   fetch_kernel_arguments<sizeof(BlockParams), 0>();
-  constexpr int DB = DP / 32, kBatch = 4;
+  constexpr int DB = DP / 32, kBatch = 4, kFours = 4 / WAYS;
   typedef typename Vec<T>::x4 x4;
-  __shared__ int tree[TREE ? MI355_MAX_TREE_NODES : 1];
-  int const tid = threadIdx.x, lane = tid % 64, wave = tid / 64, h = lane / 32, c = lane % 32;
-  int const d = (int)blockIdx.x % DB, kv = (int)blockIdx.x / DB % P.kv_heads, block = (int)blockIdx.x / DB / P.kv_heads;
+  __shared__ paged::floatx4 shared_sums[WAYS][4][64];
+  __shared__ float tops[WAYS][32], weights[WAYS][32];
+  __shared__ short tree[TREE ? MI355_MAX_TREE_NODES : 1];
+  int const tid = threadIdx.x, lane = tid % 64, wave = tid / 64, way = wave % WAYS, h = lane / 32, c = lane % 32;
+  int const d = (int)blockIdx.x % DB, rows = (int)blockIdx.x / DB % WAYS * kFours + wave / WAYS;
+  int const kv = (int)blockIdx.x / (WAYS * DB) % P.kv_heads, block = (int)blockIdx.x / (WAYS * DB) / P.kv_heads;
   Block const b = block_of<TREE>(P, block);
-  if (!b.is || 32 * wave >= b.rows) {
+  if (!b.is || 32 * rows >= b.rows || 32 * d >= P.head_dim) {
     return;
   }
-  int parts = parts_of<DP>(P, b), slot = block * P.kv_heads + kv, step = P.blocks * P.kv_heads;
+  int parts = parts_of(P, b), slot = block * P.kv_heads + kv, step = P.blocks * P.kv_heads;
   if (TREE && P.sequences > 1) {
     Cut const cut = cut_of<DP>(P, -1, b.sequence);
     parts = cut.parts;
@@ -690,7 +708,7 @@ __global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const
   if (parts == 1) {
     return;  // (it has left the result)
   }
-  int const in_block = 32 * wave + c;
+  int const in_block = 32 * rows + c;
   bool const is_row = in_block < b.rows;
   float top = -INFINITY, sum = 0.0f;
   paged::floatx4 x[4];
@@ -698,23 +716,24 @@ __global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const
   for (int four = 0; four < 4; four++) {
     x[four] = paged::floatx4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  for (int i0 = 0; i0 < parts; i0 += kBatch) {
+  for (int i0 = way; i0 < parts; i0 += kBatch * WAYS) {
     float ref[kBatch], its[kBatch];
     paged::floatx4 y[kBatch][4];
 #pragma unroll
     for (int i = 0; i < kBatch; i++) {
-      float const *const part = P.parts + (long long)(slot + (i0 + i < parts ? i0 + i : parts - 1) * step) * part_floats<DP>();
+      int const which = i0 + i * WAYS < parts ? i0 + i * WAYS : i0;
+      float const *const part = P.parts + (long long)(slot + which * step) * part_floats<DP>();
       ref[i] = part[kRows * DP + 2 * in_block];
       its[i] = part[kRows * DP + 2 * in_block + 1];
 #pragma unroll
       for (int four = 0; four < 4; four++) {
-        y[i][four] = *reinterpret_cast<paged::floatx4 const *>(part + 4 * (((d * kWaves + wave) * 4 + four) * 64 + lane));
+        y[i][four] = *reinterpret_cast<paged::floatx4 const *>(part + 4 * (((d * kWaves + rows) * 4 + four) * 64 + lane));
       }
     }
     float const before = top;
 #pragma unroll
     for (int i = 0; i < kBatch; i++) {
-      ref[i] = i0 + i < parts ? ref[i] : -INFINITY;
+      ref[i] = i0 + i * WAYS < parts ? ref[i] : -INFINITY;
       top = fmaxf(top, ref[i]);
     }
     float const base = top == -INFINITY ? 0.0f : top, less = exp2_fast(before - base);
@@ -737,39 +756,59 @@ __global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const
       }
     }
   }
+  if constexpr (WAYS > 1) {
+    static_assert(WAYS == kWaves, "a workgroup is done with its rows, or joins them, as a whole");
+#pragma unroll
+    for (int four = 0; four < 4; four++) {
+      shared_sums[way][four][lane] = x[four];
+    }
+    if (h == 0) {
+      tops[way][c] = top;
+      weights[way][c] = sum;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAYS; w++) {
+      top = fmaxf(top, tops[w][c]);
+    }
+    float const base = top == -INFINITY ? 0.0f : top;
+    sum = 0.0f;
+    x[0] = paged::floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < WAYS; w++) {
+      float const by = exp2_fast(tops[w][c] - base);
+      sum += weights[w][c] * by;
+      x[0] += shared_sums[w][way][lane] * by;
+    }
+  }
   float const by = sum == 0.0f ? 0.0f : 1.0f / sum;
-  int const row = b.row0 + (is_row ? in_block : 0), token = quotient(row, P.group, P.group_magic);
+  int const row = b.row0 + (is_row ? in_block : 0), token = quotient(row, P.group, P.group_magic), d0 = 32 * d + 8 * way;
   T *const out = static_cast<T *>(P.out) + (long long)(b.row_of_q + token) * P.out_stride + (long long)(kv * P.group + row - token * P.group) * P.head_dim;
   bool good = true;
 #pragma unroll
-  for (int four = 0; four < 4; four++) {
-    x4 y;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      y[e] = static_cast<T>(x[four][e] * by);
-    }
-    int const at = 32 * d + 8 * four + 4 * h;
+  for (int four = 0; four < kFours; four++) {
+    int const at = d0 + 8 * four + 4 * h;
     if (is_row && at < P.head_dim) {
+      x4 y;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
+        y[e] = static_cast<T>(x[four][e] * by);
         good = good && __builtin_fabsf(x[four][e] * by) < INFINITY;
       }
       *reinterpret_cast<x4 *>(out + at) = y;
     }
   }
-  uint64_t again = __ballot(!good && is_row);
+  uint64_t again = __ballot(!good);
   if (again != 0) {
     if constexpr (TREE) {  // (every wavefront for itself: they write the same)
-      for (int i = lane; i < b.new_tokens; i += 64) {
-        tree[i] = P.parents[(long long)b.sequence * b.new_tokens + i];
-      }
+      fetch_tree(P, b, tree, lane, 64);
       paged::wait_lds_reads();
     }
     Row const r = row_of<TREE>(P, b, in_block, tree);
-    int const d1 = 32 * d + 32 < P.head_dim ? 32 * d + 32 : P.head_dim;
+    int const d1 = d0 + 8 * kFours < P.head_dim ? d0 + 8 * kFours : P.head_dim;
     again = (again | again >> 32) & 0xffffffffull;
     for (; again != 0; again &= again - 1) {
-      row_again<T, DP, TREE>(P, b, kv, of_lane(r, __builtin_ctzll(again)), tree, 32 * d, d1);
+      row_again<T, 32, TREE>(P, b, kv, of_lane(r, __builtin_ctzll(again)), tree, d0, d1);
     }
   }
 }
@@ -781,21 +820,31 @@ int launch_blocks(BlockParams P) {
   static_assert(kPerUnit<DP> * lds <= 160 * 1024, "LDS of a compute unit");
   P.row_blocks = (int)row_blocks((long long)P.new_tokens * P.group);
   P.blocks = (int)(P.starts == nullptr ? (long long)P.sequences * P.row_blocks : blocks_of(P.tokens, P.group, P.sequences));
-  // Blocks that do not fill the chip are cut along their keys, of which a part has kLeastTiles tiles at least.
+  // Blocks that do not fill the chip are cut along their keys.
   long long const items = (long long)P.blocks * P.kv_heads, keys = (long long)P.table_width * P.page_size;
-  long long const seen = P.window != 0 ? (long long)P.window + P.sinks + kRows : keys, tiles = ((seen < keys ? seen : keys) + kKeys<DP> - 1) / kKeys<DP>;
+  long long const seen = P.window != 0 ? (long long)P.window + P.sinks + kRows : keys, most = seen < keys ? seen : keys;
   long long const room = (long long)(state().scratch_bytes / sizeof(float)) / part_floats<DP>(), fill = 256 * kPerUnit<DP>;
   P.slots = (int)(fill < room ? fill : room);
   long long splits = P.slots / items;
-  splits = splits < tiles / kLeastTiles ? splits : tiles / kLeastTiles;
+  splits = splits < most / kLeastKeys ? splits : most / kLeastKeys;
   splits = splits < room / items ? splits : room / items;
   P.splits = splits < 1 ? 1 : (int)splits;
+  // Trees behind contexts of different lengths are cut where that evens out what workgroups have to do, joins included.  Measured (us, whole and cut;
+  // 8 heads of 128): 126 and 92 of 36 trees behind up to 4096 keys, 145 and 131 of 48, 63 and 53 of 36 behind up to 2000; against it 75 and 85 of 64 behind
+  // up to 2000, 22.7 and 29.2 of 48 behind up to 400.
+  if (TREE && P.sequences > 1 && P.splits == 1 && items * 5 <= P.slots * 4 && keys >= 1536) {
+    P.splits = 2;
+  }
   P.parts = static_cast<float *>(state().scratch());
   MI355_GRANT_LDS(fn, lds);
   long long const grid = TREE && P.sequences > 1 && P.splits > 1 ? P.slots : items * P.splits;
   MI355_HIP(launch_kernel(fn, dim3((unsigned)grid), dim3(kThreads), lds, state().stream(), P));
   if (P.splits > 1) {
-    MI355_HIP(launch_kernel(join_blocks_kernel<T, DP, TREE>, dim3((unsigned)(items * (DP / 32))), dim3(kThreads), 0, state().stream(), P));
+    // Four wavefronts to the parts of the same rows where there are many parts of few rows: 19.4 and 22.8 us with and without of 5 x 3 heads of 80 x up to
+    // 3001 keys, 65 rows, 14.9 and 15.6 of 1 x 8 of 128 x 1000, 48 rows; against it 37.9 and 35.4 of 12 x 8 of 128 x up to 4096, 96 rows.
+    bool const several = P.splits > 4 && items * (DP / 8) <= 1024;
+    auto *join = several ? join_blocks_kernel<T, DP, TREE, 4> : join_blocks_kernel<T, DP, TREE, 1>;
+    MI355_HIP(launch_kernel(join, dim3((unsigned)(items * (DP / (several ? 8 : 32)))), dim3(kThreads), 0, state().stream(), P));
   }
   return MI355_OK;
 }
