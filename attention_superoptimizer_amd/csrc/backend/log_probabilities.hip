@@ -513,8 +513,7 @@ template <class T>
 int launch_log(LogParams P, int rows) {
   constexpr int kChunk = 64 * kRounds * (16 / (int)sizeof(T));
   // As many workgroups to a row as leave two to a compute unit, each with a chunk for every wavefront at least.  Measured (us, one, two and four to a
-  // compute unit): 13.6, 12.6 and 13.6 of 64 rows of 131072 bf16 with 20 top tokens, 24.4 us being the two of 200 rows, against 26.1 and 24.7; alike for few
-  // rows.
+  // compute unit; 131072 bf16 a row, 20 top tokens): 13.6, 12.6 and 13.6 of 64 rows, 26.1, 24.4 and 24.7 of 200; alike for few rows.
   constexpr int kFill = 512;
   int const most = (P.vocabulary - 1) / (kWaves * kChunk) + 1, wanted = rows < kFill ? (kFill - 1) / rows + 1 : 1;
   P.row_parts = wanted < most ? wanted : most;
