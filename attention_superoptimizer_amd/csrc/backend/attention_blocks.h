@@ -529,6 +529,17 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
     load(0);
     uint64_t next_there = there;
     locate(part + KT);
+    if (32 * __builtin_amdgcn_readfirstlane(wave) >= b.rows) {  // a wavefront without rows loads its share of the tiles, no more
+      for (int at = part, buffer = 1; at < part_end; at += KT, buffer ^= 1) {
+        paged::wait_loads<0>();
+        __syncthreads();
+        if (at + KT < part_end) {
+          load(buffer);
+        }
+        locate(at + 2 * KT);
+      }
+      continue;
+    }
     for (int at = part, buffer = 0; at < part_end; at += KT, buffer ^= 1) {
       uint64_t const is_there = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(next_there >> 32)) << 32 |
                                 (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)next_there);
@@ -537,10 +548,6 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
       __syncthreads();  // the tile is here, and everyone is done with the one before
       if (at + KT < part_end) {
         load(buffer ^ 1);
-      }
-      if (TREE && 32 * wave >= b.rows) {  // (a wavefront without rows loads its share of the tiles, no more)
-        locate(at + 2 * KT);
-        continue;
       }
       unsigned char const *const k_tile = lds + buffer * 2 * tile_bytes<DP>(), *const v_tile = k_tile + tile_bytes<DP>();
 

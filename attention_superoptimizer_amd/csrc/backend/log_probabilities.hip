@@ -6,7 +6,13 @@
 //
 // The top tokens are found on the way: a wavefront keeps a bound that it knows `top` of its logits to reach, and only logits above
 // it are looked at one by one.  The bound is the top-th of the lanes' own maxima, which the sums need anyway; after the first few
-// thousand logits hardly any passes it.
+// thousand logits hardly any passes it.  What passed is told apart by counting: an entry's place is the number of better ones.
+//
+// Few rows are cut over workgroups, of which the last to come (a ticket) puts the parts together, always in the same order.
+//
+// Measured: 83 us of 4096 rows of 50021 fp16 with the top token (410 MB, 4.9 TB/s, and 71 us of vector instructions: a read of so much takes 66),
+// 143 of fp32 (820 MB, 5.7 TB/s), 12.5 of 64 rows of 131072 bf16 with twenty (17 MB; trips to memory one after the other and the bounds),
+// 7.7 of one row of 32000 fp32 with five, of which a launch is 3.
 #include "common.h"
 #include "mi355_kernels/kernarg.h"
 #include "slices.h"

@@ -970,13 +970,13 @@ int launch_rows(ParamsOf<MASK> const &P, int kv_heads, bool passing) {
   if (rows <= 16) {
     return launch_group<T, DP, 1, MASK>(P, kv_heads, passing);
   }
-  if constexpr (MASK == kPlain || DP <= 128) {  // (masked heads have as many rows as attention_blocks.hip leaves here)
+  if constexpr (MASK == kPlain) {  // (masked heads have no more rows: attention_blocks.hip)
     if (rows <= 32 || DP > 128) {
       return launch_group<T, DP, 2, MASK>(P, kv_heads, passing);
     }
-  }
-  if constexpr (MASK == kPlain ? DP <= 128 : DP <= 64) {
-    return rows <= 48 ? launch_group<T, DP, 3, MASK>(P, kv_heads, passing) : launch_group<T, DP, 4, MASK>(P, kv_heads, passing);
+    if constexpr (DP <= 128) {
+      return rows <= 48 ? launch_group<T, DP, 3, MASK>(P, kv_heads, passing) : launch_group<T, DP, 4, MASK>(P, kv_heads, passing);
+    }
   }
   return fail(MI355_ERR_UNSUPPORTED, "paged attention: %lld rows of heads of %d", rows, P.head_dim);
 }

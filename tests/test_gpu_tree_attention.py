@@ -69,7 +69,7 @@ def _check(seed, nodes, lengths, kv_heads=2, group=4, head=64, page_size=16, kin
 
 @pytest.mark.parametrize("kind", ["fp16", "bf16"])
 @pytest.mark.parametrize("head", [8, 64, 72, 80, 96, 128, 136, 192, 200, 256])
-@pytest.mark.parametrize("nodes", [7, 40])
+@pytest.mark.parametrize("nodes", [4, 7, 40])
 def test_head_sizes(rt, kind, head, nodes):
     _check(head, nodes, [137, 41, 230], head=head, kind=kind)
 
@@ -88,6 +88,7 @@ def test_the_largest_trees(rt, shape):
 @pytest.mark.parametrize("heads_first", [False, True])
 @pytest.mark.parametrize("page_size", [1, 2, 7, 16, 24, 32, 100, 128, 500])
 def test_page_sizes(rt, page_size, heads_first):
+    _check(page_size, 4, [50, 99, 257, 400], page_size=page_size, heads_first=heads_first, flat=heads_first)
     _check(page_size, 12, [50, 99, 257, 400], page_size=page_size, heads_first=heads_first, flat=heads_first, kind="bf16")
     _check(page_size, 40, [50, 99, 257, 400], page_size=page_size, heads_first=heads_first, flat=heads_first)
 
@@ -107,7 +108,7 @@ def test_heads(rt, kind, kv_heads, group, nodes):
 
 
 @pytest.mark.parametrize("kind", ["fp16", "bf16"])
-@pytest.mark.parametrize("head,nodes,group", [(128, 12, 4), (64, 64, 8), (80, 13, 5), (256, 20, 2), (192, 30, 4)])
+@pytest.mark.parametrize("head,nodes,group", [(128, 12, 4), (64, 64, 8), (128, 4, 4), (64, 15, 1), (80, 3, 5), (256, 7, 2), (80, 13, 5), (256, 20, 2), (192, 30, 4)])
 def test_long_caches(rt, kind, head, nodes, group):
     _check(head, nodes, [5000, 137, 2900], nodes and 2, group, head, kind=kind, std=2.0)
     _check(head, nodes, [9000], 1, group, head, page_size=1, kind=kind)
@@ -115,6 +116,7 @@ def test_long_caches(rt, kind, head, nodes, group):
 
 @pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
 def test_scales(rt, scale):
+    _check(3, 3, [100, 250], scale=scale)
     _check(3, 12, [100, 250], scale=scale)
     _check(3, 50, [100, 250], scale=scale)
 
@@ -125,7 +127,7 @@ def test_many_sequences(rt):
 
 
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
-@pytest.mark.parametrize("nodes", [9, 40])
+@pytest.mark.parametrize("nodes", [5, 9, 40])
 @pytest.mark.parametrize("kind", ["fp16", "bf16"])
 def test_places_that_are_not_seen_hold_anything(rt, value, nodes, kind):
     """A node's key and value that its descendants alone see."""
@@ -203,7 +205,7 @@ def _abi_call(abi, **x):
                                     x["table"], x["width"], x["lengths"], x["parents"], x["sequences"], x["nodes"], x["heads"], x["scale"])
 
 
-@pytest.mark.parametrize("nodes", [6, 33])
+@pytest.mark.parametrize("nodes", [3, 6, 33])
 def test_strides_and_what_lies_between(rt, abi, nodes):
     g = G.KNGraph()
     try:
