@@ -43,6 +43,7 @@ struct BlockParams {
   int blocks;      // of all sequences, at most
   int slots;       // workgroups that the chip holds together
   int splits;      // parts that the keys of a block are cut into, at most
+  int least;       // keys of a part, at least: whole tiles
   float *parts;    // of every block and part: sums as the lanes hold them, then reference and sum of weights of its rows
   unsigned page_magic, group_magic;
   uint32_t q_keep, q_flip;
@@ -114,12 +115,8 @@ __device__ __forceinline__ float sum_of(Vec<__bf16>::x8 p, float sum) {
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1); }
 
 constexpr int kThreads = 256, kWaves = 4;
-// Of a part: one sequence, 8 heads of 128, 1000 keys, 48 rows takes 17.2, 13.8 and 15.1 us with 256, 128 and 64.
-constexpr int kLeastKeys = 128;
 template <int DP>
 constexpr int kKeys = DP == 192 ? 32 : 64;  // of a tile
-template <int DP>
-constexpr int kLeastTiles = kLeastKeys / kKeys<DP>;
 template <int DP, bool TREE>
 constexpr int kStepsOf = DP != 96 ? 2048 : (TREE ? 512 : 1024);  // keys of a run whose places a workgroup holds in LDS (96: three workgroups fit)
 template <int DP>
@@ -358,7 +355,7 @@ __device__ __forceinline__ Cut cut_of(BlockParams const &P, int work, int sequen
     return __builtin_amdgcn_readlane(paged::wave_upto(x), 63) * each;
   };
   int run = (total([](int tiles) { return tiles; }) + P.slots - 1) / P.slots;
-  run = run < kLeastTiles<DP> ? kLeastTiles<DP> : run;
+  run = run < P.least / kKeys<DP> ? P.least / kKeys<DP> : run;
   auto parts_of = [&](int tiles) { return (int)(((unsigned)tiles + run - 1) / (unsigned)run); };
   while (total(parts_of) > P.slots) {
     run += 1 + run / 16;
@@ -378,9 +375,9 @@ __device__ __forceinline__ Cut cut_of(BlockParams const &P, int work, int sequen
   }
   return cut;
 }
-// Any other block is cut into as many parts as all may have, of kLeastKeys or more.
+// Any other block is cut into as many parts as all may have, of P.least keys or more.
 __device__ __forceinline__ int parts_of(BlockParams const &P, Block const &b) {
-  int const most = b.end / kLeastKeys;
+  int const most = b.end / P.least;
   return most < 1 ? 1 : (most < P.splits ? most : P.splits);
 }
 // of a block's part
@@ -852,7 +849,11 @@ int launch_blocks(BlockParams P) {
   long long const room = (long long)(state().scratch_bytes / sizeof(float)) / part_floats<DP>(), fill = 256 * kPerUnit<DP>;
   P.slots = (int)(fill < room ? fill : room);
   long long splits = P.slots / items;
-  splits = splits < most / kLeastKeys ? splits : most / kLeastKeys;
+  // Parts of a tile where that gives no more than one for each compute unit and sixteen to be joined (a trip to memory), of two otherwise.  Measured
+  // (us, two and one; 8 heads of 128, 48 rows): 14.8 and 14.0 of one sequence of 1000 keys, 13.2 and 11.5 of 300; against it 15.1 and 16.8 of one of 2000,
+  // 17.8 and 19.4 of three of up to 1000, 96 rows.
+  P.least = most <= 1024 && items * ((most + 63) / 64) <= 256 ? 64 : 128;
+  splits = splits < most / P.least ? splits : most / P.least;
   splits = splits < room / items ? splits : room / items;
   P.splits = splits < 1 ? 1 : (int)splits;
   // Trees behind contexts of different lengths are cut where that evens out what workgroups have to do, joins included.  Measured (us, whole and cut;
