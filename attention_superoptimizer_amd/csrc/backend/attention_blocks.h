@@ -145,30 +145,36 @@ __device__ __forceinline__ Block block_of(BlockParams const &P, int block) {
     b.row_of_q = b.sequence * P.new_tokens;
     b.new_tokens = P.new_tokens;
   } else {
-    for (int base = 0;; base += 64) {
-      if (base >= P.sequences) {
-        return b;
-      }
-      int const at = base + lane;
+    // A sequence's blocks are numbered from before(its first token) + its own number on, which leaves room for all of them: the last sequence
+    // that begins no later than the block is found among 64 at a time.
+    auto before = [&](int token) { return token * P.group / kRows; };
+    int first = 0;
+    for (int n = P.sequences, step = 0; step != 1;) {
+      step = (n + 63) / 64;
+      int const at = lane * step < n ? first + lane * step : first;
       auto start = [&](int i) {
         int const s = P.starts[i];
         return s < 0 ? 0 : (s < P.tokens ? s : P.tokens);
       };
-      int const from = at < P.sequences ? start(at) : 0, to = at < P.sequences ? start(at + 1) : 0;
-      int const its = to > from ? (int)(((long long)(to - from) * P.group + kRows - 1) / kRows) : 0, upto = paged::wave_upto(its);
-      uint64_t const past = __ballot(upto > block);
-      if (past != 0) {
-        int const which = __builtin_ctzll(past);
-        b.sequence = base + which;
-        b.row_of_q = __builtin_amdgcn_readlane(from, which);
-        b.new_tokens = __builtin_amdgcn_readlane(to, which) - b.row_of_q;
-        block -= __builtin_amdgcn_readlane(upto - its, which);
-        // (as in_order, sequence by sequence: 199 -> 178 us of four chunks of up to 3000 behind up to 7001 keys, 5 x 3 heads of 80)
-        block = P.window == 0 ? __builtin_amdgcn_readlane(its, which) - 1 - block : block;
-        break;
+      int const from = start(at), to = start(at + 1);
+      uint64_t const begun = __ballot(lane * step < n && before(from) + at <= block);
+      if (begun == 0) {
+        return b;
       }
-      block -= __builtin_amdgcn_readlane(upto, 63);
+      int const which = 63 - __builtin_clzll(begun);
+      first += which * step;
+      n = n - which * step < step ? n - which * step : step;
+      b.row_of_q = __builtin_amdgcn_readlane(from, which);
+      b.new_tokens = __builtin_amdgcn_readlane(to, which) - b.row_of_q;
     }
+    b.sequence = first;
+    int const its = b.new_tokens > 0 ? (b.new_tokens * P.group + kRows - 1) / kRows : 0;
+    block -= before(b.row_of_q) + first;
+    if (block >= its) {
+      return b;
+    }
+    // (as in_order, sequence by sequence: 199 -> 178 us of four chunks of up to 3000 behind up to 7001 keys, 5 x 3 heads of 80)
+    block = P.window == 0 ? its - 1 - block : block;
   }
   b.is = true;
   int const R = b.new_tokens * P.group, most = P.table_width * P.page_size, told = P.lengths[b.sequence];

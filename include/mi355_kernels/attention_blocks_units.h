@@ -8,7 +8,7 @@ namespace blocks {
 constexpr int kRows = 128;                          // of a block
 constexpr long long kWorkgroups = (1LL << 24) - 1;  // of 256 threads
 
-// Blocks of a ragged batch, of one more for every sequence at most.
+// Blocks of a ragged batch: sequence i's begin at blocks_of(its first token, group, i), and fit before the next one's.
 inline long long blocks_of(long long tokens, long long group, long long sequences) { return tokens * group / kRows + sequences; }
 // Blocks of a sequence with `rows` rows for each key-value head, and sequences of a launch.
 inline long long row_blocks(long long rows) { return (rows + kRows - 1) / kRows; }

@@ -104,6 +104,13 @@ def test_ragged_batches(rt, kind, new, past, window):
         _check(rows, new, [n + p for n, p in zip(new, past)], window, 6, kind=kind, ragged=True, kv_heads=1, group=2, head=80, spare_rows=9)
 
 
+@pytest.mark.parametrize("sequences", [64, 65, 1000, 4200])
+def test_ragged_batches_of_many_sequences(rt, sequences):
+    new = [i * 7 % 4 for i in range(sequences)]
+    new[sequences // 3] = 40
+    _check(sequences, new, [n + i % 3 for i, n in enumerate(new)], 2, 1, head=8, page_size=8, ragged=True, kv_heads=1, group=7, spare_rows=3)
+
+
 @pytest.mark.parametrize("kind", ["fp16", "bf16"])
 @pytest.mark.parametrize("head", [64, 80, 128, 192, 256])
 @pytest.mark.parametrize("window", [0, 2500])
