@@ -5,14 +5,14 @@
 // and the two sums relative to it.
 //
 // The top tokens are found on the way: a wavefront keeps a bound that it knows `top` of its logits to reach, and only logits above
-// it are looked at one by one.  The bound is the top-th of the lanes' own maxima, which the sums need anyway; after the first few
+// it are looked at one by one.  The bound is what the top-th of the lanes' own maxima reaches, which the sums need anyway; after the first few
 // thousand logits hardly any passes it.  What passed is told apart by counting: an entry's place is the number of better ones.
 //
 // Few rows are cut over workgroups, of which the last to come (a ticket) puts the parts together, always in the same order.
 //
 // Measured: 83 us of 4096 rows of 50021 fp16 with the top token (410 MB, 4.9 TB/s, and 71 us of vector instructions: a read of so much takes 66),
-// 143 of fp32 (820 MB, 5.7 TB/s), 12.5 of 64 rows of 131072 bf16 with twenty (17 MB; trips to memory one after the other and the bounds),
-// 7.7 of one row of 32000 fp32 with five, of which a launch is 3.
+// 143 of fp32 (820 MB, 5.7 TB/s), 11.7 of 64 rows of 131072 bf16 with twenty (17 MB; trips to memory one after the other and the bounds),
+// 7.5 of one row of 32000 fp32 with five, of which a launch is 3.
 #include "common.h"
 #include "mi355_kernels/kernarg.h"
 #include "slices.h"
@@ -27,6 +27,9 @@ namespace {
 
 constexpr int kPending = 192;   // tokens that a wavefront has yet to look at; more than 128 are thinned out
 constexpr int kGathered = 512;  // entries of a workgroup that are told apart all at once
+// Maxima of a lane that bound more than 40 top tokens: what so many of 64 lanes reach rules out little (64 of 131072, 64 rows: 25.6 us with one, 15.3 with
+// two, 16.0 with four; 33: 12.3 and 12.8; twenty: 11.7, 12.4 and 14.1).
+constexpr int kMaxima = 2;
 constexpr int kThreads = 256, kWaves = kThreads / 64, kRounds = 4, kLargestParts = 64;
 
 struct LogParams {
@@ -119,17 +122,34 @@ __device__ __forceinline__ T sorted(T x, int lane, bool first) {
 // the greatest 64 of a list greatest first and one greatest last, greatest first
 __device__ __forceinline__ uint64_t merged(uint64_t a, uint64_t back, int lane) { return cleaned<32>(back > a ? back : a, lane, true); }
 
-// The n-th greatest of the lanes' values (n <= 64; no NaN), and the one in place (n + 3) / 4.
+// What n of the lanes' values reach, N of a lane (no NaN), and what (n + 3) / 4 do: the upper 16 bits of the n-th greatest, found bit by bit (0.3 us
+// of one of a lane; sorting them takes 1.2).
 struct Two {
   float nth, earlier;
 };
-__device__ __forceinline__ Two nth_of_lanes(float value, int n, int lane) {
-  if (n == 1) {
-    float const most = over_lanes(value, [](float x, float y) { return fmaxf(x, y); });
-    return {most, most};
+template <int N>
+__device__ __forceinline__ Two nth_of_lanes(float const (&value)[N], int n) {
+  uint32_t x[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    x[i] = ordered(value[i]);
   }
-  uint32_t const x = sorted(ordered(value), lane, true);
-  return {unordered((uint32_t)__builtin_amdgcn_readlane((int)x, n - 1)), unordered((uint32_t)__builtin_amdgcn_readlane((int)x, (n + 3) / 4 - 1))};
+  auto reach = [&](uint32_t least) {
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      count += __builtin_popcountll(__ballot(x[i] >= least));
+    }
+    return count;
+  };
+  uint32_t const lowest = ordered(-INFINITY);
+  uint32_t nth = 0, earlier = 0;
+#pragma unroll
+  for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
+    nth = reach(nth | bit) >= n ? nth | bit : nth;
+    earlier = reach(earlier | bit) >= (n + 3) / 4 ? earlier | bit : earlier;
+  }
+  return {unordered(nth > lowest ? nth : lowest), unordered(earlier > lowest ? earlier : lowest)};
 }
 // the least value above x
 __device__ __forceinline__ float above(float x) {
@@ -236,6 +256,7 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
   }
 
   Sums own = {-INFINITY, 0.0f, 0.0f};
+  float maxima[kMaxima] = {-INFINITY, -INFINITY};  // of the halves of what a lane sees of each chunk
   float bound = -INFINITY, quarter = -INFINITY;  // that as many as asked for, and a quarter of these, reach
   int waiting = 0;    // tokens of this wavefront's that may be among the top ones
   uint64_t best = 0;  // the best of those that were thinned out, a lane each, best first
@@ -260,11 +281,15 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
       }
       float x[kRounds * V], top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kRounds * V; i++) {
-        x[i] = static_cast<float>(h.x[i / V][i % V]);
-        top = fmaxf(top, x[i]);
+      for (int j = 0; j < kMaxima; j++) {
+#pragma unroll
+        for (int i = j * (kRounds * V / kMaxima); i < (j + 1) * (kRounds * V / kMaxima); i++) {
+          x[i] = static_cast<float>(h.x[i / V][i % V]);
+          maxima[j] = fmaxf(maxima[j], x[i]);
+        }
+        top = fmaxf(top, maxima[j]);
       }
-      own = moved_to(own, fmaxf(own.m, top), P.scale);
+      own = moved_to(own, top, P.scale);
       float const base = own.m == -INFINITY ? 0.0f : own.m;
       float s = 0.0f, t = 0.0f;
 #pragma unroll
@@ -279,7 +304,15 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
       if constexpr (TOP) {
         if (__any(top > bound)) {
           // (an element that equals an earlier bound comes behind as many that are no less)
-          Two const reached = nth_of_lanes(own.m, P.top, lane);
+          Two reached;
+          if (P.top == 1) {
+            reached.nth = reached.earlier = over_lanes(top, [](float x, float y) { return fmaxf(x, y); });
+          } else if (P.top <= 40) {
+            float const most[1] = {top};
+            reached = nth_of_lanes(most, P.top);
+          } else {
+            reached = nth_of_lanes(maxima, P.top);
+          }
           float const least = reached.nth > bound ? reached.nth : above(bound);
           bound = fmaxf(bound, reached.nth);
           quarter = reached.earlier;
