@@ -14,7 +14,7 @@
 // * Blocks that leave compute units without work are cut along their keys (of trees so that all parts are alike), and joined by a second
 //   kernel in the order of the keys, so that results do not depend on who comes first.
 //
-// Measured (8 key-value heads of 4 query heads of 128, bf16): 555 us of one prompt of 8192 tokens (550 GFLOP, 990 TFLOP/s), 158 to 171 within a
+// Measured (8 key-value heads of 4 query heads of 128, bf16): 555 to 600 us of one prompt of 8192 tokens (550 GFLOP, 990 TFLOP/s), 158 to 171 within a
 // window of 1024 (129 GFLOP, 750 to 820 TFLOP/s); a large matrix product reaches 1270.  What bounds it are the two wavefronts of a SIMD taking
 // turns: matrix instructions fill 39 % of its cycles and vector instructions, exponentials nearly half of them, 49 %.
 #pragma once

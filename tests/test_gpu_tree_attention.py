@@ -235,6 +235,31 @@ def test_strides_and_what_lies_between(rt, abi, nodes):
         g.close()
 
 
+def test_queues_side_by_side(rt, abi):
+    """Keys cut over workgroups, whose sums each queue has in memory of its own."""
+    shapes = [(20, [3000, 700, 1500]), (33, [2500]), (40, [900] * 5)]
+    cases = [_case(40 + i, nodes, lengths, 2, 4, 64, 16, "bf16") for i, (nodes, lengths) in enumerate(shapes)]
+    graphs, outs = [], []
+    try:
+        for *x, _ in cases:
+            g = G.KNGraph()
+            graphs.append(g)
+            kinds = ("bf16",) * 3 + (None,) * 3
+            outs.append(g.tree_attention(*(put(g, a) if kind is None else put(g, a, kind) for a, kind in zip(x, kinds)), scale=0.125))
+        for _ in range(10):
+            for queue, g in enumerate(graphs):
+                assert abi.mi355_queue_select(queue) == 0
+                g.execute_all()
+        assert abi.mi355_sync() == 0
+        for (*x, values), o in zip(cases, outs):
+            want, bound = _expected(x[0], values, x[4], x[5], 0.125, "bf16")
+            check(read(o).reshape(want.shape), want, bound)
+    finally:
+        abi.mi355_queue_select(0)
+        for g in reversed(graphs):
+            g.close()
+
+
 def test_refusals(rt, abi):
     g = G.KNGraph()
     try:
