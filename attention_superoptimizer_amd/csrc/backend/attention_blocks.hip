@@ -70,8 +70,8 @@ int fill(BlockParams &P, char const *name, void const *q, long long q_stride, vo
 }
 
 // Few rows of a key-value head, as many in every sequence: a head's keys are dealt over workgroups, a wavefront has 32 of them at a time to
-// itself (paged_attention.h), and reading the cache is what counts.  Measured (us, that and blocks; heads of 128 unless said): 12.0 and 16.0 of 1
-// sequence x 8 heads within a window of 4096, 4 rows, 85 and 106 of 64 x 8 within 2048, 4 rows, 9.9 and 12.9 of 1 x 8 x 1000 keys, 8 rows, 19.9 and 25.2
+// itself (paged_attention.h), and reading the cache is what counts.  Measured (us, that and blocks; heads of 128 unless said): 11.4 and 16.0 of 1
+// sequence x 8 heads within a window of 4096, 4 rows, 85 and 106 of 64 x 8 within 2048, 4 rows, 10.4 and 12.9 of 1 x 8 x 1000 keys, 8 rows, 19.9 and 25.2
 // of 8 x 8 within 2048, 16 rows, 51 and 68 of 16 x 8 heads of 256 within 2048, 16 rows; against it 41 and 39 of 32 x 8 heads of 64 x up to 4096, 16
 // rows, 24.1 and 21.4 of 5 x 3 heads of 256 x up to 3001, 15 rows, and with 32 rows 56 and 40 of the same heads of 64, 86 and 64 of 32 x 8 x up to 4096,
 // 16.4 and 12.4 of 1 x 8 x 1000.

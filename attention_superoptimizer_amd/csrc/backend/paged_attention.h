@@ -952,7 +952,11 @@ int launch_group(ParamsOf<MASK> const &P, int kv_heads, bool passing) {
       }
     }
     bool const few = RG == 1 ? heads <= 96 : heads <= 48 || (heads <= 256 && heads * units <= 300 << 10);
-    if (few && units >= 512) {
+    // with masks, whose first steps take longer, eight for few heads of fewer keys too: 12.1 and 11.4 us of 8 heads within a window of 4096, one
+    // token, 15.9 and 13.2 of trees of 16 rows behind 4000 keys, 13.9 and 11.7 of 15 heads of 80, 15 rows, behind up to 3001; against it 8.8 and 9.3 of 8
+    // within 1000, 9.9 and 10.4 of a tree of 8 rows behind 1000
+    bool const fewer = MASK != kPlain && heads <= 32 && keys >= (MASK == kTree ? 768 : 1536);
+    if ((few && units >= 512) || fewer) {
       return launch_paged<T, DP, RG, 8, false, MASK>(P, kv_heads);
     }
   }
