@@ -246,7 +246,7 @@ __device__ __forceinline__ float bias_of(int keys) {
 }
 
 // A weight of zero does not keep an infinity or NaN among the values out of a sum: rows with one in their result are done again, a
-// wavefront a row, key by key, columns d0 up to d1.  (In the loop over tiles such values would have to be looked for in every tile that
+// wavefront a row, key by key, columns d0 up to d1 (but for those whose sum of weights is none: a key that they see makes them so).  (In the loop over tiles such values would have to be looked for in every tile that
 // not all rows see.)  `r` is the same in every lane.
 template <class T, int DP, bool TREE>
 __device__ void row_again(BlockParams const &P, Block const &b, int kv, Row r, short const *tree, int d0, int d1) {
@@ -703,7 +703,7 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
       }
     }
   }
-  uint64_t again = __ballot(!good && is_row);
+  uint64_t again = __ballot(!good && sum == sum && is_row);
   again = (again | again >> 32) & 0xffffffffull;
   for (; again != 0; again &= again - 1) {
     row_again<T, DP, TREE>(P, b, kv, of_lane(r, __builtin_ctzll(again)), tree, 0, P.head_dim);
@@ -827,7 +827,7 @@ __global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const
       *reinterpret_cast<x4 *>(out + at) = y;
     }
   }
-  uint64_t again = __ballot(!good);
+  uint64_t again = __ballot(!good && sum == sum);
   if (again != 0) {
     if constexpr (TREE) {  // (every wavefront for itself: they write the same)
       fetch_tree(P, b, tree, lane, 64);

@@ -231,6 +231,33 @@ def test_places_that_are_not_seen_hold_anything(rt, value, new):
         assert (np.isnan(wild) if np.isnan(value) else wild == value).all()
 
 
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("new,length", [(1, 300), (4, 300), (40, 300), (40, 3000), (600, 900)])
+def test_keys_that_are_not_finite(rt, value, new, length):
+    """Rows that see such a key, whose score is no number or an infinity of either sign, and rows that do not."""
+    q, k, v, table, n, values = _case(18, [new], [length], 1, 3, 80, 16, "bf16")
+    want, bound = _expected(q, values, [new], [length], 200, 6, 0.1, "bf16")
+    j = length - 1 - new // 2
+    k[table[0, j // 16], j % 16] = 0.0
+    k[table[0, j // 16], j % 16, :, 5] = value
+    got = _run(q, k, v, table, n, "bf16", 200, 6, 0.1)
+    sees = window_seen(length, new, 200, 6)[:, j]
+    assert sees.any()
+    check(got[~sees], want[~sees], bound[~sees])
+    wild = np.isnan(got[sees]).all(-1)
+    if np.isnan(value):
+        assert wild.all()
+    else:
+        # a score of minus infinity is a key of no weight
+        down = (q[sees, :, 5] * np.sign(value)) < 0
+        without = window_seen(length, new, 200, 6)
+        without[:, j] = False
+        other, off = attended(q, values[0][0][:length], values[0][1][:length], without, 0.1, "bf16")
+        np.testing.assert_array_equal(wild, ~down)
+        assert new == 1 or (down.any() and not down.all())
+        check(got[sees][down], other[sees][down], off[sees][down])
+
+
 @pytest.mark.parametrize("ragged", [False, True])
 def test_such_places_among_keys_that_several_workgroups_read(rt, ragged):
     q, k, v, table, n, values = _case(16, [40], [3000], 1, 3, 128, 16, "fp16")
