@@ -392,7 +392,7 @@ constexpr int part_floats() { return kRows * (DP + 2); }
 
 template <class T, int DP, bool TREE>
 __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kernel(BlockParams const P) {
-  fetch_kernel_arguments<sizeof(BlockParams), 1>();
+  fetch_kernel_arguments<sizeof(BlockParams), 0>();  // (gridDim is not read: no word behind them is the launch's)
   constexpr int KT = kKeys<DP>, G = KT / 32, C = DP / 8, LOADS = KT * C / kThreads, KK = DP / 16, DB = DP / 32, kSteps = kStepsOf<DP, TREE>;
   typedef typename Vec<T>::x8 x8;
   typedef typename Vec<T>::x4 x4;
