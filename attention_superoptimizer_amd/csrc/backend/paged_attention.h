@@ -700,13 +700,15 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
     float *const mine = P.parts + (2 * (long long)me + (first == 0 ? 1 : 0)) * part_floats<DP, RG>();
     auto of_sum = [](float all) { return all == 0.0f ? 0.0f : 1.0f / (1.0f + kPart<T>) / all; };
     T *const out = static_cast<T *>(P.out) + (long long)sequence * P.new_tokens * P.out_stride + (long long)kv * P.group * P.head_dim;
-    auto store_row = [&](int row, int d, floatx4 x, float by) {  // row of the head, columns d .. d + 3
+    // Row of the head, columns d .. d + 3.  One without a weight (by is zero) is zeros whatever its sums are: where no row of a tile has a weight, an
+    // infinity or NaN among the values is in them all the same.
+    auto store_row = [&](int row, int d, floatx4 x, float by) {
       if (d < P.head_dim) {
         int const t = P.new_tokens == 1 ? 0 : quotient(row, P.group, P.group_magic);
         x4 y;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          y[e] = static_cast<T>(x[e] * by);
+          y[e] = static_cast<T>(by == 0.0f ? 0.0f : x[e] * by);
         }
         *reinterpret_cast<x4 *>(out + t * P.out_stride + (row - t * P.group) * P.head_dim + d) = y;
       }
