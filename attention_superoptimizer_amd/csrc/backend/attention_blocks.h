@@ -779,7 +779,7 @@ __global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const
 #pragma unroll
     for (int i = 0; i < kBatch; i++) {
       float const by = exp2_fast(ref[i] - base);
-      sum += ref[i] > -INFINITY ? its[i] * by : 0.0f;
+      sum += its[i] * by;  // (NaN where every score is NaN that the row sees in the part, which then has no reference)
 #pragma unroll
       for (int four = 0; four < 4; four++) {  // (a part without tiles left no sums)
         paged::floatx4 const z = by * y[i][four];
