@@ -240,6 +240,9 @@ __device__ __forceinline__ Row row_of(BlockParams const &P, Block const &b, int 
 }
 // weights are at most 2^(bias + kSlack)
 constexpr float kSlack = 6.0f;
+// Weights are 2^(scale s + (bias - scale ref)) with one rounding of what is in brackets, which all weights have alike; from a reference of 2^25 on it would take them
+// past the types' ends.  Above this the difference of scores comes first.
+constexpr float kLarge = 0x1p20f;
 template <class T>
 __device__ __forceinline__ float bias_of(int keys) {
   return std::is_same<T, _Float16>::value ? 9.0f : (float)(__builtin_clz((unsigned)keys | 1u) - 33) - kSlack;
@@ -284,7 +287,7 @@ __device__ void row_again(BlockParams const &P, Block const &b, int kv, Row r, s
       }
     }
     x = P.q_keep == 0 ? x * 0.0f : x;
-    return (P.q_flip != 0 ? -x : x) * P.scale;
+    return P.q_flip != 0 ? -x : x;
   };
   float high = -INFINITY;
   bool wild = false;
@@ -304,10 +307,10 @@ __device__ void row_again(BlockParams const &P, Block const &b, int kv, Row r, s
   for (int i = 0; i < N; i++) {
     o[i] = 0.0f;
   }
-  float const base = high == -INFINITY ? 0.0f : bias_of<T>(b.end) - high;
+  float const base = high == -INFINITY ? 0.0f : high, bias = bias_of<T>(b.end);
   for (int key = 0; key < b.end && !wild; key += 64) {
     uint32_t const at = find(key + lane);
-    float const w = at == ~0u ? 0.0f : exp2_fast(score(at) + base);
+    float const w = at == ~0u ? 0.0f : exp2_fast((score(at) - base) * P.scale + bias);
     total += w;
     for (uint64_t left = __ballot(at != ~0u); left != 0; left &= left - 1) {
       int const j = __builtin_ctzll(left);
@@ -464,7 +467,8 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
   }
 
   floatx16 acc[DB];
-  float ref = -INFINITY, sum = 0.0f;
+  float ref = -INFINITY, base = 0.0f, sum = 0.0f;
+  bool large = false;  // some row's reference, times the scale
 #pragma unroll
   for (int d = 0; d < DB; d++) {
 #pragma unroll
@@ -625,17 +629,27 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
           top = fmaxf(top, s[j][e]);
         }
       }
-      top = over_halves(top, [](float a, float b) { return fmaxf(a, b); }) * P.scale;
-      if (__any(top > ref + kSlack || (ref == -INFINITY && top > ref))) {
-        float const most = fmaxf(ref, top), less = exp2_fast(ref - (most == -INFINITY ? 0.0f : most));
+      top = over_halves(top, [](float a, float b) { return fmaxf(a, b); });
+      if (__any((top - ref) * P.scale > kSlack) || large) {
+        float const most = fmaxf(ref, top), from = most == -INFINITY ? 0.0f : most, less = exp2_fast((ref - from) * P.scale);
         ref = most;
         sum *= less;
 #pragma unroll
         for (int d = 0; d < DB; d++) {
           acc[d] *= less;
         }
+        large = __any(__builtin_fabsf(from) * P.scale > kLarge);
+        base = most == -INFINITY ? 0.0f : (large ? bias : bias - from * P.scale);
+        if (large) {
+#pragma unroll
+          for (int j = 0; j < G; j++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+              s[j][e] -= from;
+            }
+          }
+        }
       }
-      float const base = ref == -INFINITY ? 0.0f : bias - ref;
 
       // Weights of sixteen keys at a time, and their products with the values.  O^T: lane has columns 32 d + 8 (e / 4) + 4 h + e % 4 of row c.
 #pragma unroll
@@ -770,7 +784,7 @@ __global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const
       ref[i] = i0 + i * WAYS < parts ? ref[i] : -INFINITY;
       top = fmaxf(top, ref[i]);
     }
-    float const base = top == -INFINITY ? 0.0f : top, less = exp2_fast(before - base);
+    float const base = top == -INFINITY ? 0.0f : top, less = exp2_fast((before - base) * P.scale);
     sum *= less;
 #pragma unroll
     for (int four = 0; four < 4; four++) {
@@ -778,7 +792,7 @@ __global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const
     }
 #pragma unroll
     for (int i = 0; i < kBatch; i++) {
-      float const by = exp2_fast(ref[i] - base);
+      float const by = exp2_fast((ref[i] - base) * P.scale);
       sum += its[i] * by;  // (NaN where every score is NaN that the row sees in the part, which then has no reference)
 #pragma unroll
       for (int four = 0; four < 4; four++) {  // (a part without tiles left no sums)
@@ -810,7 +824,7 @@ __global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const
     x[0] = paged::floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < WAYS; w++) {
-      float const by = exp2_fast(tops[w][c] - base);
+      float const by = exp2_fast((tops[w][c] - base) * P.scale);
       sum += weights[w][c] * by;
       x[0] += shared_sums[w][way][lane] * by;
     }

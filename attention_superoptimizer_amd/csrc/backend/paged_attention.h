@@ -549,12 +549,15 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
         bool const whole = is_there == ~0u && key >= all_least && key + kTile <= all_limit;
         uintx4 p[RG], rest[RG];
         uint32_t seen_by[RG];
+        float x[RG][8], base[RG];
+        // Weights are 2^(scale x + (bias - scale m)) with one rounding of what is in brackets, which all weights of a row have alike; where the product is 2^25 and more it
+        // would take them past the types' ends.  Long before that the difference of scores comes first.
+        bool large = false;
 #pragma unroll
         for (int r = 0; r < RG; r++) {
-          float x[8];
 #pragma unroll
           for (int e = 0; e < 8; e++) {
-            x[e] = s[r][e / 4][e % 4];
+            x[r][e] = s[r][e / 4][e % 4];
           }
           if (!whole) {
             int const upto = limit[r] - key, from = least[r] - key;
@@ -572,10 +575,10 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
             seen_by[r] = seen;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-              x[e] = (seen >> (16 * (e / 4) + 4 * g + e % 4)) & 1 ? x[e] : -INFINITY;
+              x[r][e] = (seen >> (16 * (e / 4) + 4 * g + e % 4)) & 1 ? x[r][e] : -INFINITY;
             }
           }
-          float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+          float top = fmaxf(fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3])), fmaxf(fmaxf(x[r][4], x[r][5]), fmaxf(x[r][6], x[r][7])));
           top = over_groups(top, [](float a, float b) { return fmaxf(a, b); });
           if (__any(top > m[r])) {
             float const higher = fmaxf(m[r], top), less = exp2_fast((m[r] - (higher == -INFINITY ? 0.0f : higher)) * P.scale);
@@ -586,10 +589,25 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
               acc[r][d] *= less;
             }
           }
-          float const base = m[r] == -INFINITY ? 0.0f : bias - m[r] * P.scale;
+          base[r] = m[r] == -INFINITY ? 0.0f : bias - m[r] * P.scale;
+          large = large || __builtin_fabsf(base[r]) > 0x1p20f;
+        }
+        if (__builtin_expect(__any(large), 0)) {
+#pragma unroll
+          for (int r = 0; r < RG; r++) {
+            float const from = m[r] == -INFINITY ? 0.0f : m[r];
+            base[r] = m[r] == -INFINITY ? 0.0f : bias;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              x[r][e] -= from;
+            }
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
 #pragma unroll
           for (int e = 0; e < 8; e += 2) {
-            float const w0 = exp2_fast(__builtin_fmaf(x[e], P.scale, base)), w1 = exp2_fast(__builtin_fmaf(x[e + 1], P.scale, base));
+            float const w0 = exp2_fast(__builtin_fmaf(x[r][e], P.scale, base[r])), w1 = exp2_fast(__builtin_fmaf(x[r][e + 1], P.scale, base[r]));
             sum[r] += w0 + w1;
             uint32_t one_pair, its_rest;
             split(w0, w1, one_pair, its_rest, T());
@@ -717,7 +735,7 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
     for (int r = 0; r < RG; r++) {
       float const whole_sum = over_groups(sum[r], [](float a, float b) { return a + b; });
       if (g == 0) {
-        stat[2 * (wave * 16 * RG + 16 * r + c)] = m[r] * P.scale;
+        stat[2 * (wave * 16 * RG + 16 * r + c)] = m[r];
         stat[2 * (wave * 16 * RG + 16 * r + c) + 1] = whole_sum;
       }
     }
@@ -734,7 +752,7 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
         its[w][1] = stat[2 * (w * 16 * RG + row) + 1];
         top = fmaxf(top, its[w][0]);
       }
-      float const base = top == -INFINITY ? 0.0f : top, less = exp2_fast(m[r] * P.scale - base);
+      float const base = top == -INFINITY ? 0.0f : top, less = exp2_fast((m[r] - base) * P.scale);
 #pragma unroll
       for (int d = 0; d < DB; d++) {
         *reinterpret_cast<floatx4 *>(sums + (wave * 16 * RG + row) * kRow + 16 * d + 4 * g) = acc[r][d] * less;
@@ -743,7 +761,7 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
         float whole_sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; w++) {
-          whole_sum += exp2_fast(its[w][0] - base) * its[w][1];
+          whole_sum += exp2_fast((its[w][0] - base) * P.scale) * its[w][1];
         }
         row_by[row] = of_sum(whole_sum);
         if (!alone) {
@@ -829,7 +847,7 @@ __global__ __launch_bounds__(64 * WAVES, ((WAVES * per_compute_unit<DP, RG, WAVE
 #pragma unroll
                 for (int k = 0; k < kItems; k++) {
                   float const higher = fmaxf(top[k], low_of(ms[k][j])), base = higher == -INFINITY ? 0.0f : higher;
-                  float const less = exp2_fast(top[k] - base), its = exp2_fast(low_of(ms[k][j]) - base);
+                  float const less = exp2_fast((top[k] - base) * P.scale), its = exp2_fast((low_of(ms[k][j]) - base) * P.scale);
                   top[k] = higher;
                   all_sum[k] = all_sum[k] * less + high_of(ms[k][j]) * its;
                   x[k] = x[k] * less + its * floatx4{low_of(a[k][j]), high_of(a[k][j]), low_of(b[k][j]), high_of(b[k][j])};
