@@ -65,7 +65,7 @@ int fill(BlockParams &P, char const *name, void const *q, long long q_stride, vo
   P.group_magic = paged::magic_of(P.group);
   P.q_keep = scale == 0.0f ? 0 : ~0u;
   P.q_flip = scale < 0.0f ? 0x80008000u : 0;
-  P.scale = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504088896341f;
+  P.scale = scale == 0.0f ? 1.0f : fminf(fabsf(scale) * 1.44269504088896341f, FLT_MAX);  // (a score of zero stays zero)
   return MI355_OK;
 }
 

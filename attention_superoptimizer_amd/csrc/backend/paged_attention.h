@@ -20,6 +20,7 @@
 #include "mi355_kernels/kernarg.h"
 #include "mi355_kernels/paged_units.h"
 
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <type_traits>

@@ -89,7 +89,7 @@ extern "C" int mi355_paged_attention(void const *q, long long q_stride, void *ou
   P.group_magic = magic_of(P.group);
   P.q_keep = scale == 0.0f ? 0 : ~0u;
   P.q_flip = scale < 0.0f ? 0x80008000u : 0;
-  P.scale = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504088896341f;
+  P.scale = scale == 0.0f ? 1.0f : fminf(fabsf(scale) * 1.44269504088896341f, FLT_MAX);  // (a score of zero stays zero)
   // Loads that are not to be kept in the caches, from three quarters of the 256 MB on that the last-level cache holds: measured
   // (us, kept and not) 106 and 95 of 539 MB in 64 sequences, 49.5 and 45.8 of 201 MB in 24, 53.6 and 47.6 of 255 MB in 9; against it
   // 31.6 and 32.4 of 150 MB in 16, 28.2 and 29.3 of 136 MB in 14.

@@ -51,3 +51,25 @@ def test_equal_keys(rt, form, new, length, head, kind, size):
         want, bound = _mean(values[0][1][:length - (new - 1 - t)], 2, kind)
         check(got[t], want, bound, t)
 
+
+@pytest.mark.parametrize("form,new", [("window", 1), ("window", 5), ("window", 40), ("tree", 2), ("tree", 40), ("paged", 1), ("paged", 40)])
+@pytest.mark.parametrize("largest", [1.0, -1.0])
+def test_the_largest_scale(rt, form, new, largest):
+    """Scores are zero, or pass 32 bits: those below zero are minus infinity."""
+    k, v, table, values = caches(3, [200], 1, 64, 16, "fp16")
+    q = np.zeros((new, 1, 64))
+    q[-1] = -largest
+    k[np.isfinite(k)] = 1.0
+    k[table[0, 2], 5] = 0.0
+    n, scale = np.array([200], np.int32), largest * float(np.finfo(np.float32).max)
+    if form == "tree":
+        got = run_tree(q, k, v, table, n, np.arange(new, dtype=np.int32)[None] - 1, "fp16", scale)
+    elif form == "paged":
+        got = _paged(q, k, v, table, n, "fp16", scale)
+    else:
+        got = run_window(q, k, v, table, n, "fp16", 0, 0, scale)
+    for t in range(new - 1):
+        want, bound = _mean(values[0][1][:200 - (new - 1 - t)], 1, "fp16")
+        check(got[t], want, bound, t)
+    want, bound = _mean(values[0][1][37:38], 1, "fp16")
+    check(got[-1], want, bound)
