@@ -280,14 +280,19 @@ __device__ void row_again(BlockParams const &P, Block const &b, int kv, Row r, s
       return -INFINITY;
     }
     for (int d = 0; d < P.head_dim; d += 8) {
-      x8 const k = *reinterpret_cast<x8 const *>(k_base + 16ull * (at + d / 8)), a = *reinterpret_cast<x8 const *>(q + d);
+      x8 const k = *reinterpret_cast<x8 const *>(k_base + 16ull * (at + d / 8));
+      uintx4 bits = *reinterpret_cast<uintx4 const *>(q + d);
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        bits[w] = (bits[w] & P.q_keep) ^ P.q_flip;
+      }
+      x8 const a = __builtin_bit_cast(x8, bits);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         x += static_cast<float>(a[e]) * static_cast<float>(k[e]);
       }
     }
-    x = P.q_keep == 0 ? x * 0.0f : x;
-    return P.q_flip != 0 ? -x : x;
+    return x;
   };
   float high = -INFINITY;
   bool wild = false;
