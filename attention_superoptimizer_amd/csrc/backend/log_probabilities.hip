@@ -41,7 +41,7 @@ struct LogParams {
   float *parts;  // of each workgroup of a row: maximum, two sums, then the top logits and their tokens
   int *tickets;  // one a row, kJoinStep apart, zero between launches
   int asked, top, vocabulary, row_parts;
-  float scale;  // times log2 e
+  float scale, natural;  // times log2 e, and as given
 };
 constexpr int kPartWords = 4 + 2 * MI355_MAX_TOP;
 
@@ -440,7 +440,8 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
     bool const empty = own.m == -INFINITY && own.s == 0.0f, wild = !(own.s < INFINITY) || own.m == INFINITY;
     float const log_z = log2f(own.s), nan = __builtin_nanf("");
     auto log_of = [&](float x) {
-      return wild ? nan : (empty || x == -INFINITY ? -INFINITY : kLn2 * ((x - own.m) * P.scale - log_z));
+      // (in natural units from the start: a token masked by the type's lowest value has a log probability that 32 bits hold, and log2 e times it passes them)
+      return wild ? nan : (empty || x == -INFINITY ? -INFINITY : (x - own.m) * P.natural - kLn2 * log_z);
     };
     if (wave == 0) {
       for (int i = lane; i < P.asked; i += 64) {
@@ -602,6 +603,6 @@ extern "C" int mi355_log_probabilities(void const *logits, long long stride, int
   }
   State &s = state();
   LogParams const P{logits, stride, tokens, log_probs, entropy, top_log_probs, top_tokens, static_cast<float *>(s.scratch()), s.queue_join_tickets(),
-                    asked, top, vocabulary, 1, fminf(scale * 1.44269504088896341f, FLT_MAX)};
+                    asked, top, vocabulary, 1, fminf(scale * 1.44269504088896341f, FLT_MAX), scale};
   return type == MI355_TYPE_F16 ? launch_log<_Float16>(P, rows) : type == MI355_TYPE_BF16 ? launch_log<__bf16>(P, rows) : launch_log<float>(P, rows);
 }
