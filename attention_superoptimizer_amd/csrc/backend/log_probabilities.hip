@@ -41,7 +41,9 @@ struct LogParams {
   float *parts;  // of each workgroup of a row: maximum, two sums, then the top logits and their tokens
   int *tickets;  // one a row, kJoinStep apart, zero between launches
   int asked, top, vocabulary, row_parts;
-  float scale, natural;  // times log2 e, and as given
+  // A difference of logits is that of `part` of each, a half where the scale is below 1: two logits may lie farther apart than 32 bits reach.  The scale of such a
+  // difference, times log2 e and as it is.
+  float part, scale, natural;
 };
 constexpr int kPartWords = 4 + 2 * MI355_MAX_TOP;
 
@@ -163,20 +165,22 @@ struct Sums {
 };
 // scale (m - base) for sums that base is to be the maximum of: 0 where there are none yet (nor is there a maximum), and no less than
 // -200, whose power is zero as that of minus infinity is, but not a product with it
-__device__ __forceinline__ float shift(float m, float s, float base, float scale) { return s == 0.0f ? 0.0f : fmaxf((m - base) * scale, -200.0f); }
-__device__ __forceinline__ Sums moved_to(Sums a, float m, float scale) {  // m: not below a's
-  float const z = shift(a.m, a.s, m == -INFINITY ? 0.0f : m, scale), less = __builtin_amdgcn_exp2f(z);
+__device__ __forceinline__ float shift(LogParams const &P, float m, float s, float base) {
+  return s == 0.0f ? 0.0f : fmaxf(__builtin_fmaf(m, P.part, -P.part * base) * P.scale, -200.0f);
+}
+__device__ __forceinline__ Sums moved_to(LogParams const &P, Sums a, float m) {  // m: not below a's
+  float const z = shift(P, a.m, a.s, m == -INFINITY ? 0.0f : m), less = __builtin_amdgcn_exp2f(z);
   return {m, a.s * less, less * (a.t + z * a.s)};
 }
-__device__ __forceinline__ Sums joined(Sums a, Sums b, float scale) {
+__device__ __forceinline__ Sums joined(LogParams const &P, Sums a, Sums b) {
   float const m = fmaxf(a.m, b.m);
-  a = moved_to(a, m, scale);
-  b = moved_to(b, m, scale);
+  a = moved_to(P, a, m);
+  b = moved_to(P, b, m);
   return {m, a.s + b.s, a.t + b.t};
 }
-__device__ __forceinline__ Sums over_lanes(Sums a, float scale) {
+__device__ __forceinline__ Sums over_lanes(LogParams const &P, Sums a) {
   auto add = [](float x, float y) { return x + y; };
-  a = moved_to(a, over_lanes(a.m, [](float x, float y) { return fmaxf(x, y); }), scale);
+  a = moved_to(P, a, over_lanes(a.m, [](float x, float y) { return fmaxf(x, y); }));
   asm("" : "+v"(a.s), "+v"(a.t));  // (a product fused with the first addition would be rounded in one lane of each two only, and the lanes disagree)
   return {a.m, over_lanes(a.s, add), over_lanes(a.t, add)};
 }
@@ -289,13 +293,13 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
         }
         top = fmaxf(top, maxima[j]);
       }
-      own = moved_to(own, top, P.scale);
-      float const base = own.m == -INFINITY ? 0.0f : own.m;
+      own = moved_to(P, own, top);
+      float const base = own.m == -INFINITY ? 0.0f : -P.part * own.m;
       float s = 0.0f, t = 0.0f;
 #pragma unroll
       for (int i = 0; i < kRounds * V; i++) {
         // (the difference first: the product of a large maximum would be off by more than the lanes' maxima differ)
-        float const z = (x[i] - base) * P.scale, w = __builtin_amdgcn_exp2f(z);
+        float const z = __builtin_fmaf(x[i], P.part, base) * P.scale, w = __builtin_amdgcn_exp2f(z);
         s += w;
         t = __builtin_fmaf(fmaxf(z, -200.0f), w, t);  // (2^-200 is zero: a z of minus infinity would make it NaN)
       }
@@ -340,7 +344,7 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
   }
 
   // The wavefronts' sums together, and their entries that no bound rules out.
-  own = over_lanes(own, P.scale);
+  own = over_lanes(P, own);
   if (lane == 0) {
     sums[wave] = own;
     bounds[wave] = bound;
@@ -415,7 +419,7 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
     }
   };
   __syncthreads();
-  own = joined(joined(sums[0], sums[1], P.scale), joined(sums[2], sums[3], P.scale), P.scale);
+  own = joined(P, joined(P, sums[0], sums[1]), joined(P, sums[2], sums[3]));
   if constexpr (TOP) {
     static_assert(kWaves == 4, "sums and bounds");
     bound = fmaxf(fmaxf(bounds[0], bounds[1]), fmaxf(bounds[2], bounds[3]));
@@ -441,7 +445,7 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
     float const log_z = log2f(own.s), nan = __builtin_nanf("");
     auto log_of = [&](float x) {
       // (in natural units from the start: a token masked by the type's lowest value has a log probability that 32 bits hold, and log2 e times it passes them)
-      return wild ? nan : (empty || x == -INFINITY ? -INFINITY : (x - own.m) * P.natural - kLn2 * log_z);
+      return wild ? nan : (empty || x == -INFINITY ? -INFINITY : __builtin_fmaf(x, P.part, -P.part * own.m) * P.natural - kLn2 * log_z);
     };
     if (wave == 0) {
       for (int i = lane; i < P.asked; i += 64) {
@@ -516,7 +520,7 @@ __global__ __launch_bounds__(kThreads) void log_probabilities_kernel(LogParams c
     ask(0, its);
   }
   own = lane < P.row_parts ? Sums{low_of(m_s), low_of(m_s >> 32), low_of(t)} : Sums{-INFINITY, 0.0f, 0.0f};
-  own = over_lanes(own, P.scale);
+  own = over_lanes(P, own);
   if constexpr (TOP) {
     // what every list's last one reaches, and what its share of them does
     auto reached = [](uint64_t entry) { return entry != 0 ? logit_of(entry) : -INFINITY; };
@@ -602,7 +606,8 @@ extern "C" int mi355_log_probabilities(void const *logits, long long stride, int
     return fail(MI355_ERR_INVALID, "mi355_log_probabilities: logits begin between two elements");
   }
   State &s = state();
+  float const part = scale < 1.0f ? 0.5f : 1.0f, natural = scale / part;
   LogParams const P{logits, stride, tokens, log_probs, entropy, top_log_probs, top_tokens, static_cast<float *>(s.scratch()), s.queue_join_tickets(),
-                    asked, top, vocabulary, 1, fminf(scale * 1.44269504088896341f, FLT_MAX), scale};
+                    asked, top, vocabulary, 1, part, fminf(natural * 1.44269504088896341f, FLT_MAX), natural};
   return type == MI355_TYPE_F16 ? launch_log<_Float16>(P, rows) : type == MI355_TYPE_BF16 ? launch_log<__bf16>(P, rows) : launch_log<float>(P, rows);
 }

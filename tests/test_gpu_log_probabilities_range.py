@@ -1,4 +1,4 @@
-"""log_probabilities of logits far apart: tokens masked by the type's lowest value."""
+"""log_probabilities of logits far apart: tokens masked by the type's lowest value, and scales that bring the largest and smallest logits close."""
 import numpy as np
 import pytest
 
@@ -28,3 +28,13 @@ def test_tokens_masked_by_the_lowest_value(rt, kind, scale, rows):
     logits = np.full((rows, 3001), LOWEST[kind])
     logits[:, [4, 1000, 3000]] = normal(rng, (rows, 3), kind)
     _check(logits, np.tile(np.array([7, 1000, 4, 2999], np.int32), (rows, 1)), 6, kind, scale)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("scale", [1e-38, 3e-38, 0.1])
+@pytest.mark.parametrize("rows", [2, 600])
+def test_logits_whose_difference_passes_32_bits(rt, kind, scale, rows):
+    rng = np.random.default_rng(rows)
+    logits = rounded(rng.uniform(-3.3e38, 3.3e38, (rows, 2500)), kind)
+    logits[:, 0], logits[:, 2400] = rounded(3.35e38, kind), LOWEST[kind]
+    _check(logits, np.tile(np.array([0, 2400, 11], np.int32), (rows, 1)), 5, kind, scale)
