@@ -105,12 +105,11 @@ int launch_few(BlockParams const &B, int type, bool tree) {
   P.scale = B.scale;
   P.sinks = B.sinks;
   long long const keys = (long long)B.table_width * B.page_size, rows = (long long)B.new_tokens * B.group;
-  long long const seen = B.window != 0 ? (long long)B.window + B.new_tokens - 1 + B.sinks : keys;
-  P.most_keys = (int)(seen < keys ? seen : keys);
+  P.most_keys = (int)paged::keys_seen(keys, B.window, B.sinks, B.new_tokens);
   // loads that pass the caches: as in mi355_paged_attention
   long long const visible = (long long)B.sequences * P.most_keys, all = (long long)B.pages * B.page_size;
   bool const passing = 4 * (visible < all ? visible : all) * B.kv_heads * B.head_dim > 192LL << 20;
-  long long const slice = paged::sequences_at_once(B.kv_heads, rows, keys);
+  long long const slice = paged::masked_at_once(B.kv_heads, rows, P.most_keys);
   return in_slices(B.sequences, slice, [&](long long at, long long count) -> int {
     P.sequences = (int)count;
     P.q = static_cast<char const *>(B.q) + 2 * at * B.new_tokens * B.q_stride;

@@ -31,5 +31,13 @@ inline long long sequences_at_once(long long kv_heads, long long rows, long long
   return fit < 1 ? 1 : fit;
 }
 
+// With a window, and the first `sinks` tokens: the keys that new_tokens rows in a row see together, at most, and the sequences of a launch.  Which kernel has the call
+// goes by these keys and not by the table's, and so does the size of its units.
+inline long long keys_seen(long long keys, long long window, long long sinks, long long new_tokens) {
+  long long const seen = window != 0 ? window + new_tokens - 1 + sinks : keys;
+  return seen < keys ? seen : keys;
+}
+inline long long masked_at_once(long long kv_heads, long long rows, long long seen) { return sequences_at_once(kv_heads, rows, seen); }
+
 }  // namespace paged
 }  // namespace mi355
