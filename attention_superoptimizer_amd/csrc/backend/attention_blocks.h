@@ -122,7 +122,7 @@ constexpr int kStepsOf = DP != 96 ? 2048 : (TREE ? 512 : 1024);  // keys of a ru
 template <int DP>
 constexpr int tile_bytes() { return kKeys<DP> * DP * 2; }
 template <int DP, bool TREE>
-constexpr int lds_bytes() { return 4 * tile_bytes<DP>() + 4 * kStepsOf<DP, TREE> + kStepsOf<DP, TREE> / 8 + (TREE ? 2 * MI355_MAX_TREE_NODES : 0); }
+constexpr int lds_bytes() { return 4 * tile_bytes<DP>() + 4 * kStepsOf<DP, TREE> + kStepsOf<DP, TREE> / 8 + 32 + (TREE ? 2 * MI355_MAX_TREE_NODES : 0); }
 // Workgroups that a compute unit holds, its registers and LDS (of trees with heads up to 64: three, 45 us, where two are asked for, 50; 4 x 4 heads x up to
 // 16384 keys, 512 rows).  Heads of 256: one, of tiles of 64 keys (one prompt of 8192 tokens, 32 heads, a window
 // of 1024: 440 us; two of tiles of 32, with registers spilled, 459).
@@ -193,8 +193,8 @@ __device__ __forceinline__ Block block_of(BlockParams const &P, int block) {
 }
 
 // the parents of its nodes, -2 in the place of any that is none
-__device__ __forceinline__ void fetch_tree(BlockParams const &P, Block const &b, short *tree, int first, int step) {
-  for (int i = first; i < b.new_tokens; i += step) {
+__device__ __forceinline__ void fetch_tree(BlockParams const &P, Block const &b, short *tree) {
+  for (int i = threadIdx.x; i < b.new_tokens; i += kThreads) {
     int const p = P.parents[(long long)b.sequence * b.new_tokens + i];
     tree[i] = (short)(p >= -1 && p < i ? p : -2);
   }
@@ -236,6 +236,10 @@ __device__ __forceinline__ Row row_of(BlockParams const &P, Block const &b, int 
     }
     r.limit = at == -1 ? (r.limit < 0 ? 0 : r.limit) : -1;
   }
+  if (in_block >= b.rows) {  // no tile is masked for rows that are not there (131 -> 127 us of ragged chunks)
+    r.limit = INT_MAX;
+    r.least = 0;
+  }
   return r;
 }
 // weights are at most 2^(bias + kSlack)
@@ -248,105 +252,6 @@ __device__ __forceinline__ float bias_of(int keys) {
   return std::is_same<T, _Float16>::value ? 9.0f : (float)(__builtin_clz((unsigned)keys | 1u) - 33) - kSlack;
 }
 
-// A weight of zero does not keep an infinity or NaN among the values out of a sum: rows with one in their result are done again, a
-// wavefront a row, key by key, columns d0 up to d1 (but for those whose sum of weights is none: a key that they see makes them so).  (In the loop over tiles such values would have to be looked for in every tile that
-// not all rows see.)  `r` is the same in every lane.
-template <class T, int DP, bool TREE>
-__device__ void row_again(BlockParams const &P, Block const &b, int kv, Row r, short const *tree, int d0, int d1) {
-  typedef typename Vec<T>::x8 x8;
-  int const lane = threadIdx.x % 64;
-  T const *const q = static_cast<T const *>(P.q) + (long long)(b.row_of_q + r.token) * P.q_stride + (long long)(kv * P.group + r.row - r.token * P.group) * P.head_dim;
-  T *const out = static_cast<T *>(P.out) + (long long)(b.row_of_q + r.token) * P.out_stride + (long long)(kv * P.group + r.row - r.token * P.group) * P.head_dim;
-  int const *const table = P.table + (long long)b.sequence * P.table_width;
-  uint64_t const k_base = reinterpret_cast<uint64_t>(P.k) + 16ull * kv * P.head_step, v_base = reinterpret_cast<uint64_t>(P.v) + 16ull * kv * P.head_step;
-  int const context = b.length - b.new_tokens;
-  // the key of this lane of 64: where it lies, or all ones where the row does not see it
-  auto find = [&](int key) {
-    int const real = key < b.kept ? key : key + b.shift, page = quotient(real, P.page_size, P.page_magic);
-    bool sees = key < b.end && ((key < r.limit && key >= r.least) || (!TREE && key < r.always));
-    if constexpr (TREE) {
-      if (r.limit >= 0) {
-        for (int node = r.token; node >= 0; node = tree[node]) {
-          sees = sees || key == context + node;
-        }
-      }
-    }
-    int const number = sees ? table[page] : -1;
-    return (unsigned)number < (unsigned)P.pages ? (uint32_t)number * P.page_step + (uint32_t)(real - page * P.page_size) * P.token_step : ~0u;
-  };
-  auto score = [&](uint32_t at) {
-    float x = 0.0f;
-    if (at == ~0u) {
-      return -INFINITY;
-    }
-    for (int d = 0; d < P.head_dim; d += 8) {
-      x8 const k = *reinterpret_cast<x8 const *>(k_base + 16ull * (at + d / 8));
-      uintx4 bits = *reinterpret_cast<uintx4 const *>(q + d);
-#pragma unroll
-      for (int w = 0; w < 4; w++) {
-        bits[w] = (bits[w] & P.q_keep) ^ P.q_flip;
-      }
-      x8 const a = __builtin_bit_cast(x8, bits);
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        x += static_cast<float>(a[e]) * static_cast<float>(k[e]);
-      }
-    }
-    return x;
-  };
-  float high = -INFINITY;
-  bool wild = false;
-  for (int key = 0; key < b.end; key += 64) {
-    float const x = score(find(key + lane));
-    wild = wild || x != x;
-    high = fmaxf(high, x);
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    high = fmaxf(high, __shfl_xor(high, off, 64));
-  }
-  wild = __any(wild) || high == INFINITY;
-  constexpr int N = (DP + 63) / 64;
-  float total = 0.0f, o[N];
-#pragma unroll
-  for (int i = 0; i < N; i++) {
-    o[i] = 0.0f;
-  }
-  float const base = high == -INFINITY ? 0.0f : high, bias = bias_of<T>(b.end);
-  for (int key = 0; key < b.end && !wild; key += 64) {
-    uint32_t const at = find(key + lane);
-    float const w = at == ~0u ? 0.0f : exp2_fast((score(at) - base) * P.scale + bias);
-    total += w;
-    for (uint64_t left = __ballot(at != ~0u); left != 0; left &= left - 1) {
-      int const j = __builtin_ctzll(left);
-      float const its = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), j));
-      T const *const v = reinterpret_cast<T const *>(v_base + 16ull * (uint32_t)__builtin_amdgcn_readlane((int)at, j));
-#pragma unroll
-      for (int i = 0; i < N; i++) {
-        int const d = d0 + 64 * i + lane;
-        if (d < d1) {
-          float const x = static_cast<float>(v[d]);
-          o[i] += __builtin_fabsf(x) == INFINITY && high != -INFINITY ? x : its * x;
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    total += __shfl_xor(total, off, 64);
-  }
-#pragma unroll
-  for (int i = 0; i < N; i++) {
-    int const d = d0 + 64 * i + lane;
-    if (d < d1) {
-      out[d] = static_cast<T>(wild ? __builtin_nanf("") : (total == 0.0f ? 0.0f : o[i] * (1.0f / total)));
-    }
-  }
-}
-__device__ __forceinline__ Row of_lane(Row r, int lane) {
-  return {__builtin_amdgcn_readlane(r.row, lane), __builtin_amdgcn_readlane(r.token, lane), __builtin_amdgcn_readlane(r.limit, lane),
-          __builtin_amdgcn_readlane(r.least, lane), __builtin_amdgcn_readlane(r.always, lane)};
-}
 // How the blocks of a batch of trees are cut along their keys: a tree's all into as many parts as leave each at most `run` tiles, with the
 // least run for which the parts of all are no more than the workgroups that the chip holds together (P.slots, and the launch's).
 struct Cut {
@@ -398,6 +303,64 @@ __device__ __forceinline__ int parts_of(BlockParams const &P, Block const &b) {
 template <int DP>
 constexpr int part_floats() { return kRows * (DP + 2); }
 
+// What sums are scaled by at least where there may be infinities among them: as good as zero, but zero times an infinity is NaN.
+constexpr float kNone = 0x1p-126f;
+// Adds the values of a tile that are infinite or NaN to the rows that see their keys (of both halves' lanes, a bit each), whatever the weights, and leaves
+// zeros in their places.  All wavefronts do; `keys` are two words of LDS.
+template <class T, int DP>
+__device__ __forceinline__ void add_wild(unsigned char *v_tile, uint32_t *keys, uint64_t seen, floatx16 (&acc)[DP / 32]) {
+  constexpr int C = DP / 8, LOADS = kKeys<DP> * C / kThreads;
+  constexpr uint32_t top = Vec<T>::exponent;
+  typedef typename Vec<T>::x4 x4;
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // (what is made of it here is not to be kept through the loop over tiles)
+  int const h = tid % 64 / 32;
+  auto is_wild = [](uint32_t x) { return (x & top) == top || (x & top << 16) == top << 16; };
+  if (tid < 2) {
+    keys[tid] = 0;
+  }
+  __syncthreads();
+  for (int i = 0; i < LOADS; i++) {
+    int const n = kThreads * i + tid, its = n / C;
+    uintx4 const x = *reinterpret_cast<uintx4 const *>(v_tile + 16 * n);
+    if (is_wild(x[0]) || is_wild(x[1]) || is_wild(x[2]) || is_wild(x[3])) {
+      __hip_atomic_fetch_or(keys + its / 32, 1u << its % 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
+  }
+  __syncthreads();
+  uint64_t const all = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)keys[1]) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)keys[0]);
+  if (all == 0) {
+    return;
+  }
+  for (uint64_t left = all; left != 0; left &= left - 1) {
+    int const j = __builtin_ctzll(left);
+    bool const sees = (seen >> j & 1) != 0;
+#pragma unroll
+    for (int d = 0; d < DP / 32; d++) {
+#pragma unroll
+      for (int four = 0; four < 4; four++) {
+        x4 const x = *reinterpret_cast<x4 const *>(v_tile + j * (2 * DP) + 16 * place_of<C>(j, 4 * d + four) + 8 * h);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          float const value = static_cast<float>(x[e]);
+          acc[d][4 * four + e] += sees && !(__builtin_fabsf(value) < INFINITY) ? value : 0.0f;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = 0; i < LOADS; i++) {
+    uintx4 *const place = reinterpret_cast<uintx4 *>(v_tile + 16 * (kThreads * i + tid));
+    uintx4 x = *place;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      x[w] &= ((x[w] & top) == top ? 0u : 0xffffu) | ((x[w] & top << 16) == top << 16 ? 0u : 0xffff0000u);
+    }
+    *place = x;
+  }
+  __syncthreads();
+}
+
 template <class T, int DP, bool TREE>
 __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kernel(BlockParams const P) {
   fetch_kernel_arguments<sizeof(BlockParams), 0>();  // (gridDim is not read: no word behind them is the launch's)
@@ -407,7 +370,8 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   uint64_t *const exist = reinterpret_cast<uint64_t *>(lds + 4 * tile_bytes<DP>());
   uint32_t *const steps = reinterpret_cast<uint32_t *>(exist + kSteps / 64);
-  short *const tree = reinterpret_cast<short *>(steps + kSteps);
+  uint32_t *const wild = steps + kSteps;  // for each wavefront whether its rows have sums that are not finite; keys of a tile with such values, a bit each
+  short *const tree = reinterpret_cast<short *>(wild + 8);
   int const tid = threadIdx.x, lane = tid % 64, wave = tid / 64, h = lane / 32, c = lane % 32;
   uint32_t const lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void const *)lds;
 
@@ -438,7 +402,7 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
     return;
   }
   if constexpr (TREE) {
-    fetch_tree(P, b, tree, tid, kThreads);
+    fetch_tree(P, b, tree);
     __syncthreads();
   }
   int const context = b.length - b.new_tokens, kept = b.kept, shift = b.shift;
@@ -472,15 +436,7 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
   }
 
   floatx16 acc[DB];
-  float ref = -INFINITY, base = 0.0f, sum = 0.0f;
-  bool large = false;  // some row's reference, times the scale
-#pragma unroll
-  for (int d = 0; d < DB; d++) {
-#pragma unroll
-    for (int e = 0; e < 16; e++) {
-      acc[d][e] = 0.0f;
-    }
-  }
+  float ref, base, sum;
   // The reference follows the maximum only where weights would pass 2^(bias + kSlack), so that sums are seldom scaled.  fp16: small ones stay
   // above the type's end.  bf16: as values reach the end of 32 bits themselves, n weights add up to less than 1/2.
   float const bias = bias_of<T>(b.end);
@@ -500,193 +456,240 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
     real[i] = chunk <= last;
   }
 
-  for (int part = begin; part < end; part += kSteps) {
-    int const part_end = end - part < kSteps ? end : part + kSteps;
-    // Where the part's keys lie, in 16 bytes, and which of them exist, a bit each.  In the place of a key that does not any of the 64 that do: it is
-    // masked, and what lies elsewhere may be no number.
-    __syncthreads();
-    for (int i = tid; i < (part_end - part + 63) / 64 * 64; i += kThreads) {
-      int const key = part + i, real = key < kept ? key : key + shift, page = quotient(real, P.page_size, P.page_magic);
-      int const number = key < part_end ? table[page] : -1;
-      bool const is = (unsigned)number < (unsigned)P.pages;
-      uint64_t const there = __ballot(is);
-      uint32_t const step = (uint32_t)number * P.page_step + (uint32_t)(real - page * P.page_size) * P.token_step;
-      uint32_t const some = there != 0 ? (uint32_t)__builtin_amdgcn_readlane((int)step, __builtin_ctzll(there)) : 0;
-      steps[i] = is ? step : some;
-      if (lane == 0) {
-        exist[i / 64] = there;
+  // A weight of zero does not keep an infinity or NaN among the values out of a sum, and looking for them in every tile that not all rows see would take too long:
+  // where a sum comes out as none of the finite numbers the workgroup starts again with care, and each tile's are added to the rows that see them by
+  // themselves, and zero from then on.  (One infinite value that all rows see: 57.8 us of a prompt of 1024 tokens, 36 without, 1284 of one of 8192, 567; 8 x 4 heads
+  // of 128.)
+  for (bool careful = false;; careful = true) {
+    bool large = false;  // some row's reference, times the scale
+    ref = -INFINITY;
+    base = sum = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DB; d++) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        acc[d][e] = 0.0f;
       }
     }
-    __syncthreads();
+    for (int part = begin; part < end; part += kSteps) {
+      int const part_end = end - part < kSteps ? end : part + kSteps;
+      // Where the part's keys lie, in 16 bytes, and which of them exist, a bit each.  In the place of a key that does not any of the 64 that do: it is
+      // masked, and what lies elsewhere may be no number.
+      __syncthreads();
+      for (int i = tid; i < (part_end - part + 63) / 64 * 64; i += kThreads) {
+        int const key = part + i, real = key < kept ? key : key + shift, page = quotient(real, P.page_size, P.page_magic);
+        int const number = key < part_end ? table[page] : -1;
+        bool const is = (unsigned)number < (unsigned)P.pages;
+        uint64_t const there = __ballot(is);
+        uint32_t const step = (uint32_t)number * P.page_step + (uint32_t)(real - page * P.page_size) * P.token_step;
+        uint32_t const some = there != 0 ? (uint32_t)__builtin_amdgcn_readlane((int)step, __builtin_ctzll(there)) : 0;
+        steps[i] = is ? step : some;
+        if (lane == 0) {
+          exist[i / 64] = there;
+        }
+      }
+      __syncthreads();
 
-    // the rows that this thread loads chunks of, looked up a tile before their loads
-    uint32_t from[LOADS];
-    uint64_t there;
-    auto locate = [&](int at) {
-      int const in_part = at < part_end ? at - part : 0;
+      // the rows that this thread loads chunks of, looked up a tile before their loads
+      uint32_t from[LOADS];
+      uint64_t there;
+      auto locate = [&](int at) {
+        int const in_part = at < part_end ? at - part : 0;
 #pragma unroll
-      for (int i = 0; i < LOADS; i++) {
-        from[i] = steps[in_part + (kThreads * i + tid) / C] + chunk_of[i];
-      }
-      there = exist[in_part / 64];
-    };
-    auto load = [&](int buffer) {
-      uint32_t const base = lds_at + buffer * 2 * tile_bytes<DP>() + 1024 * wave;
-#pragma unroll
-      for (int i = 0; i < LOADS; i++) {
-        uint64_t const key = k_base + 16ull * from[i];
-        paged::load_to_lds<false>(!padded || real[i] ? key : reinterpret_cast<uint64_t>(&paged::kZeros), base + 16 * kThreads * i);
-      }
-#pragma unroll
-      for (int i = 0; i < LOADS; i++) {
-        paged::load_to_lds<false>(v_base + 16ull * from[i], base + tile_bytes<DP>() + 16 * kThreads * i);
-      }
-    };
-    locate(part);
-    load(0);
-    uint64_t next_there = there;
-    locate(part + KT);
-    if (32 * __builtin_amdgcn_readfirstlane(wave) >= b.rows) {  // a wavefront without rows loads its share of the tiles, no more
-      for (int at = part, buffer = 1; at < part_end; at += KT, buffer ^= 1) {
-        paged::wait_loads<0>();
-        __syncthreads();
-        if (at + KT < part_end) {
-          load(buffer);
+        for (int i = 0; i < LOADS; i++) {
+          from[i] = steps[in_part + (kThreads * i + tid) / C] + chunk_of[i];
         }
-        locate(at + 2 * KT);
-      }
-      continue;
-    }
-    for (int at = part, buffer = 0; at < part_end; at += KT, buffer ^= 1) {
-      uint64_t const is_there = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(next_there >> 32)) << 32 |
-                                (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)next_there);
-      next_there = there;
-      paged::wait_loads<0>();
-      __syncthreads();  // the tile is here, and everyone is done with the one before
-      if (at + KT < part_end) {
-        load(buffer ^ 1);
-      }
-      unsigned char const *const k_tile = lds + buffer * 2 * tile_bytes<DP>(), *const v_tile = k_tile + tile_bytes<DP>();
-
-      floatx16 s[G];
+        there = exist[in_part / 64];
+      };
+      auto load = [&](int buffer) {
+        uint32_t const base = lds_at + buffer * 2 * tile_bytes<DP>() + 1024 * wave;
 #pragma unroll
-      for (int j = 0; j < G; j++) {
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          s[j][e] = 0.0f;
+        for (int i = 0; i < LOADS; i++) {
+          uint64_t const key = k_base + 16ull * from[i];
+          paged::load_to_lds<false>(!padded || real[i] ? key : reinterpret_cast<uint64_t>(&paged::kZeros), base + 16 * kThreads * i);
         }
-      }
 #pragma unroll
-      for (int kk = 0; kk < KK; kk++) {
-#pragma unroll
-        for (int j = 0; j < G; j++) {
-          int const its = 32 * j + c;
-          s[j] = mfma(*reinterpret_cast<x8 const *>(k_tile + its * (2 * DP) + 16 * place_of<C>(its, 2 * kk + h)), q[kk], s[j]);
+        for (int i = 0; i < LOADS; i++) {
+          paged::load_to_lds<false>(v_base + 16ull * from[i], base + tile_bytes<DP>() + 16 * kThreads * i);
         }
-      }
-      locate(at + 2 * KT);
-      // operands of the products some ahead of them
-      __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
-#pragma unroll
-      for (int i = 0; i < KK * G - 8; i++) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-
-      // element e of s[j]: key 32 j + 8 (e / 4) + 4 h + e % 4 of row c
-      int const half = KT == 32 ? (at - part) % 64 : 0;  // of a word of bits
-      bool const all_there = KT == 64 ? is_there == ~0ull : (uint32_t)(is_there >> half) == ~0u;
-      if (!all_there || __any(r.limit < at + KT || r.least > at)) {
-        uint32_t seen[G];
-#pragma unroll
-        for (int j = 0; j < G; j++) {
-          int const first = at + 32 * j;
-          seen[j] = (bits_below(r.limit - first) & ~bits_below(r.least - first)) | (TREE ? 0u : bits_below(r.always - first));
-        }
-        if constexpr (TREE) {
-          int node = r.limit >= 0 ? r.token : -1;
-          while (__any(node >= 0)) {
-            int const place = context + node - at;
-            if (node >= 0) {
-#pragma unroll
-              for (int j = 0; j < G; j++) {
-                seen[j] |= (unsigned)(place - 32 * j) < 32u ? 1u << (place - 32 * j) : 0u;
-              }
-              node = place > 0 ? tree[node] : -1;
-            }
+      };
+      locate(part);
+      load(0);
+      uint64_t next_there = there;
+      locate(part + KT);
+      if (32 * __builtin_amdgcn_readfirstlane(wave) >= b.rows && !careful) {  // a wavefront without rows loads its share of the tiles, no more
+        for (int at = part, buffer = 1; at < part_end; at += KT, buffer ^= 1) {
+          paged::wait_loads<0>();
+          __syncthreads();
+          if (at + KT < part_end) {
+            load(buffer);
           }
+          locate(at + 2 * KT);
         }
+        continue;
+      }
+      for (int at = part, buffer = 0; at < part_end; at += KT, buffer ^= 1) {
+        uint64_t const is_there = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(next_there >> 32)) << 32 |
+                                  (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)next_there);
+        next_there = there;
+        paged::wait_loads<0>();
+        __syncthreads();  // the tile is here, and everyone is done with the one before
+        if (at + KT < part_end) {
+          load(buffer ^ 1);
+        }
+        unsigned char *const k_tile = lds + buffer * 2 * tile_bytes<DP>(), *const v_tile = k_tile + tile_bytes<DP>();
+
+        floatx16 s[G];
 #pragma unroll
         for (int j = 0; j < G; j++) {
-          seen[j] = (seen[j] & (uint32_t)(is_there >> (32 * j + half))) >> (4 * h);
 #pragma unroll
           for (int e = 0; e < 16; e++) {
-            s[j][e] = (seen[j] >> (8 * (e / 4) + e % 4)) & 1 ? s[j][e] : -INFINITY;
+            s[j][e] = 0.0f;
           }
         }
-      }
-
-      float top = s[0][0];
 #pragma unroll
-      for (int j = 0; j < G; j++) {
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          top = fmaxf(top, s[j][e]);
-        }
-      }
-      top = over_halves(top, [](float a, float b) { return fmaxf(a, b); });
-      if (__any((top - ref) * P.scale > kSlack) || large) {
-        float const most = fmaxf(ref, top), from = most == -INFINITY ? 0.0f : most, less = exp2_fast((ref - from) * P.scale);
-        ref = most;
-        sum *= less;
-#pragma unroll
-        for (int d = 0; d < DB; d++) {
-          acc[d] *= less;
-        }
-        large = __any(__builtin_fabsf(from) * P.scale > kLarge);
-        base = most == -INFINITY ? 0.0f : (large ? bias : bias - from * P.scale);
-        if (large) {
+        for (int kk = 0; kk < KK; kk++) {
 #pragma unroll
           for (int j = 0; j < G; j++) {
+            int const its = 32 * j + c;
+            s[j] = mfma(*reinterpret_cast<x8 const *>(k_tile + its * (2 * DP) + 16 * place_of<C>(its, 2 * kk + h)), q[kk], s[j]);
+          }
+        }
+        locate(at + 2 * KT);
+        // operands of the products some ahead of them
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+        for (int i = 0; i < KK * G - 8; i++) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+
+        // element e of s[j]: key 32 j + 8 (e / 4) + 4 h + e % 4 of row c
+        int const half = KT == 32 ? (at - part) % 64 : 0;  // of a word of bits
+        bool const all_there = KT == 64 ? is_there == ~0ull : (uint32_t)(is_there >> half) == ~0u;
+        if (!all_there || __any(r.limit < at + KT || r.least > at) || careful) {
+          uint32_t seen[G];
+#pragma unroll
+          for (int j = 0; j < G; j++) {
+            int const first = at + 32 * j;
+            seen[j] = (bits_below(r.limit - first) & ~bits_below(r.least - first)) | (TREE ? 0u : bits_below(r.always - first));
+          }
+          if constexpr (TREE) {
+            int node = r.limit >= 0 ? r.token : -1;
+            while (__any(node >= 0)) {
+              int const place = context + node - at;
+              if (node >= 0) {
+#pragma unroll
+                for (int j = 0; j < G; j++) {
+                  seen[j] |= (unsigned)(place - 32 * j) < 32u ? 1u << (place - 32 * j) : 0u;
+                }
+                node = place > 0 ? tree[node] : -1;
+              }
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < G; j++) {
+            seen[j] &= (uint32_t)(is_there >> (32 * j + half));
+          }
+          if (__builtin_expect(careful, 0)) {
+            add_wild<T, DP>(v_tile, wild + 4, G == 1 ? seen[0] : (uint64_t)seen[G - 1] << 32 | seen[0], acc);
+          }
+#pragma unroll
+          for (int j = 0; j < G; j++) {
+            seen[j] >>= 4 * h;
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-              s[j][e] -= from;
+              s[j][e] = (seen[j] >> (8 * (e / 4) + e % 4)) & 1 ? s[j][e] : -INFINITY;
             }
           }
         }
-      }
 
-      // Weights of sixteen keys at a time, and their products with the values.  O^T: lane has columns 32 d + 8 (e / 4) + 4 h + e % 4 of row c.
+        float top = s[0][0];
 #pragma unroll
-      for (int k = 0; k < 2 * G; k++) {
-        x8 p;
+        for (int j = 0; j < G; j++) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          p[e] = static_cast<T>(exp2_fast(__builtin_fmaf(s[k / 2][8 * (k % 2) + e], P.scale, base)));
-        }
-        sum = sum_of(p, sum);
-#pragma unroll
-        for (int d = 0; d < DB; d++) {
-          uint64_t v[2];
-#pragma unroll
-          for (int half = 0; half < 2; half++) {
-            int const its = 16 * k + 8 * half + 4 * h + lane % 16 / 4, chunk = 4 * d + 2 * (lane / 16 % 2) + lane % 4 / 2;
-            typedef short shortx4 __attribute__((ext_vector_type(4)));
-            unsigned char const *const at_v = v_tile + its * (2 * DP) + 16 * place_of<C>(its, chunk) + 8 * (lane % 2);
-            v[half] = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                       (shortx4 __attribute__((address_space(3))) *)(__attribute__((address_space(3))) void const *)at_v));
+          for (int e = 0; e < 16; e++) {
+            top = fmaxf(top, s[j][e]);
           }
-          uintx4 const both = {(uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1], (uint32_t)(v[1] >> 32)};
-          acc[d] = mfma(__builtin_bit_cast(x8, both), p, acc[d]);
+        }
+        top = over_halves(top, [](float a, float b) { return fmaxf(a, b); });
+        if (__any((top - ref) * P.scale > kSlack) || large) {
+          float const most = fmaxf(ref, top), from = most == -INFINITY ? 0.0f : most;
+          float less = exp2_fast((ref - from) * P.scale);
+          less = careful ? fmaxf(less, kNone) : less;
+          ref = most;
+          sum *= less;
+#pragma unroll
+          for (int d = 0; d < DB; d++) {
+            acc[d] *= less;
+          }
+          large = __any(__builtin_fabsf(from) * P.scale > kLarge);
+          base = most == -INFINITY ? 0.0f : (large ? bias : bias - from * P.scale);
+          if (__builtin_expect(large, 0)) {
+#pragma unroll
+            for (int j = 0; j < G; j++) {
+#pragma unroll
+              for (int e = 0; e < 16; e++) {
+                s[j][e] -= from;
+              }
+            }
+          }
+        }
+
+        // Weights of sixteen keys at a time, and their products with the values.  O^T: lane has columns 32 d + 8 (e / 4) + 4 h + e % 4 of row c.
+#pragma unroll
+        for (int k = 0; k < 2 * G; k++) {
+          x8 p;
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            p[e] = static_cast<T>(exp2_fast(__builtin_fmaf(s[k / 2][8 * (k % 2) + e], P.scale, base)));
+          }
+          sum = sum_of(p, sum);
+#pragma unroll
+          for (int d = 0; d < DB; d++) {
+            uint64_t v[2];
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+              int const its = 16 * k + 8 * half + 4 * h + lane % 16 / 4, chunk = 4 * d + 2 * (lane / 16 % 2) + lane % 4 / 2;
+              typedef short shortx4 __attribute__((ext_vector_type(4)));
+              unsigned char const *const at_v = v_tile + its * (2 * DP) + 16 * place_of<C>(its, chunk) + 8 * (lane % 2);
+              v[half] = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                         (shortx4 __attribute__((address_space(3))) *)(__attribute__((address_space(3))) void const *)at_v));
+            }
+            uintx4 const both = {(uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1], (uint32_t)(v[1] >> 32)};
+            acc[d] = mfma(__builtin_bit_cast(x8, both), p, acc[d]);
+          }
         }
       }
+    }
+
+    sum = over_halves(sum, [](float a, float b) { return a + b; });
+    if (__builtin_expect(careful, 0)) {
+      break;
+    }
+    // (columns past the head's end are its last ones again; without a sum of weights the row is NaN whatever the values are)
+    paged::floatx4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int d = 0; d < DB; d++) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        none[e % 4] = __builtin_fmaf(acc[d][e], 0.0f, none[e % 4]);
+      }
+    }
+    float const any = (none[0] + none[1]) + (none[2] + none[3]);
+    bool const again = __any(any != any && sum == sum && is_row);
+    if (lane == 0) {
+      wild[wave] = again;
+    }
+    __syncthreads();
+    if (__builtin_expect((wild[0] | wild[1] | wild[2] | wild[3]) == 0, 1)) {
+      break;
     }
   }
 
   if (32 * wave >= b.rows) {
     return;
   }
-  sum = over_halves(sum, [](float a, float b) { return a + b; });
   if (parts > 1) {  // left as it is, for the kernel below
     float *const part = P.parts + (long long)blockIdx.x * part_floats<DP>();
     if (h == 0) {
@@ -705,9 +708,12 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
     }
     return;
   }
-  float const by = sum == 0.0f ? 0.0f : 1.0f / sum;
-  bool good = true;
-  T *const out = static_cast<T *>(P.out) + (long long)(b.row_of_q + r.token) * P.out_stride + (long long)(kv * P.group + r.row - r.token * P.group) * P.head_dim;
+  float const by = 1.0f / sum;
+  int in_block = tid;
+  asm volatile("" : "+v"(in_block));  // (the row's number and token are not to be kept through the loop over tiles)
+  in_block = in_block / 64 * 32 + in_block % 32;
+  int const row = b.row0 + (is_row ? in_block : 0), token = quotient(row, P.group, P.group_magic);
+  T *const out = static_cast<T *>(P.out) + (long long)(b.row_of_q + token) * P.out_stride + (long long)(kv * P.group + row - token * P.group) * P.head_dim;
 #pragma unroll
   for (int d = 0; d < DB; d++) {
 #pragma unroll
@@ -715,22 +721,13 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
       x4 y;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        y[e] = static_cast<T>(acc[d][4 * four + e] * by);
+        y[e] = static_cast<T>(sum == 0.0f ? 0.0f : acc[d][4 * four + e] * by);
       }
       int const at = 32 * d + 8 * four + 4 * h;
       if (is_row && at < P.head_dim) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          good = good && __builtin_fabsf(acc[d][4 * four + e] * by) < INFINITY;  // (false for NaN)
-        }
         *reinterpret_cast<x4 *>(out + at) = y;
       }
     }
-  }
-  uint64_t again = __ballot(!good && sum == sum && is_row);
-  again = (again | again >> 32) & 0xffffffffull;
-  for (; again != 0; again &= again - 1) {
-    row_again<T, DP, TREE>(P, b, kv, of_lane(r, __builtin_ctzll(again)), tree, 0, P.head_dim);
   }
 }
 
@@ -743,7 +740,6 @@ __global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const
   typedef typename Vec<T>::x4 x4;
   __shared__ paged::floatx4 shared_sums[WAYS][4][64];
   __shared__ float tops[WAYS][32], weights[WAYS][32];
-  __shared__ short tree[TREE ? MI355_MAX_TREE_NODES : 1];
   int const tid = threadIdx.x, lane = tid % 64, wave = tid / 64, way = wave % WAYS, h = lane / 32, c = lane % 32;
   int const d = (int)blockIdx.x % DB, rows = (int)blockIdx.x / DB % WAYS * kFours + wave / WAYS;
   int const kv = (int)blockIdx.x / (WAYS * DB) % P.kv_heads, block = (int)blockIdx.x / (WAYS * DB) / P.kv_heads;
@@ -793,18 +789,18 @@ __global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const
     sum *= less;
 #pragma unroll
     for (int four = 0; four < 4; four++) {
-      x[four] *= less;
+      x[four] *= fmaxf(less, kNone);
     }
 #pragma unroll
     for (int i = 0; i < kBatch; i++) {
       float const by = exp2_fast((ref[i] - base) * P.scale);
       sum += its[i] * by;  // (NaN where every score is NaN that the row sees in the part, which then has no reference)
 #pragma unroll
-      for (int four = 0; four < 4; four++) {  // (a part without tiles left no sums)
-        paged::floatx4 const z = by * y[i][four];
+      for (int four = 0; four < 4; four++) {
+        paged::floatx4 const z = fmaxf(by, kNone) * y[i][four];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          x[four][e] += ref[i] > -INFINITY ? z[e] : 0.0f;
+          x[four][e] += i0 + i * WAYS < parts ? z[e] : 0.0f;
         }
       }
     }
@@ -831,13 +827,12 @@ __global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const
     for (int w = 0; w < WAYS; w++) {
       float const by = exp2_fast((tops[w][c] - base) * P.scale);
       sum += weights[w][c] * by;
-      x[0] += shared_sums[w][way][lane] * by;
+      x[0] += shared_sums[w][way][lane] * fmaxf(by, kNone);
     }
   }
-  float const by = sum == 0.0f ? 0.0f : 1.0f / sum;
+  float const by = 1.0f / sum;
   int const row = b.row0 + (is_row ? in_block : 0), token = quotient(row, P.group, P.group_magic), d0 = 32 * d + 8 * way;
   T *const out = static_cast<T *>(P.out) + (long long)(b.row_of_q + token) * P.out_stride + (long long)(kv * P.group + row - token * P.group) * P.head_dim;
-  bool good = true;
 #pragma unroll
   for (int four = 0; four < kFours; four++) {
     int const at = d0 + 8 * four + 4 * h;
@@ -845,23 +840,9 @@ __global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const
       x4 y;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        y[e] = static_cast<T>(x[four][e] * by);
-        good = good && __builtin_fabsf(x[four][e] * by) < INFINITY;
+        y[e] = static_cast<T>(sum == 0.0f ? 0.0f : x[four][e] * by);
       }
       *reinterpret_cast<x4 *>(out + at) = y;
-    }
-  }
-  uint64_t again = __ballot(!good && sum == sum);
-  if (again != 0) {
-    if constexpr (TREE) {  // (every wavefront for itself: they write the same)
-      fetch_tree(P, b, tree, lane, 64);
-      paged::wait_lds_reads();
-    }
-    Row const r = row_of<TREE>(P, b, in_block, tree);
-    int const d1 = d0 + 8 * kFours < P.head_dim ? d0 + 8 * kFours : P.head_dim;
-    again = (again | again >> 32) & 0xffffffffull;
-    for (; again != 0; again &= again - 1) {
-      row_again<T, 32, TREE>(P, b, kv, of_lane(r, __builtin_ctzll(again)), tree, d0, d1);
     }
   }
 }
