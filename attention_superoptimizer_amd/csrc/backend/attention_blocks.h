@@ -458,8 +458,8 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
 
   // A weight of zero does not keep an infinity or NaN among the values out of a sum, and looking for them in every tile that not all rows see would take too long:
   // where a sum comes out as none of the finite numbers the workgroup starts again with care, and each tile's are added to the rows that see them by
-  // themselves, and zero from then on.  (One infinite value that all rows see: 57.8 us of a prompt of 1024 tokens, 36 without, 1284 of one of 8192, 567; 8 x 4 heads
-  // of 128.)
+  // themselves, and zero from then on.  (One infinite value that all rows see: 57.8 us of a prompt of 1024 tokens, 36 without, 1284 of one of 8192, 567; 8 x 4
+  // heads of 128.)
   for (bool careful = false;; careful = true) {
     bool large = false;  // some row's reference, times the scale
     ref = -INFINITY;
@@ -664,6 +664,24 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
     }
 
     sum = over_halves(sum, [](float a, float b) { return a + b; });
+    if (parts > 1 && 32 * wave < b.rows) {  // left as it is, for the kernel below
+      int mine = tid;
+      asm volatile("" : "+v"(mine));  // (places are not to be kept through the loop over tiles)
+      int const wave = mine / 64, lane = mine % 64;
+      float *const part = P.parts + (long long)blockIdx.x * part_floats<DP>();
+      if (lane < 32) {
+        part[kRows * DP + 2 * (32 * wave + lane)] = ref;
+        part[kRows * DP + 2 * (32 * wave + lane) + 1] = sum;
+      }
+#pragma unroll
+      for (int d = 0; d < DB; d++) {
+#pragma unroll
+        for (int four = 0; four < 4; four++) {
+          *reinterpret_cast<paged::floatx4 *>(part + 4 * (((d * kWaves + wave) * 4 + four) * 64 + lane)) =
+              paged::floatx4{acc[d][4 * four], acc[d][4 * four + 1], acc[d][4 * four + 2], acc[d][4 * four + 3]};
+        }
+      }
+    }
     if (__builtin_expect(careful, 0)) {
       break;
     }
@@ -687,25 +705,7 @@ __global__ __launch_bounds__(kThreads, kPerUnit<DP>) void attention_blocks_kerne
     }
   }
 
-  if (32 * wave >= b.rows) {
-    return;
-  }
-  if (parts > 1) {  // left as it is, for the kernel below
-    float *const part = P.parts + (long long)blockIdx.x * part_floats<DP>();
-    if (h == 0) {
-      part[kRows * DP + 2 * (32 * wave + c)] = ref;
-      part[kRows * DP + 2 * (32 * wave + c) + 1] = sum;
-    }
-    if (begin < end) {
-#pragma unroll
-      for (int d = 0; d < DB; d++) {
-#pragma unroll
-        for (int four = 0; four < 4; four++) {
-          *reinterpret_cast<paged::floatx4 *>(part + 4 * (((d * kWaves + wave) * 4 + four) * 64 + lane)) =
-              paged::floatx4{acc[d][4 * four], acc[d][4 * four + 1], acc[d][4 * four + 2], acc[d][4 * four + 3]};
-        }
-      }
-    }
+  if (32 * wave >= b.rows || parts > 1) {
     return;
   }
   float const by = 1.0f / sum;
