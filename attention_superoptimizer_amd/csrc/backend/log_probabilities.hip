@@ -6,13 +6,14 @@
 //
 // The top tokens are found on the way: a wavefront keeps a bound that it knows `top` of its logits to reach, and only logits above
 // it are looked at one by one.  The bound is what the top-th of the lanes' own maxima reaches, which the sums need anyway; after the first few
-// thousand logits hardly any passes it.  What passed is told apart by counting: an entry's place is the number of better ones.
+// thousand logits hardly any passes it.  (It is asked for again in nearly every chunk all the same, with more than one top token: the greatest of the lanes' maxima
+// of all chunks so far lies above the top-th.)  What passed is told apart by counting: an entry's place is the number of better ones.
 //
 // Few rows are cut over workgroups, of which the last to come (a ticket) puts the parts together, always in the same order.
 //
-// Measured: 83 us of 4096 rows of 50021 fp16 with the top token (410 MB, 4.9 TB/s, and 71 us of vector instructions: a read of so much takes 66),
-// 143 of fp32 (820 MB, 5.7 TB/s), 11.7 of 64 rows of 131072 bf16 with twenty (17 MB; trips to memory one after the other and the bounds),
-// 7.5 of one row of 32000 fp32 with five, of which a launch is 3.
+// Measured: 83 - 86 us of 4096 rows of 50021 fp16 with the top token (410 MB, 4.9 TB/s, and 71 us of vector instructions: a read of so much takes 66),
+// 102 with five, 107 with twenty and 124 with fifty, which the bounds take; 143 of fp32 (820 MB, 5.7 TB/s), 11.9 - 13 of 64 rows of 131072 bf16 with
+// twenty (17 MB; trips to memory one after the other and the bounds), 22.6 of 200 of these, 7.5 of one row of 32000 fp32 with five, of which a launch is 3.
 #include "common.h"
 #include "mi355_kernels/kernarg.h"
 #include "slices.h"
@@ -557,7 +558,7 @@ template <class T>
 int launch_log(LogParams P, int rows) {
   constexpr int kChunk = 64 * kRounds * (16 / (int)sizeof(T));
   // As many workgroups to a row as leave two to a compute unit, each with a chunk for every wavefront at least.  Measured (us, one, two and four to a
-  // compute unit; 131072 bf16 a row, 20 top tokens): 13.6, 12.6 and 13.6 of 64 rows, 26.1, 24.4 and 24.7 of 200; alike for few rows.
+  // compute unit; 131072 bf16 a row, 20 top tokens): 13.4, 11.9 and 12.9 of 64 rows, 24.1, 22.7 and 23.9 of 200; alike for few rows.
   constexpr int kFill = 512;
   int const most = (P.vocabulary - 1) / (kWaves * kChunk) + 1, wanted = rows < kFill ? (kFill - 1) / rows + 1 : 1;
   P.row_parts = wanted < most ? wanted : most;

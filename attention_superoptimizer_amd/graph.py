@@ -334,7 +334,9 @@ class KNGraph:
         nodes: the node that node i follows, one before it; -1: it follows the sequence itself.  lengths count the nodes, whose
         keys are in the caches already, node i's at place length - nodes + i.  A node with any other parent, or a place below
         zero, is not there, nor is what follows it: its row is zeros and no row sees its key (mark what fewer drafts leave by
-        -2).  Everything else as in `paged_attention`."""
+        -2).  Everything else as in `paged_attention`, but for the weights where nodes times the query heads of a key-value head are
+        more than 16: each is rounded once to the values' type, so that a result may be off by as much again as by its own
+        rounding."""
         if scale is None:
             scale = float(k_cache.dims[-1]) ** -0.5
         return self._wrap(self._rt.mirage_graph_tree_attention(self._g, q._h, k_cache._h, v_cache._h, table._h, lengths._h, parents._h,
@@ -349,7 +351,8 @@ class KNGraph:
         head_dim] or [tokens, q_heads * head_dim]; without `starts` every sequence has tokens / sequences of them in a row; with
         starts [sequences + 1] int32, ascending from 0, sequence b has the rows starts[b] to starts[b + 1] - 1, none or any
         number, and rows of the result from starts[sequences] on are left as they were.  Everything else as in
-        `paged_attention`."""
+        `paged_attention`, but for the weights, which are rounded to the values' type as in `tree_attention`: with starts always, a
+        single token's too."""
         if scale is None:
             scale = float(k_cache.dims[-1]) ** -0.5
         window, sinks = (max(-1, min(int(n), 2 ** 31 - 1)) for n in (window, sinks))  # (ctypes would take their lowest 32 bits)

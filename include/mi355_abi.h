@@ -488,8 +488,12 @@ int mi355_verify_drafts(void const *target, void const *draft, int const *tokens
 /* mi355_paged_attention for a tree of `nodes` new tokens of each sequence: the row of node i sees the keys before
  * lengths[sequence] - nodes, its own (at that place + i) and those of its ancestors.  parents[sequence][i] is the node that
  * node i follows, below i; -1: the sequence itself.  A node with any other parent, or whose place is below zero, is not
- * there, nor is what follows it: its row is zeros, its key seen by none.  Up to MI355_MAX_TREE_NODES nodes; types, strides,
- * alignment, and what is out of range or infinite, as there. */
+ * there, nor is what follows it: its row is zeros, its key seen by none.  Up to MI355_MAX_TREE_NODES nodes (a row climbs to its ancestors
+ * one by one, in every 64 keys of the tree: 1024 nodes in a chain take 920 us where 1024 that follow the sequence itself take 63, 128 of them 55 and 22;
+ * 8 x 4 heads of 128 behind 1000 keys); types, strides, alignment, and what is out of range or infinite, as there.
+ * Weights: up to 16 rows (nodes times the query heads of a key-value head) have them to 2^-16, as there.  With more, each is rounded once to the values'
+ * type, and the sum of weights is that of the rounded ones: a result may be off by as much again as by its own rounding.  sequences * nodes times
+ * the query heads of a key-value head is up to 2^30. */
 #define MI355_MAX_TREE_NODES 1024
 int mi355_tree_attention(void const *q, long long q_stride, void *out, long long out_stride, mi355_paged_cache const *cache,
                          int const *table, int table_width, int const *lengths, int const *parents, int sequences, int nodes,
@@ -498,7 +502,9 @@ int mi355_tree_attention(void const *q, long long q_stride, void *out, long long
  * lengths[sequence] - (new - 1 - t) with j >= L - window (any, where window is 0) or j < sinks.  `tokens` rows of q and out;
  * starts null: tokens / sequences of them, a whole number, for each sequence; else starts[sequence] .. starts[sequence + 1] - 1,
  * ascending from 0 to at most tokens, none or any number (out of order, rows may be left as they were); rows of out from
- * starts[sequences] on are left as they were.  Types, strides, alignment, and what is out of range or infinite, as there. */
+ * starts[sequences] on are left as they were.  Types, strides, alignment, and what is out of range or infinite, as there.  Weights as in
+ * mi355_tree_attention, new tokens in the place of nodes; with starts they are rounded to the values' type whatever the rows, a single token's too.  `tokens` times
+ * the query heads of a key-value head is up to 2^30; with starts, a 128th of that and sequences, times the key-value heads, are below 2^24. */
 int mi355_window_attention(void const *q, long long q_stride, void *out, long long out_stride, mi355_paged_cache const *cache,
                            int const *table, int table_width, int const *lengths, int const *starts, int sequences, int tokens,
                            int q_heads, float scale, int window, int sinks);

@@ -86,7 +86,8 @@ public:
 // that node i follows, one before it; -1: it follows the sequence itself.  The keys of node i are at place
 // length - nodes + i.  A node with any other parent, or a place below zero, is not there, nor is what follows it: its row is
 // zeros and no row sees its key (so fewer drafts are padded).  Values, scores and page numbers that are out of order: as in
-// paged attention.
+// paged attention.  Where nodes times the query heads of a key-value head are more than 16, weights are rounded once to the values' type
+// (in paged attention to 2^-16), and the sum of weights is that of the rounded ones: as much error again as the result's own rounding.
 class KNTreeAttentionOp : public KNDecodingOp {
 public:
   KNTreeAttentionOp(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table, DTensor const &lengths,
@@ -99,7 +100,8 @@ public:
 // Attention within a window, and to the first tokens of the sequence: as paged attention, but new token t sees the keys j <
 // L = length - (new - 1 - t) with j >= L - window (all, where window is 0) or j < sinks.  One new token of every sequence, whole
 // prompts, or anything between; with starts [sequences + 1], ascending from 0, sequence b's new tokens are the rows starts[b] to
-// starts[b + 1] - 1 of q, and rows from the last of them on are left as they were; without, every sequence has as many.
+// starts[b + 1] - 1 of q, and rows from the last of them on are left as they were; without, every sequence has as many.  Weights are
+// rounded as in attention of trees, with starts whatever the rows.
 class KNWindowAttentionOp : public KNDecodingOp {
 public:
   KNWindowAttentionOp(DTensor const &q, DTensor const &k_cache, DTensor const &v_cache, DTensor const &table, DTensor const &lengths,
