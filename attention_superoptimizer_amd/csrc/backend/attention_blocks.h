@@ -779,6 +779,13 @@ __global__ __launch_bounds__(kThreads) void join_blocks_kernel(BlockParams const
         y[i][four] = *reinterpret_cast<paged::floatx4 const *>(part + 4 * (((d * kWaves + rows) * 4 + four) * 64 + lane));
       }
     }
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) {  // (whether they count or not: what is asked for later is a trip of its own)
+#pragma unroll
+      for (int four = 0; four < 4; four++) {
+        asm volatile("" : "+v"(y[i][four]));
+      }
+    }
     float const before = top;
 #pragma unroll
     for (int i = 0; i < kBatch; i++) {
