@@ -10,13 +10,13 @@
 // * Keys are counted as the block sees them: the first `kept` of the sequence, then those from `first` on, in one run without a gap;
 //   where up to 2048 of the run lie is looked up at once and kept in LDS.
 // * Weights are rounded to the values' type once, and added up as rounded: an error of as much again as rounding the result makes, at
-//   two thirds of the matrix products that weights in two words would take.
+//   two thirds of the matrix products that weights in two words would take.  (The ABI says so.)
 // * Blocks that leave compute units without work are cut along their keys (of trees so that all parts are alike), and joined by a second
 //   kernel in the order of the keys, so that results do not depend on who comes first.
 //
-// Measured (8 key-value heads of 4 query heads of 128, bf16): 555 to 600 us of one prompt of 8192 tokens (550 GFLOP, 990 TFLOP/s), 158 to 171 within a
-// window of 1024 (129 GFLOP, 750 to 820 TFLOP/s); a large matrix product reaches 1270.  What bounds it are the two wavefronts of a SIMD taking
-// turns: matrix instructions fill 39 % of its cycles and vector instructions, exponentials nearly half of them, 49 %.
+// Measured (8 key-value heads of 4 query heads of 128, bf16): 555 to 597 us of one prompt of 8192 tokens (550 GFLOP, 920 to 990 TFLOP/s), 164 to 177 within a
+// window of 1024 (129 GFLOP, 730 to 790 TFLOP/s); a large matrix product reaches 1270.  What bounds it are the two wavefronts of a SIMD taking
+// turns: matrix instructions fill 37 % of its cycles and vector instructions, exponentials nearly half of them, 48 %.
 #pragma once
 
 #include "mi355_kernels/attention_blocks_units.h"
