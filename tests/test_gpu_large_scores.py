@@ -28,14 +28,12 @@ def _paged(q, k, v, table, n, kind, scale):
         g.close()
 
 
-@pytest.mark.parametrize("kind", ["fp16", "bf16"])
-@pytest.mark.parametrize("size", [100.0, 999.0, 5001.0, 20011.0, 60013.0, -60013.0, 3e9, 3e17])
+@pytest.mark.parametrize("kind,size", [(kind, size) for size in (100.0, 999.0, 5001.0, 20011.0, 60013.0, -60013.0) for kind in ("fp16", "bf16")] +
+                         [("bf16", 3e9), ("bf16", 3e17)])
 @pytest.mark.parametrize("head", [64, 80, 192])
 @pytest.mark.parametrize("form,new,length", [("window", 1, 1), ("window", 4, 4), ("window", 40, 500), ("ragged", 1, 77), ("ragged", 600, 700), ("tree", 3, 3),
                                              ("tree", 40, 3000), ("paged", 1, 1), ("paged", 1, 3000), ("paged", 12, 300), ("paged", 40, 300)])
 def test_equal_keys(rt, form, new, length, head, kind, size):
-    if kind == "fp16" and abs(size) > 65504:
-        pytest.skip("fp16 has no such values")
     k, v, table, values = caches(length, [length], 1, head, 16, kind)
     k[np.isfinite(k)] = size
     size = float(np.float32(size))
