@@ -1,4 +1,4 @@
-"""A scale of zero beside values that are not finite, of which rows are done again: weights are equal however large queries and keys are."""
+"""A scale of zero beside values that are not finite: weights are equal however large queries and keys are."""
 import numpy as np
 import pytest
 
